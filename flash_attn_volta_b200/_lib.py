@@ -25,6 +25,7 @@ BWD_DETERMINISTIC = 1
 
 STATUS_TIMEOUT = 1
 STATUS_RANGE = 2
+STATUS_PAGE = 4
 
 DTYPE_F16 = 0
 DTYPE_BF16 = 1
@@ -80,6 +81,22 @@ def load() -> ctypes.CDLL:
             lib.fa_sm100_bwd_noalloc.restype = _c_int
             lib.fa_sm100_bwd_workspace_bytes.argtypes = [_c_int, _c_int, _c_int, _c_int]
             lib.fa_sm100_bwd_workspace_bytes.restype = _c_size
+            _c_ll = ctypes.c_longlong
+            lib.fa_sm100_rotary.argtypes = [_vp, _vp, _vp, _c_int, _c_int, _c_float, _c_int, _vp,
+                                            _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_int,
+                                            _vp]
+            lib.fa_sm100_rotary.restype = _c_int
+            lib.fa_sm100_kv_append.argtypes = [_vp] * 5 + [_c_int] + [_vp] * 3 + [
+                _c_int, _c_int, _c_float, _c_int, _c_int, _vp, _vp]
+            lib.fa_sm100_kv_append.restype = _c_int
+            lib.fa_sm100_kv_read.argtypes = [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp,
+                                             _vp]
+            lib.fa_sm100_kv_read.restype = _c_int
+            lib.fa_sm100_decode_workspace_bytes.argtypes = [_vp] + [_c_int] * 4
+            lib.fa_sm100_decode_workspace_bytes.restype = _c_size
+            lib.fa_sm100_decode.argtypes = [_vp] * 5 + [_c_int] + [_vp] * 3 + [_c_size] + [
+                _c_int] * 3 + [_c_float, _c_int, _vp, _vp]
+            lib.fa_sm100_decode.restype = _c_int
             lib.fa_sm100_set_wait_timeout_ns.argtypes = [ctypes.c_uint64]
             lib.fa_sm100_set_wait_timeout_ns.restype = None
             lib.fa_sm100_set_debug_flags.argtypes = [_c_int]
@@ -101,7 +118,8 @@ def check(rc: int, what: str) -> None:
 # ----------------------------------------------------------------- status word
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device int32 the kernels OR error bits into (bit 0: an on-device wait
-    timed out; bit 1: a backward row term was clamped).  One word per device,
+    timed out; bit 1: a backward row term was clamped; bit 2: a page id or a length
+    outside the key/value cache).  One word per device,
     shared with the torch.ops.fav operators."""
     from . import ops
     idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -123,6 +141,19 @@ def _raw_stream_fallback(idx: int) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _raw_stream_fallback
+
+
+class Heads(ctypes.Structure):
+    """fa_sm100_heads of include/fa_sm100.h."""
+    _fields_ = [("inp", _vp), ("out", _vp), ("stride_batch", ctypes.c_longlong),
+                ("stride_seq", ctypes.c_longlong), ("stride_head", ctypes.c_longlong),
+                ("heads", _c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """fa_sm100_kv_cache of include/fa_sm100.h."""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("num_pages", _c_int), ("page_size", _c_int),
+                ("nheads_kv", _c_int), ("head_dim", _c_int), ("dtype", _c_int), ("bits", _c_int)]
 
 
 class on_device:
@@ -158,7 +189,8 @@ def check_status(device: torch.device | None = None) -> None:
             raise RuntimeError(f"flash_attn_volta_b200 kernel reported status {v} on {d} "
                                "(bit 0: an on-device wait timed out; bit 1: a backward row "
                                "term, LSE/sm_scale or rowsum(O*dO), was beyond the range the "
-                               "kernel represents and was clamped)")
+                               "kernel represents and was clamped; bit 2: a page id or a length "
+                               "was outside the key/value cache)")
 
 
 _debug_sync = os.environ.get("FA_B200_SYNC_CHECK", "0") == "1"

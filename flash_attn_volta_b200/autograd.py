@@ -12,6 +12,7 @@ import torch
 
 from .backward import flash_attn_backward
 from .forward import flash_attn_forward
+from .rotary import Rotary, rotate_for_attention
 
 
 class _FlashAttnFn(torch.autograd.Function):
@@ -42,7 +43,8 @@ class _FlashAttnFn(torch.autograd.Function):
 
 def flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                causal: bool = False, sm_scale: float | None = None, *,
-               deterministic: bool | None = None) -> torch.Tensor:
+               deterministic: bool | None = None, rotary: Rotary | None = None,
+               positions: torch.Tensor | None = None) -> torch.Tensor:
     """Attention with gradients: the B200 forward, and the B200 backward when
     autograd reaches it.
 
@@ -51,6 +53,12 @@ def flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     to keys at or before its own position.  ``sm_scale`` multiplies the scores
     before the softmax and defaults to head_dim ** -0.5.  The result has q's
     shape and dtype.  ``deterministic`` selects the backward's dQ mode (see
-    flash_attn_backward).
+    flash_attn_backward).  With ``rotary`` (a flash_attn_volta_b200.rotary.Rotary)
+    q and k are rotated first, with gradients: keys at ``positions`` ((N_k,) or
+    (batch, N_k), default 0 ..), queries at the last N of them.
     """
+    if rotary is not None:
+        q, k = rotate_for_attention(q, k, rotary, positions)
+    else:
+        assert positions is None, "positions are used with rotary only"
     return _FlashAttnFn.apply(q, k, v, causal, sm_scale, deterministic)

@@ -128,6 +128,31 @@ WsLayout ws_layout(int B, int S, int H, int D, bool sep) {
 }
 
 }  // namespace
+
+int bind_device() { return check_device(); }
+
+unsigned long long wait_timeout_ns() { return g_timeout_ns.load(); }
+
+int make_rows_map(CUtensorMap* m, const void* ptr, long long rows, int D, int box_rows, int dtype) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return FA_ERR_DEVICE;
+  const int swb = D * 2 >= 128 ? 128 : D * 2;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+  const cuuint32_t box[2] = {(cuuint32_t)(swb / 2), (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapSwizzle swz = swb == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                 : swb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                             : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUtensorMapDataType ty =
+      dtype == FA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return enc(m, ty, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? FA_OK
+             : FA_ERR_TMA;
+}
+
 }  // namespace fa_sm100
 
 using namespace fa_sm100;

@@ -1,0 +1,926 @@
+// Attention of a few query tokens per sequence over the paged key/value cache
+// (fa_kv_cache.cuh): o_i = sum_j softmax_j(scale q_i . k_j) v_j over the cached
+// tokens j below row i's limit.
+//
+// Bound by HBM: the cache is read once, 4 rows D flops a token and K/V head
+// (rows: the query heads that share it times the query tokens), so at 8 rows
+// 16 flops a 16-bit byte.  That needs no 128-row tensor-core tiles; what it
+// needs is loads in flight and few instructions per cached byte:
+//
+// * Work split.  The tiles (4 warps x U blocks of 16 tokens) of all (sequence,
+//   K/V head, row block) segments form one list, cut into equal contiguous
+//   shares, one per CTA, whatever the lengths are.  The lengths stay on the
+//   device: each CTA sums them itself.  A segment inside one share is finished
+//   there; one that crosses shares leaves fp32 partial results (maximum, sum,
+//   O) that fa_decode_merge_kernel joins in a fixed order.
+// * Each warp streams its own blocks through a private ring of bulk copies (TMA
+//   tiles for 16-bit pages, plain bulk copies for 4-bit blocks) with its own
+//   mbarriers, running maximum, sum and O, across segment borders; the warps
+//   meet only at the end of a segment.
+// * The products run transposed, S^T = K Q^T and O^T += V^T P^T (mma.sync
+//   m16n8k16): 16 tokens, or dims, are the rows and 8 query rows the columns, so
+//   nothing is wasted at 8 rows; the running maximum of a query row is per
+//   lane column in S^T and in O^T alike, and P^T becomes the second product's
+//   operand by one 8x8 transpose (movmatrix) each.
+// * 4-bit codes are used as they are: a nibble masked out of its word is the
+//   fp16 subnormal c 2^-24 (bits 0..3) or c 2^-20 (bits 4..7), exact in the
+//   matrix instruction, so 8 codes cost one shift and four ANDs.  The power of
+//   two goes into q (K) or the final factor (V).  Scales and minima enter
+//   outside: S = sum_g s_g (c_g . q_g) + m_g sum(q_g), with the second sum as
+//   one more matrix instruction on the parameter words themselves (q's group
+//   sums as an fp16 head and tail), and O = sum_t (p_t s_t) c_t + p_t m_t.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <type_traits>
+
+#include "fa_kernels.h"
+#include "fa_kv_cache.cuh"
+#include "sm100_ptx.cuh"
+
+namespace fa_sm100 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kCtasPerSm = 2;
+constexpr float kLn2 = 0.69314718055994531f;
+
+// Per-instantiation constants.
+template <int D, int BITS>
+struct Cfg {
+  static constexpr int kU = (BITS == 16 && D == 128) ? 1 : 2;  // blocks of a warp per tile
+  static constexpr int kBlockBytes = BITS == 16 ? 64 * D : 20 * D;
+  static constexpr int kStageBytes = kU * kBlockBytes;
+  static constexpr int kStages = BITS == 16 ? (D == 128 ? 3 : 3) : (D == 128 ? 4 : 6);
+  static constexpr int kTile = kWarps * kU * kBlockTokens;  // tokens
+  static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kJoinStride = D + 4;  // floats of a row in the join buffer
+  static constexpr int kJoinBytes = kWarps * 8 * kJoinStride * 4;
+  static constexpr int kMiscBytes = 512;         // barriers and small shared variables
+  // two CTAs per SM: 2 x (kSmem + 1 KB) <= 228 KB
+  static constexpr int kSmem = kRingBytes + kJoinBytes + kMiscBytes;
+  static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
+  static constexpr int kGroups = D / 32;
+};
+
+struct DecodeParams {
+  KvView kv;
+  const void* q;       // (B, Sq, H, D)
+  void* out;           // (B, Sq, H, D)
+  float* lse;          // (B, H, Sq) or null
+  const int* lengths;  // (B)
+  const int* starts;   // (B) or null: length - Sq
+  float* part_o;       // (2 * grid, ROWS, D)
+  float2* part_ml;     // (2 * grid, ROWS): maximum (log2 domain), sum
+  int B, Sq, H, group, row_blocks, causal;
+  int grid;
+  float scale_log2;
+  unsigned long long timeout_ns;
+};
+
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(a));
+  } else if constexpr (N == 2) {
+    const uint2 v = lds64(a);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = lds32(a);
+  }
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(T) == 2 && Elem<T>::kIdescAB == 0) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float low_half(uint32_t w) {
+  return __half2float(__ushort_as_half((uint16_t)w));
+}
+
+// Position in the tile list.
+struct Cursor {
+  int b, hr, tt, nt, len;  // sequence, K/V head * row_blocks + row block, tile of nt, length
+};
+
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int len) {
+  const int n = (len + TILE - 1) / TILE;
+  return n < 1 ? 1 : n;  // a sequence without tokens has one tile, which writes its zeros
+}
+
+// Sums the tile counts of all sequences (`total`) and, for one position `want`
+// of the list, finds the sequence that holds it and the tiles before that
+// sequence.  All threads of the CTA take part.
+template <int TILE>
+__device__ __forceinline__ void locate(const DecodeParams& p, int per_tile, long long (&box)[3],
+                                       long long* warp_sum, long long want_num, long long want_den,
+                                       int want_b) {
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int chunk = (p.B + kThreads - 1) / kThreads;
+  const int b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += (long long)tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) * per_tile;
+  long long before = mine;  // inclusive scan
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long o = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += o;
+  }
+  if (lane == 31) warp_sum[w] = before;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < w) before += warp_sum[i];
+    total += warp_sum[i];
+  }
+  before -= mine;
+  // want_b >= 0: the tiles before that sequence; else the position total * num / den
+  const long long want = want_b >= 0 ? 0 : total * want_num / want_den;
+  if (tid == 0) box[0] = total;
+  long long at = before;
+  for (int b = b0; b < b1; ++b) {
+    const long long n = (long long)tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) * per_tile;
+    if (want_b >= 0 ? b == want_b : (want >= at && want < at + n)) {
+      box[1] = b;
+      box[2] = at;
+    }
+    at += n;
+  }
+  __syncthreads();
+}
+
+template <typename T, int D, int BITS, int NT>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    fa_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v) {
+  using C = Cfg<D, BITS>;
+  using M = typename std::conditional<BITS == 4, __half, T>::type;  // operand type
+  constexpr int U = C::kU, NS = C::kStages, ROWS = 8 * NT, NG = BITS == 4 ? C::kGroups : 1;
+  constexpr int KSTEPS = D / 16;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  struct Misc {
+    uint64_t bars[kWarps * NS];
+    long long box[3], warp_sum[kWarps];
+    float2 join_ml[kWarps][8];
+    int abort_flag;
+  };
+  static_assert(sizeof(Misc) <= C::kMiscBytes, "small shared variables");
+  float* join = reinterpret_cast<float*>(smem_raw + C::kRingBytes);
+  Misc& sh = *reinterpret_cast<Misc*>(smem_raw + C::kRingBytes + C::kJoinBytes);
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t my_ring = smem_u32(smem_raw) + warp * NS * C::kStageBytes;
+  const uint32_t my_bars = smem_u32(sh.bars + warp * NS);
+
+  if (tid == 0) sh.abort_flag = 0;
+  if (lane < NS) mbar_init(my_bars + lane * 8, U);
+  fence_barrier_init();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int segs = p.kv.heads * p.row_blocks;  // segments of a sequence
+  locate<C::kTile>(p, segs, sh.box, sh.warp_sum, blockIdx.x, p.grid, -1);  // ends with __syncthreads
+  const long long total = sh.box[0];
+  const long long begin = total * blockIdx.x / p.grid, end = total * (blockIdx.x + 1) / p.grid;
+  if (begin >= end) return;
+  const WaitCtx wait{&sh.abort_flag, p.kv.status, p.timeout_ns};
+
+  Cursor cur;
+  {
+    cur.b = (int)sh.box[1];
+    const int given = p.lengths[cur.b];
+    cur.len = p.kv.clamp_length(given);
+    cur.nt = tiles_of<C::kTile>(cur.len);
+    const long long in = begin - sh.box[2];
+    cur.hr = (int)(in / cur.nt);
+    cur.tt = (int)(in % cur.nt);
+  }
+  auto advance = [&](Cursor& c) {
+    if (++c.tt < c.nt) return;
+    c.tt = 0;
+    if (++c.hr < segs) return;
+    c.hr = 0;
+    if (++c.b >= p.B) return;
+    c.len = p.kv.clamp_length(p.lengths[c.b]);
+    c.nt = tiles_of<C::kTile>(c.len);
+  };
+
+  // ---- producer: lane u < U brings block u of the warp's share of a tile
+  Cursor pc = cur;
+  long long to_issue = end - begin;
+  int next_id = -1;
+  uint32_t ok_bits = 0;  // this lane's block of each stage holds tokens
+  uint32_t in_flight = 0;  // stages whose copies have not been waited for
+  auto block_token = [&](const Cursor& c, int u) {
+    return c.tt * C::kTile + (warp * U + u) * kBlockTokens;
+  };
+  auto look_up = [&]() {  // page of the next block to issue: read ahead of its use
+    next_id = -2;
+    if (lane < U && to_issue > 0) {
+      const int tok = block_token(pc, lane);
+      if (tok < pc.len) next_id = p.kv.table[(long long)pc.b * p.kv.table_width + tok / p.kv.page];
+    }
+  };
+  auto issue = [&](int stage) {
+    if (to_issue <= 0) return;
+    if (lane < U) {
+      const uint32_t bar = my_bars + stage * 8;
+      const bool ok = next_id != -2 && !p.kv.bad_page(next_id);
+      if (next_id != -2 && !ok) p.kv.report(kStatusPage);
+      ok_bits = ok ? ok_bits | (1u << stage) : ok_bits & ~(1u << stage);
+      if (ok) {
+        const int tok = block_token(pc, lane) & (p.kv.page - 1), h = pc.hr / p.row_blocks;
+        const uint32_t dst = my_ring + stage * C::kStageBytes + lane * C::kBlockBytes;
+        mbar_arrive_expect_tx(bar, C::kBlockBytes);
+        if constexpr (BITS == 4) {
+          bulk_load(dst, p.kv.k + p.kv.block4(next_id, h, tok), C::kBlockBytes, bar);
+        } else {
+          const int row = (next_id * p.kv.heads + h) * p.kv.page + tok;
+#pragma unroll
+          for (int x = 0; x < D; x += 64) {
+            tma_load_2d(dst + x * 32, &tm_k, bar, x, row);
+            tma_load_2d(dst + 32 * D + x * 32, &tm_v, bar, x, row);
+          }
+        }
+      } else {
+        mbar_arrive(bar);
+      }
+    }
+    in_flight |= 1u << stage;
+    advance(pc);
+    --to_issue;
+    look_up();
+  };
+  look_up();
+#pragma unroll 1
+  for (int s = 0; s < NS; ++s) issue(s);
+
+  // ---- consumer state
+  uint32_t qf[NT][KSTEPS][2];   // q as the second operand of S^T
+  uint32_t qsum[NT][2];         // 4-bit: (0, head), (0, tail) of group t's sum
+  float f[NT][2];               // factor of a score to the log2 domain, per column
+  int lim[NT][2];               // tokens that a column's query row sees
+  int col_q[NT][2];             // query token of a column's row; -1: none
+  float o[KSTEPS][NT][4], om[NT][4], m[NT][2], l[NT][2];
+  int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
+
+  auto limit_of = [&](int qpos) {
+    if (!p.causal) return cur.len;
+    const long long n = (long long)start + qpos + 1;
+    return n < 0 ? 0 : n < cur.len ? (int)n : cur.len;
+  };
+
+  auto begin_segment = [&]() {
+    const int h = cur.hr / p.row_blocks, rb = cur.hr % p.row_blocks;
+    const int rows = p.Sq * p.group;
+    start = p.starts ? p.starts[cur.b] : cur.len - p.Sq;
+    qp_first = rb * ROWS / p.group;
+    qp_last = (min(rows, (rb + 1) * ROWS) - 1) / p.group;
+    min_lim = limit_of(qp_first);
+    max_lim = limit_of(qp_last);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = rb * ROWS + n * 8 + 2 * t + i;
+        lim[n][i] = rr < rows ? limit_of(rr / p.group) : 0;
+        col_q[n][i] = rr < rows ? rr / p.group : -1;
+        m[n][i] = -INFINITY;
+        l[n][i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) om[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+
+      const int rr = rb * ROWS + n * 8 + g;
+      const bool there = rr < rows;
+      const int qpos = there ? rr / p.group : 0, hq = h * p.group + (there ? rr % p.group : 0);
+      const T* src = static_cast<const T*>(p.q) + (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D;
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) {
+          qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * t) : 0u;
+          qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 + 2 * t) : 0u;
+        }
+        f[n][0] = f[n][1] = p.scale_log2;
+      } else {
+        // q scaled by a power of two, largest element in [2^10, 2^11), as fp16;
+        // its elements are exact down to 2^-24 of the largest
+        uint4 raw[NG];
+        float top = 0.f;
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          raw[grp] = there ? *reinterpret_cast<const uint4*>(src + 32 * grp + 8 * t)
+                           : make_uint4(0, 0, 0, 0);
+          const uint32_t ws[4] = {raw[grp].x, raw[grp].y, raw[grp].z, raw[grp].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = Elem<T>::unpack2(ws[i]);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
+        e = max(-90, min(e, 110));
+        const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+        const float down = __uint_as_float((uint32_t)(127 + 10 + e) << 23) * p.scale_log2;  // 2^20 / up
+        float mine = 0.f;  // sum of group t
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          const uint32_t ws[4] = {raw[grp].x, raw[grp].y, raw[grp].z, raw[grp].w};
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = Elem<T>::unpack2(ws[i]);
+            const uint32_t h2 = Elem<__half>::pack2(v.x * up, v.y * up);
+            const float2 r = Elem<__half>::unpack2(h2);
+            sum += r.x + r.y;
+            // codes of the first two dims of four stand 4 bits lower: their q is 2^4 larger
+            qf[n][2 * grp + i / 2][i % 2] = i % 2 ? h2 : Elem<__half>::pack2(r.x * 16.f, r.y * 16.f);
+          }
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          if (t == grp) mine = sum * 0.015625f;  // 2^-6: below 2^11
+        }
+        const __half head = __float2half_rn(mine);
+        const __half tail = __float2half_rn(mine - __half2float(head));
+        qsum[n][0] = (uint32_t)__half_as_ushort(head) << 16;
+        qsum[n][1] = (uint32_t)__half_as_ushort(tail) << 16;
+        f[n][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        f[n][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+      }
+    }
+  };
+
+  auto step = [&](int stage) {
+    const uint32_t base = my_ring + stage * C::kStageBytes;
+    float s[U][NT][4];
+    bool ok[U];
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
+    // ---- S^T = K Q^T
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int tok0 = block_token(cur, u);
+      ok[u] = ((__shfl_sync(0xffffffffu, ok_bits, u) >> stage) & 1u) && tok0 < max_lim;
+      if (!ok[u]) continue;
+      const uint32_t blk = base + u * C::kBlockBytes;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k) {
+          uint32_t a[4];
+          constexpr int WB = D * 2 >= 128 ? 128 : D * 2;  // bytes of a swizzled row
+          const int r = (lane & 7) + (lane & 8);
+          const int ch = 2 * k + (lane >> 4);  // 16-byte chunk of the row
+          const int sw = WB == 128 ? (r & 7) : WB == 64 ? (r >> 1 & 3) : (r >> 2 & 1);
+          ldsm4(blk + (ch / (WB / 16)) * (16 * WB) + r * WB + ((ch % (WB / 16)) ^ sw) * 16, a);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            mma16816<M>(s[u][n], a[0], a[1], a[2], a[3], qf[n][k][0], qf[n][k][1]);
+        }
+      } else {
+        const Kv4 lay(D);
+        uint32_t w0[NG], w1[NG], q0[NG], q1[NG];  // codes and parameters of tokens g, g + 8
+        lds_words<NG>(blk + (g * 4 + t) * NG * 4, w0);
+        lds_words<NG>(blk + ((g + 8) * 4 + t) * NG * 4, w1);
+        lds_words<NG>(blk + lay.k_params() + g * NG * 4, q0);
+        lds_words<NG>(blk + lay.k_params() + (g + 8) * NG * 4, q1);
+        uint32_t p0 = 0, p1 = 0;  // parameters of group t
+        if (t < NG) {
+          p0 = lds32(blk + lay.k_params() + (g * NG + t) * 4);
+          p1 = lds32(blk + lay.k_params() + ((g + 8) * NG + t) * 4);
+        }
+        float c[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+          mma16816<M>(c[n], p0, p1, p0, p1, qsum[n][0], qsum[n][1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][n][i] = c[n][i] * 0x1p-14f;
+        }
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
+          const float s0 = low_half(q0[grp]), s1 = low_half(q1[grp]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+            mma16816<M>(c[n], w0[grp] & 0x000F000Fu, w1[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
+                        w1[grp] & 0x00F000F0u, qf[n][2 * grp][0], qf[n][2 * grp][1]);
+            mma16816<M>(c[n], x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u,
+                        x1 & 0x00F000F0u, qf[n][2 * grp + 1][0], qf[n][2 * grp + 1][1]);
+            s[u][n][0] = fmaf(s0, c[n][0], s[u][n][0]);
+            s[u][n][1] = fmaf(s0, c[n][1], s[u][n][1]);
+            s[u][n][2] = fmaf(s1, c[n][2], s[u][n][2]);
+            s[u][n][3] = fmaf(s1, c[n][3], s[u][n][3]);
+          }
+        }
+      }
+      // ---- log2 domain, mask, maximum
+      const bool partial = tok0 + kBlockTokens > min_lim;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[u][n][i] *= f[n][i & 1];
+          if (partial && tok0 + g + (i >> 1) * 8 >= lim[n][i & 1]) s[u][n][i] = -INFINITY;
+        }
+        top[n][0] = fmaxf(top[n][0], fmaxf(s[u][n][0], s[u][n][2]));
+        top[n][1] = fmaxf(top[n][1], fmaxf(s[u][n][1], s[u][n][3]));
+      }
+    }
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) any |= ok[u];
+    if (!any) return;
+    // ---- running maximum; O and the sum follow it
+    float base_m[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2)
+          top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], d));
+        const float now = fmaxf(m[n][i], top[n][i]);
+        const float safe = now == -INFINITY ? 0.f : now;  // no token seen yet
+        const float keep = ex2(m[n][i] - safe);
+        m[n][i] = now;
+        base_m[n][i] = safe;
+        if (keep != 1.f) {
+          l[n][i] *= keep;
+          om[n][i] *= keep;
+          om[n][i + 2] *= keep;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            o[k][n][i] *= keep;
+            o[k][n][i + 2] *= keep;
+          }
+        }
+      }
+    // ---- P^T, O^T += V^T P^T
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!ok[u]) continue;
+      const int tok0 = block_token(cur, u);
+      const uint32_t blk = base + u * C::kBlockBytes;
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = ex2(s[u][n][i] - base_m[n][i & 1]);
+        l[n][0] += e[0] + e[2];
+        l[n][1] += e[1] + e[3];
+        pf[n][0] = transpose8x8(Elem<M>::pack2(e[0], e[1]));
+        pf[n][1] = transpose8x8(Elem<M>::pack2(e[2], e[3]));
+      }
+      // Values that a row does not see must not reach its sum even as 0 x NaN,
+      // so in a block that some row sees in part, the values behind the limit
+      // are set to zero, and where the rows' limits differ, each query token's
+      // rows are multiplied apart (`apart`) and the other columns kept.
+      const bool partial = tok0 + kBlockTokens > min_lim;
+      const int passes = partial && p.causal ? qp_last - qp_first + 1 : 1;
+#pragma unroll 1
+      for (int pass = 0; pass < passes; ++pass) {
+        uint32_t keep0 = ~0u, keep1 = ~0u;  // token pairs (2t, 2t + 1), (2t + 8, 2t + 9)
+        const bool apart = passes > 1;
+        bool mine[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) mine[n][i] = col_q[n][i] == qp_first + pass;
+        auto add = [&](float (&acc)[4], int n, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                       uint32_t b0, uint32_t b1) {
+          if (!apart) {
+            mma16816<M>(acc, a0, a1, a2, a3, b0, b1);
+          } else {
+            float c[4] = {acc[0], acc[1], acc[2], acc[3]};
+            mma16816<M>(c, a0, a1, a2, a3, b0, b1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = mine[n][i & 1] ? c[i] : acc[i];
+          }
+        };
+        if (partial) {
+          const int to = limit_of(qp_first + pass) - tok0;
+          if (to <= 0) continue;
+          keep0 = (2 * t < to ? 0xFFFFu : 0u) | (2 * t + 1 < to ? 0xFFFF0000u : 0u);
+          keep1 = (2 * t + 8 < to ? 0xFFFFu : 0u) | (2 * t + 9 < to ? 0xFFFF0000u : 0u);
+        }
+        if constexpr (BITS == 16) {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            uint32_t a[4];
+            constexpr int WB = D * 2 >= 128 ? 128 : D * 2;
+            const int r = (lane & 7) + ((lane >> 4) << 3);
+            const int ch = 2 * k + ((lane >> 3) & 1);
+            const int sw = WB == 128 ? (r & 7) : WB == 64 ? (r >> 1 & 3) : (r >> 2 & 1);
+            ldsm4_trans(blk + 32 * D + (ch / (WB / 16)) * (16 * WB) + r * WB +
+                            ((ch % (WB / 16)) ^ sw) * 16, a);
+            if (partial) {
+              a[0] &= keep0;
+              a[1] &= keep0;
+              a[2] &= keep1;
+              a[3] &= keep1;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              add(o[k][n], n, a[0], a[1], a[2], a[3], pf[n][0], pf[n][1]);
+          }
+        } else {
+          const Kv4 lay(D);
+          uint32_t w0[NG], w1[NG];
+          lds_words<NG>(blk + lay.v_codes() + lane * NG * 4, w0);
+          lds_words<NG>(blk + lay.v_codes() + (32 + lane) * NG * 4, w1);
+          uint2 mm = make_uint2(0, 0);
+          if (g < NG) mm = lds64(blk + lay.v_params() + 32 * NG + (g * 4 + t) * 8);
+          mm.x &= keep0;
+          mm.y &= keep1;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) add(om[n], n, mm.x, 0u, mm.y, 0u, pf[n][0], pf[n][1]);
+#pragma unroll
+          for (int grp = 0; grp < NG; ++grp) {
+            const uint2 sc = lds64(blk + lay.v_params() + (grp * 4 + t) * 8);
+            const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint32_t b0 = hmul2(pf[n][0], sc.x & keep0), b1 = hmul2(pf[n][1], sc.y & keep1);
+              add(o[2 * grp][n], n, w0[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
+                  w1[grp] & 0x000F000Fu, w1[grp] & 0x00F000F0u, b0, b1);
+              add(o[2 * grp + 1][n], n, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
+                  x1 & 0x00F000F0u, b0, b1);
+            }
+          }
+        }
+      }
+    }
+  };
+
+  // The warps' results of a segment, joined; `first`: this share holds the
+  // segment's first tile, `last`: its last.
+  auto end_segment = [&](bool first, bool last) {
+    const int h = cur.hr / p.row_blocks, rb = cur.hr % p.row_blocks, rows = p.Sq * p.group;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
+        if (g == 0) sh.join_ml[warp][2 * t + i] = make_float2(m[n][i], l[n][i]);
+        float* dst = join + (warp * 8 + 2 * t + i) * C::kJoinStride;
+        if constexpr (BITS == 16) {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            dst[16 * k + g] = o[k][n][i];
+            dst[16 * k + 8 + g] = o[k][n][i + 2];
+          }
+        } else {
+#pragma unroll
+          for (int grp = 0; grp < NG; ++grp) {
+            const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t);
+            *reinterpret_cast<float4*>(dst + 32 * grp + 4 * g) =
+                make_float4(fmaf(o[2 * grp][n][i], 0x1p24f, mm), fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
+                            fmaf(o[2 * grp + 1][n][i], 0x1p24f, mm),
+                            fmaf(o[2 * grp + 1][n][i + 2], 0x1p20f, mm));
+          }
+        }
+      }
+      __syncthreads();
+      constexpr int PER_ROW = D / 8;
+      for (int i = tid; i < 8 * PER_ROW; i += kThreads) {
+        const int r = i / PER_ROW, d = i % PER_ROW * 8, rr = rb * ROWS + n * 8 + r;
+        float top = -INFINITY, sum = 0.f, x[8] = {};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.join_ml[w][r].x);
+        const float safe = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 ml = sh.join_ml[w][r];
+          const float e = ex2(ml.x - safe);
+          sum = fmaf(e, ml.y, sum);
+          const float* src = join + (w * 8 + r) * C::kJoinStride + d;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = fmaf(e, src[j], x[j]);
+        }
+        if (rr >= rows) continue;
+        if (first && last) {
+          const int qpos = rr / p.group, hq = h * p.group + rr % p.group;
+          const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = Elem<T>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
+                                    (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D + d) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+          if (p.lse && d == 0)
+            p.lse[((long long)cur.b * p.H + hq) * p.Sq + qpos] =
+                sum == 0.f ? INFINITY : (top + log2f(sum)) * kLn2;
+        } else {
+          const long long slot = (2LL * blockIdx.x + (first ? 1 : 0)) * ROWS + n * 8 + r;
+          float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + d);
+          dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+          dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+          if (d == 0) p.part_ml[slot] = make_float2(top, sum);
+        }
+      }
+      __syncthreads();
+    }
+  };
+
+  // ---- the share, tile by tile
+  int stage = 0;
+  uint32_t phase = 0;
+  bool fresh = true, first = false;
+#pragma unroll 1
+  for (long long left = end - begin; left > 0; --left) {
+    if (fresh) {
+      first = cur.tt == 0;
+      begin_segment();
+      if (first && tid == 0 && cur.hr == 0 && p.kv.bad_length(p.lengths[cur.b])) p.kv.report(kStatusPage);
+    }
+    const bool here = mbar_wait(my_bars + stage * 8, phase, wait);
+    if (here) {
+      in_flight &= ~(1u << stage);
+      step(stage);
+    }
+    __syncwarp();
+    if (here) {
+      issue(stage);
+    } else {
+      to_issue = 0;  // a copy did not arrive: bring no more
+    }
+    const bool last = cur.tt + 1 == cur.nt;
+    if (last || left == 1) end_segment(first, last);
+    fresh = last;
+    advance(cur);
+    if (++stage == NS) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  // After a wait that ran out, copies may still be under way into this CTA's memory.
+  for (int s = 0; s < NS; ++s)
+    if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, s >= stage ? phase : phase ^ 1u, p.timeout_ns);
+}
+
+// Joins the partial results of the segments that cross shares, in the order of
+// the shares.  One CTA per segment; a thread holds 8 dims of a row.
+template <typename T, int D, int BITS, int NT>
+__global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeParams p) {
+  using C = Cfg<D, BITS>;
+  constexpr int ROWS = 8 * NT, PER_ROW = D / 8;
+  __shared__ long long box[3], warp_sum[kWarps];
+  const int segs = p.kv.heads * p.row_blocks;
+  const int b = blockIdx.x / segs, hr = blockIdx.x % segs;
+  const int h = hr / p.row_blocks, rb = hr % p.row_blocks;
+  locate<C::kTile>(p, segs, box, warp_sum, 0, 1, b);
+  const long long total = box[0];
+  const int nt = tiles_of<C::kTile>(p.kv.clamp_length(p.lengths[b]));
+  const long long t0 = box[2] + (long long)hr * nt, t1 = t0 + nt - 1;
+  const int c0 = (int)(((t0 + 1) * p.grid - 1) / total), c1 = (int)(((t1 + 1) * p.grid - 1) / total);
+  griddep_wait();
+  griddep_launch_dependents();
+  if (c0 == c1) return;
+  const int rows = p.Sq * p.group;
+  for (int i = threadIdx.x; i < ROWS * PER_ROW; i += kThreads) {
+    const int r = i / PER_ROW, d = i % PER_ROW * 8, rr = rb * ROWS + r;
+    if (rr >= rows) break;
+    auto slot = [&](int c) { return (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r; };
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c)
+      if (total * (c + 1) / p.grid > total * c / p.grid) top = fmaxf(top, p.part_ml[slot(c)].x);
+    const float safe = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x[8] = {};
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
+      const float2 ml = p.part_ml[slot(c)];
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(c) * D + d);
+      const float4 u = src[0], v = src[1];
+      const float e = ex2(ml.x - safe);
+      sum = fmaf(e, ml.y, sum);
+      x[0] = fmaf(e, u.x, x[0]);
+      x[1] = fmaf(e, u.y, x[1]);
+      x[2] = fmaf(e, u.z, x[2]);
+      x[3] = fmaf(e, u.w, x[3]);
+      x[4] = fmaf(e, v.x, x[4]);
+      x[5] = fmaf(e, v.y, x[5]);
+      x[6] = fmaf(e, v.z, x[6]);
+      x[7] = fmaf(e, v.w, x[7]);
+    }
+    const int qpos = rr / p.group, hq = h * p.group + rr % p.group;
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = Elem<T>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
+                              (((long long)b * p.Sq + qpos) * p.H + hq) * D + d) =
+        make_uint4(w[0], w[1], w[2], w[3]);
+    if (p.lse && d == 0)
+      p.lse[((long long)b * p.H + hq) * p.Sq + qpos] =
+          sum == 0.f ? INFINITY : (top + log2f(sum)) * kLn2;
+  }
+}
+
+template <typename T, int D, int BITS, int NT>
+int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv, bool split,
+                  cudaStream_t st) {
+  using C = Cfg<D, BITS>;
+  auto kernel = fa_decode_kernel<T, D, BITS, NT>;
+  constexpr int kTag = 1000 + ((sizeof(T) == 2 && Elem<T>::kIdescAB == 0) ? 0 : 1) + 2 * NT +
+                       8 * (BITS == 4) + 16 * D;
+  if (!smem_attr_set<kTag>(reinterpret_cast<const void*>(kernel), C::kSmem)) return FA_ERR_LAUNCH;
+  if (launch_pdl(kernel, dim3(p.grid), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
+    return FA_ERR_LAUNCH;
+  if (!split) return FA_OK;
+  const long long segs = (long long)p.B * p.kv.heads * p.row_blocks;
+  return launch_pdl(fa_decode_merge_kernel<T, D, BITS, NT>, dim3((unsigned)segs), dim3(kThreads), 0,
+                    st, p) == cudaSuccess
+             ? FA_OK
+             : FA_ERR_LAUNCH;
+}
+
+template <typename T, int D>
+int launch_decode_d(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
+                    bool split, cudaStream_t st) {
+  if (p.kv.bits == 4) {
+    if constexpr (D >= 32)
+      return nt == 1 ? launch_decode<T, D, 4, 1>(p, tk, tv, split, st)
+                     : launch_decode<T, D, 4, 2>(p, tk, tv, split, st);
+    return FA_ERR_ARG;
+  }
+  return nt == 1 ? launch_decode<T, D, 16, 1>(p, tk, tv, split, st)
+                 : launch_decode<T, D, 16, 2>(p, tk, tv, split, st);
+}
+
+template <typename T>
+int launch_decode_t(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
+                    bool split, cudaStream_t st) {
+  switch (p.kv.D) {
+    case 16: return launch_decode_d<T, 16>(p, nt, tk, tv, split, st);
+    case 32: return launch_decode_d<T, 32>(p, nt, tk, tv, split, st);
+    case 64: return launch_decode_d<T, 64>(p, nt, tk, tv, split, st);
+    default: return launch_decode_d<T, 128>(p, nt, tk, tv, split, st);
+  }
+}
+
+int tile_tokens(int D, int bits) { return (bits == 16 && D == 128) ? 64 : 128; }
+
+struct Plan {
+  int nt, row_blocks, grid;
+  bool split;
+};
+
+// Rows of 8 (one column block of the matrix instructions) or 16; CTAs for two
+// per SM, fewer when the tables have room for fewer tiles.
+Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen, int nheads) {
+  Plan pl;
+  const long long rows = (long long)seqlen * (nheads / c->nheads_kv);
+  pl.nt = rows <= 8 ? 1 : 2;
+  pl.row_blocks = (int)((rows + 8 * pl.nt - 1) / (8 * pl.nt));
+  const int tile = tile_tokens(c->head_dim, c->bits);
+  const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
+  const long long tiles = (long long)batch * c->nheads_kv * pl.row_blocks * per_seg;
+  const long long most = (long long)sm_count() * kCtasPerSm;
+  pl.grid = (int)(tiles < most ? tiles : most);
+  pl.split = per_seg > 1;
+  return pl;
+}
+
+size_t partial_bytes(const Plan& pl, int D) {
+  return pl.split ? (size_t)2 * pl.grid * 8 * pl.nt * (D * sizeof(float) + sizeof(float2)) : 0;
+}
+
+bool decode_shape_ok(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen, int nheads) {
+  return check_kv_cache(c) == FA_OK && table_width >= 1 && batch >= 1 && seqlen >= 1 && nheads >= 1 &&
+         nheads % c->nheads_kv == 0 && (long long)seqlen * nheads <= (1LL << 24) &&
+         (long long)table_width * c->page_size <= 2147483647LL - 65536 &&
+         (long long)batch * seqlen * nheads <= 2147483647LL;
+}
+
+}  // namespace
+}  // namespace fa_sm100
+
+extern "C" size_t fa_sm100_decode_workspace_bytes(const fa_sm100_kv_cache* cache, int table_width,
+                                                  int batch, int seqlen, int nheads) {
+  using namespace fa_sm100;
+  if (!decode_shape_ok(cache, table_width, batch, seqlen, nheads)) return 0;
+  return partial_bytes(plan_of(cache, table_width, batch, seqlen, nheads), cache->head_dim) + 256;
+}
+
+extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, void* out, float* lse,
+                               const int* page_table, int table_width, const int* lengths,
+                               const int* starts, void* workspace, size_t workspace_bytes, int batch,
+                               int seqlen, int nheads, float sm_scale, int causal, int* status,
+                               void* stream) {
+  using namespace fa_sm100;
+  if (!cache || !decode_shape_ok(cache, table_width, batch, seqlen, nheads)) return FA_ERR_ARG;
+  if (!q || !out || !page_table || !lengths) return FA_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) return FA_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(page_table) |
+       reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(starts)) & 3u)
+    return FA_ERR_ARG;
+  int rc = bind_device();
+  if (rc != FA_OK) return rc;
+  const Plan pl = plan_of(cache, table_width, batch, seqlen, nheads);
+  const size_t need = partial_bytes(pl, cache->head_dim);
+  if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return FA_ERR_WORKSPACE;
+  if (pl.grid < 1) return FA_ERR_DEVICE;
+  CUtensorMap tk = {}, tv = {};
+  if (cache->bits == 16) {
+    const long long rows = (long long)cache->num_pages * cache->nheads_kv * cache->page_size;
+    if ((rc = make_rows_map(&tk, cache->k_pages, rows, cache->head_dim, kBlockTokens, cache->dtype)) != FA_OK)
+      return rc;
+    if ((rc = make_rows_map(&tv, cache->v_pages, rows, cache->head_dim, kBlockTokens, cache->dtype)) != FA_OK)
+      return rc;
+  }
+  DecodeParams p = {};
+  p.kv = kv_view(cache, page_table, table_width, status);
+  p.q = q;
+  p.out = out;
+  p.lse = lse;
+  p.lengths = lengths;
+  p.starts = starts;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) +
+                                        (size_t)2 * pl.grid * 8 * pl.nt * cache->head_dim * sizeof(float));
+  p.B = batch;
+  p.Sq = seqlen;
+  p.H = nheads;
+  p.group = nheads / cache->nheads_kv;
+  p.row_blocks = pl.row_blocks;
+  p.causal = causal ? 1 : 0;
+  p.grid = pl.grid;
+  p.scale_log2 = sm_scale * 1.44269504088896341f;
+  p.timeout_ns = wait_timeout_ns();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return cache->dtype == FA_DTYPE_BF16
+             ? launch_decode_t<__nv_bfloat16>(p, pl.nt, tk, tv, pl.split, st)
+             : launch_decode_t<__half>(p, pl.nt, tk, tv, pl.split, st);
+}

@@ -158,6 +158,15 @@ int launch_bwd(const BwdArgs& a, cudaStream_t stream, int phase);
 int launch_bwd_dq(const BwdArgs& a, cudaStream_t stream);
 int bwd_q_rows(int D);
 
+// Makes the current device's primary context current in this thread; FA_OK or
+// FA_ERR_DEVICE when it is not compute capability 10.0.
+int bind_device();
+// Limit of the on-device waits (fa_sm100_set_wait_timeout_ns).
+unsigned long long wait_timeout_ns();
+// Tensor map over `rows` contiguous rows of D 16-bit elements, box_rows rows
+// and min(D, 64) elements to a box, swizzled by the box's row width.
+int make_rows_map(CUtensorMap* m, const void* ptr, long long rows, int D, int box_rows, int dtype);
+
 // Argument checks, tensor maps and launches of the backward on a caller-given
 // workspace (phase as in launch_bwd).  Shared by the C ABI entry points.
 int bwd_impl(int phase, const void* dout, const void* q, const void* k, const void* v,

@@ -1,0 +1,32 @@
+// The angle of a rotary position, shared by the rotation (fa_rotary.cu) and the
+// cache append that rotates on the way (fa_kv_cache.cu).
+#pragma once
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace fa_sm100 {
+
+// (M cos a, M sin a) of a = pos * inv_freq.  The angle of a far position is
+// large (10^5 rad and more), where an fp32 product is off by 10^-2 rad, so the
+// product and its reduction to turns are made in 64 bits: t = a / (2 pi), less
+// the whole turns, leaves 2 t in [-1, 1] half turns, exact to 2^-34 at a
+// million positions.  The sine and cosine of its fp32 head come from
+// sincospif; the tail d (below 2^-24) is added to first order:
+// cos(x + d) = cos x - d sin x.
+__device__ __forceinline__ float2 rotary_cos_sin(double pos, double inv_freq, float magnitude) {
+  const double t = pos * inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
+  const double half = 2.0 * (t - rint(t));
+  const float head = (float)half;
+  const float d = (float)(half - (double)head) * 3.14159265358979f;
+  float s, c;
+  sincospif(head, &s, &c);
+  return make_float2(magnitude * fmaf(-d, s, c), magnitude * fmaf(d, c, s));
+}
+
+// N consecutive 16-bit elements as one load or store.
+template <int N>
+struct alignas(2 * N) Pack16 {
+  uint16_t v[N];
+};
+
+}  // namespace fa_sm100

@@ -30,6 +30,7 @@ enum : int {
   kStatusOk = 0,
   kStatusTimeout = 1,   // a bounded mbarrier wait ran out
   kStatusRange = 2,     // a backward row term (LSE / scale or delta) beyond the representable range
+  kStatusPage = 4,      // a page id or length outside the key/value cache (those tokens are skipped)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -134,6 +135,16 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* m, 
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// 2-D tiled load, as tma_load_4d.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar,
+                                            int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
 

@@ -5,6 +5,8 @@
 //       -> (dq, dk, dv)
 //   torch.ops.fav.status(device) -> the device's int32 status word
 //   torch.ops.fav.merge_(acc_o, acc_lse, o, lse, first)  (ring: in-place LSE merge)
+//   torch.ops.fav.rotary, rotary_qk                      (rotary positions, with gradients)
+//   torch.ops.fav.kv_append, kv_read, decode             (paged key/value cache)
 //
 // These are the only callers of the C core on the Python side
 // (flash_attn_volta_b200/forward.py, backward.py, autograd.py): the
@@ -22,6 +24,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <mutex>
@@ -178,6 +181,357 @@ void merge_cuda(at::Tensor& acc_o, at::Tensor& acc_lse, const at::Tensor& o_in,
   check_rc(rc, "fa_sm100_merge");
 }
 
+// ------------------------------------------------------------ rotary positions
+using OptTensor = std::optional<at::Tensor>;
+
+// (B, S, heads, D) as the C ABI takes it: any strides but a dense last
+// dimension, pairs of elements 4-byte aligned where `pairs`; anything else is
+// copied.
+at::Tensor heads_input(const at::Tensor& t, const char* name, bool pairs) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 4, name, " must be (batch, seqlen, heads, head_dim)");
+  bool fine = t.size(3) <= 1 || t.stride(3) == 1;
+  if (pairs) {
+    fine = fine && reinterpret_cast<uintptr_t>(t.data_ptr()) % 4 == 0;
+    for (int i = 0; i < 3; ++i) fine = fine && (t.size(i) <= 1 || t.stride(i) % 2 == 0);
+  }
+  return fine ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+fa_sm100_heads heads_of(const at::Tensor& t, const at::Tensor* out) {
+  fa_sm100_heads h;
+  h.in = t.data_ptr();
+  h.out = out ? out->data_ptr() : nullptr;
+  // a dimension of one element has no stride worth keeping
+  h.stride_batch = t.size(0) > 1 ? t.stride(0) : 0;
+  h.stride_seq = t.size(1) > 1 ? t.stride(1) : 0;
+  h.stride_head = t.size(2) > 1 ? t.stride(2) : 0;
+  h.heads = (int)t.size(2);
+  return h;
+}
+
+void check_freq(const at::Tensor& inv_freq, const at::Tensor& q) {
+  TORCH_CHECK(inv_freq.scalar_type() == at::kDouble && inv_freq.dim() == 1 && inv_freq.size(0) > 0,
+              "inv_freq must be a 1-D fp64 tensor");
+  TORCH_CHECK(inv_freq.device() == q.device(), "inv_freq is on ", inv_freq.device(), ", q on ",
+              q.device());
+  TORCH_CHECK(2 * inv_freq.size(0) <= q.size(3) && q.size(3) % 2 == 0, "rotary dim ",
+              2 * inv_freq.size(0), " does not fit head_dim ", q.size(3));
+}
+
+void rotary_launch(const at::Tensor& q_in, const at::Tensor* k_in, at::Tensor& q_out,
+                   at::Tensor* k_out, const at::Tensor& inv_freq_in, const OptTensor& positions_in,
+                   int64_t first, bool interleaved, double magnitude, bool inverse) {
+  const at::Tensor q = heads_input(q_in, "q", interleaved);
+  const int dt = dtype_code(q);
+  check_freq(inv_freq_in, q);
+  const at::Tensor inv_freq = inv_freq_in.contiguous();
+  const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
+  at::Tensor k;
+  if (k_in) {
+    k = heads_input(*k_in, "k", interleaved);
+    TORCH_CHECK(k.scalar_type() == q.scalar_type(), "q and k must have the same dtype");
+    check_like(k, {B, S, k.size(2), D}, q, "k");
+  }
+  at::Tensor positions;
+  int64_t pos_stride = 0;
+  if (positions_in) {
+    positions = *positions_in;
+    TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+                "positions must be int32 or int64");
+    if (positions.dim() == 1) {
+      check_like(positions, {S}, q, "positions");
+    } else {
+      check_like(positions, {B, S}, q, "positions");
+    }
+    if (S > 1 && positions.stride(-1) != 1) positions = positions.contiguous();
+    pos_stride = positions.dim() == 2 && B > 1 ? positions.stride(0) : 0;
+  }
+  if (B * S == 0) return;
+  const bool no_q = q.size(2) == 0, no_k = !k_in || k.size(2) == 0;
+  if (no_q && no_k) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  fa_sm100_heads hq, hk;
+  if (!no_q) hq = heads_of(q, &q_out);
+  if (!no_k) hk = heads_of(k, k_out);
+  const int rc = fa_sm100_rotary(
+      no_q ? &hk : &hq, no_q || no_k ? nullptr : &hk, inv_freq.data_ptr<double>(),
+      2 * (int)inv_freq.size(0), interleaved, (float)magnitude, inverse,
+      positions.defined() ? positions.data_ptr() : nullptr,
+      positions.defined() && positions.scalar_type() == at::kLong, pos_stride, first, (int)B, (int)S,
+      (int)D, dt, at::cuda::getCurrentCUDAStream().stream());
+  check_rc(rc, "fa_sm100_rotary");
+}
+
+at::Tensor rotary_cuda(const at::Tensor& x, const at::Tensor& inv_freq, const OptTensor& positions,
+                       int64_t first, bool interleaved, double magnitude, bool inverse) {
+  c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor out = at::empty(x.sizes(), x.options());
+  rotary_launch(x, nullptr, out, nullptr, inv_freq, positions, first, interleaved, magnitude, inverse);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_qk_cuda(const at::Tensor& q, const at::Tensor& k,
+                                                  const at::Tensor& inv_freq,
+                                                  const OptTensor& positions, int64_t first,
+                                                  bool interleaved, double magnitude, bool inverse) {
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor qo = at::empty(q.sizes(), q.options());
+  at::Tensor ko = at::empty(k.sizes(), k.options());
+  rotary_launch(q, &k, qo, &ko, inv_freq, positions, first, interleaved, magnitude, inverse);
+  return {qo, ko};
+}
+
+at::Tensor rotary_op(const at::Tensor& x, const at::Tensor& inv_freq, const OptTensor& positions,
+                     int64_t first, bool interleaved, double magnitude, bool inverse) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fav::rotary", "")
+                       .typed<decltype(rotary_cuda)>();
+  return op.call(x, inv_freq, positions, first, interleaved, magnitude, inverse);
+}
+std::tuple<at::Tensor, at::Tensor> rotary_qk_op(const at::Tensor& q, const at::Tensor& k,
+                                                const at::Tensor& inv_freq,
+                                                const OptTensor& positions, int64_t first,
+                                                bool interleaved, double magnitude, bool inverse) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fav::rotary_qk", "")
+                       .typed<decltype(rotary_qk_cuda)>();
+  return op.call(q, k, inv_freq, positions, first, interleaved, magnitude, inverse);
+}
+
+// The gradient of a rotation by a is the rotation by -a, through the same
+// operators (so it has a gradient itself).
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+void save_turn(AutogradContext* ctx, const at::Tensor& inv_freq, const OptTensor& positions,
+               int64_t first, bool interleaved, double magnitude, bool inverse) {
+  ctx->save_for_backward({inv_freq, positions.value_or(at::Tensor())});
+  ctx->saved_data["first"] = first;
+  ctx->saved_data["interleaved"] = interleaved;
+  ctx->saved_data["magnitude"] = magnitude;
+  ctx->saved_data["inverse"] = inverse;
+}
+
+struct RotaryFn : public torch::autograd::Function<RotaryFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& inv_freq,
+                          const OptTensor& positions, int64_t first, bool interleaved,
+                          double magnitude, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    save_turn(ctx, inv_freq, positions, first, interleaved, magnitude, inverse);
+    return rotary_op(x, inv_freq, positions, first, interleaved, magnitude, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptTensor positions = saved[1].defined() ? OptTensor(saved[1]) : OptTensor();
+    at::Tensor dx;
+    if (grads[0].defined())
+      dx = rotary_op(grads[0], saved[0], positions, ctx->saved_data["first"].toInt(),
+                     ctx->saved_data["interleaved"].toBool(), ctx->saved_data["magnitude"].toDouble(),
+                     !ctx->saved_data["inverse"].toBool());
+    return {dx, Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
+  }
+};
+
+struct RotaryQkFn : public torch::autograd::Function<RotaryQkFn> {
+  static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k,
+                               const Variable& inv_freq, const OptTensor& positions, int64_t first,
+                               bool interleaved, double magnitude, bool inverse) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    save_turn(ctx, inv_freq, positions, first, interleaved, magnitude, inverse);
+    ctx->set_materialize_grads(false);
+    auto [qo, ko] = rotary_qk_op(q, k, inv_freq, positions, first, interleaved, magnitude, inverse);
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const OptTensor positions = saved[1].defined() ? OptTensor(saved[1]) : OptTensor();
+    const int64_t first = ctx->saved_data["first"].toInt();
+    const bool inter = ctx->saved_data["interleaved"].toBool();
+    const double mag = ctx->saved_data["magnitude"].toDouble();
+    const bool inv = !ctx->saved_data["inverse"].toBool();
+    const bool want_q = grads[0].defined() && ctx->needs_input_grad(0);
+    const bool want_k = grads[1].defined() && ctx->needs_input_grad(1);
+    at::Tensor dq, dk;
+    if (want_q && want_k) {
+      std::tie(dq, dk) = rotary_qk_op(grads[0], grads[1], saved[0], positions, first, inter, mag, inv);
+    } else if (want_q) {
+      dq = rotary_op(grads[0], saved[0], positions, first, inter, mag, inv);
+    } else if (want_k) {
+      dk = rotary_op(grads[1], saved[0], positions, first, inter, mag, inv);
+    }
+    return {dq, dk, Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
+  }
+};
+
+at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& inv_freq,
+                           const OptTensor& positions, int64_t first, bool interleaved,
+                           double magnitude, bool inverse) {
+  if (at::GradMode::is_enabled() && x.requires_grad())
+    return RotaryFn::apply(x, inv_freq, positions, first, interleaved, magnitude, inverse);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rotary_op(x, inv_freq, positions, first, interleaved, magnitude, inverse);
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_qk_autograd(const at::Tensor& q, const at::Tensor& k,
+                                                      const at::Tensor& inv_freq,
+                                                      const OptTensor& positions, int64_t first,
+                                                      bool interleaved, double magnitude,
+                                                      bool inverse) {
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
+    auto r = RotaryQkFn::apply(q, k, inv_freq, positions, first, interleaved, magnitude, inverse);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return rotary_qk_op(q, k, inv_freq, positions, first, interleaved, magnitude, inverse);
+}
+
+// ------------------------------------------------------------ key/value cache
+// 16-bit: two page tensors; 4-bit (v_pages absent): blocks of 20 * head_dim bytes.
+fa_sm100_kv_cache cache_of(const at::Tensor& k_pages, const OptTensor& v_pages, int dtype) {
+  TORCH_CHECK(k_pages.is_cuda(), "the cache must be a CUDA tensor");
+  TORCH_CHECK(k_pages.dim() == 4 && k_pages.is_contiguous(), "cache pages must be contiguous and 4-D");
+  fa_sm100_kv_cache c;
+  c.k_pages = k_pages.data_ptr();
+  c.num_pages = (int)k_pages.size(0);
+  c.nheads_kv = (int)k_pages.size(1);
+  c.dtype = dtype;
+  TORCH_CHECK(k_pages.size(0) <= 2147483647 && k_pages.size(1) <= 2147483647, "too many pages");
+  if (v_pages) {
+    TORCH_CHECK(dtype_code(k_pages) == dtype, "the tensors must have the cache's dtype");
+    TORCH_CHECK(v_pages->scalar_type() == k_pages.scalar_type() && v_pages->is_contiguous(),
+                "v_pages must be contiguous, of k_pages' dtype");
+    check_like(*v_pages, k_pages.sizes(), k_pages, "v_pages");
+    c.v_pages = v_pages->data_ptr();
+    c.page_size = (int)k_pages.size(2);
+    c.head_dim = (int)k_pages.size(3);
+    c.bits = 16;
+  } else {
+    TORCH_CHECK(k_pages.scalar_type() == at::kByte && k_pages.size(3) % 20 == 0,
+                "4-bit pages must be uint8 (pages, kv heads, page_size / 16, 20 * head_dim)");
+    c.v_pages = nullptr;
+    c.page_size = (int)k_pages.size(2) * 16;
+    c.head_dim = (int)k_pages.size(3) / 20;
+    c.bits = 4;
+  }
+  return c;
+}
+
+// (batch, ...) int32, on the cache's device, contiguous.
+at::Tensor int_input(const at::Tensor& t, int64_t dim, int64_t batch, const at::Tensor& pages,
+                     const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.size(0) == batch, name,
+              " must be int32 with ", dim, " dimension(s), the first of ", batch);
+  TORCH_CHECK(t.device() == pages.device(), name, " is on ", t.device(), ", the cache on ",
+              pages.device());
+  return t.contiguous();
+}
+
+at::Tensor kv_append_cuda(const at::Tensor& k_pages, const OptTensor& v_pages, const at::Tensor& k_in,
+                          const at::Tensor& v_in, const OptTensor& q_in,
+                          const at::Tensor& table_in, const at::Tensor& starts_in,
+                          const OptTensor& counts_in, const OptTensor& freq_in, bool interleaved,
+                          double magnitude) {
+  const at::Tensor k = heads_input(k_in, "k", false), v = heads_input(v_in, "v", false);
+  const int dt = dtype_code(k);
+  const fa_sm100_kv_cache cache = cache_of(k_pages, v_pages, dt);
+  const int64_t B = k.size(0), S = k.size(1), D = k.size(3);
+  check_like(k, {B, S, cache.nheads_kv, cache.head_dim}, k_pages, "k");
+  check_like(v, k.sizes(), k, "v");
+  TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have the same dtype");
+  at::Tensor q, q_out;
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  if (q_in) {
+    q = heads_input(*q_in, "q", false);
+    check_like(q, {B, S, q.size(2), D}, k, "q");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type(), "q must have k's dtype");
+    q_out = at::empty(q.sizes(), q.options());
+  } else {
+    q_out = at::empty({0}, k.options());
+  }
+  const at::Tensor table = int_input(table_in, 2, B, k_pages, "page_table");
+  const at::Tensor starts = int_input(starts_in, 1, B, k_pages, "starts");
+  at::Tensor counts, freq;
+  if (counts_in) counts = int_input(*counts_in, 1, B, k_pages, "counts");
+  if (freq_in) {
+    check_freq(*freq_in, k);
+    freq = freq_in->contiguous();
+  }
+  if (B * S == 0) return q_out;
+  const fa_sm100_heads hk = heads_of(k, nullptr), hv = heads_of(v, nullptr);
+  fa_sm100_heads hq;
+  const bool with_q = q.defined() && q.size(2) > 0;
+  if (with_q) hq = heads_of(q, &q_out);
+  at::Tensor st = status_word(k_pages.get_device());
+  const int rc = fa_sm100_kv_append(
+      &cache, &hk, &hv, with_q ? &hq : nullptr, table.data_ptr<int>(), (int)table.size(1),
+      starts.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr,
+      freq.defined() ? freq.data_ptr<double>() : nullptr,
+      freq.defined() ? 2 * (int)freq.size(0) : 0, interleaved, (float)magnitude, (int)B, (int)S,
+      st.data_ptr<int>(), at::cuda::getCurrentCUDAStream().stream());
+  check_rc(rc, "fa_sm100_kv_append");
+  return q_out;
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_read_cuda(const at::Tensor& k_pages, const OptTensor& v_pages,
+                                                at::ScalarType dtype, const at::Tensor& table_in,
+                                                const at::Tensor& lengths_in, int64_t max_len) {
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "fp16 or bf16 only");
+  const fa_sm100_kv_cache cache =
+      cache_of(k_pages, v_pages, dtype == at::kHalf ? FA_DTYPE_F16 : FA_DTYPE_BF16);
+  const int64_t B = lengths_in.numel();
+  const at::Tensor table = int_input(table_in, 2, B, k_pages, "page_table");
+  const at::Tensor lengths = int_input(lengths_in, 1, B, k_pages, "lengths");
+  TORCH_CHECK(max_len >= 0 && max_len <= 2147483647, "max_len out of range");
+  c10::cuda::CUDAGuard guard(k_pages.device());
+  const auto opts = k_pages.options().dtype(dtype);
+  at::Tensor k = at::empty({B, max_len, cache.nheads_kv, cache.head_dim}, opts);
+  at::Tensor v = at::empty({B, max_len, cache.nheads_kv, cache.head_dim}, opts);
+  if (B == 0 || max_len == 0) return {k, v};
+  at::Tensor st = status_word(k_pages.get_device());
+  const int rc = fa_sm100_kv_read(&cache, table.data_ptr<int>(), (int)table.size(1),
+                                  lengths.data_ptr<int>(), k.data_ptr(), v.data_ptr(), (int)B,
+                                  (int)max_len, st.data_ptr<int>(),
+                                  at::cuda::getCurrentCUDAStream().stream());
+  check_rc(rc, "fa_sm100_kv_read");
+  return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> decode_cuda(const at::Tensor& q_in, const at::Tensor& k_pages,
+                                               const OptTensor& v_pages, const at::Tensor& table_in,
+                                               const at::Tensor& lengths_in,
+                                               const OptTensor& starts_in, bool causal,
+                                               double sm_scale, bool need_lse) {
+  const at::Tensor q = kernel_input(q_in, "q");
+  const fa_sm100_kv_cache cache = cache_of(k_pages, v_pages, dtype_code(q));
+  const int64_t B = q.size(0), S = q.size(1), H = q.size(2);
+  check_like(q, {B, S, H, cache.head_dim}, k_pages, "q");
+  TORCH_CHECK(H > 0 && cache.nheads_kv > 0 && H % cache.nheads_kv == 0,
+              "the query heads must be a multiple of the cache's heads");
+  const at::Tensor table = int_input(table_in, 2, B, k_pages, "page_table");
+  const at::Tensor lengths = int_input(lengths_in, 1, B, k_pages, "lengths");
+  at::Tensor starts;
+  if (starts_in) starts = int_input(*starts_in, 1, B, k_pages, "starts");
+  c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse = at::empty(need_lse ? std::vector<int64_t>{B, H, S} : std::vector<int64_t>{0},
+                             q.options().dtype(at::kFloat));
+  if (B * S == 0) return {out, lse};
+  const size_t nbytes = fa_sm100_decode_workspace_bytes(&cache, (int)table.size(1), (int)B, (int)S, (int)H);
+  TORCH_CHECK(nbytes > 0, "fa_sm100_decode: unsupported shape");
+  at::Tensor ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
+  at::Tensor st = status_word(q.get_device());
+  const int rc = fa_sm100_decode(
+      &cache, q.data_ptr(), out.data_ptr(), need_lse ? lse.data_ptr<float>() : nullptr,
+      table.data_ptr<int>(), (int)table.size(1), lengths.data_ptr<int>(),
+      starts.defined() ? starts.data_ptr<int>() : nullptr, ws.data_ptr(), nbytes, (int)B, (int)S,
+      (int)H, (float)sm_scale, causal ? 1 : 0, st.data_ptr<int>(),
+      at::cuda::getCurrentCUDAStream().stream());
+  check_rc(rc, "fa_sm100_decode");
+  return {out, lse};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fav, m) {
@@ -187,10 +541,36 @@ TORCH_LIBRARY(fav, m) {
       "float sm_scale, bool deterministic=False) -> (Tensor, Tensor, Tensor)");
   m.def("status(int device) -> Tensor", &status_word);
   m.def("merge_(Tensor(a!) acc_o, Tensor(b!) acc_lse, Tensor o, Tensor lse, bool first) -> ()");
+  m.def(
+      "rotary(Tensor x, Tensor inv_freq, Tensor? positions, int first, bool interleaved, "
+      "float magnitude, bool inverse) -> Tensor");
+  m.def(
+      "rotary_qk(Tensor q, Tensor k, Tensor inv_freq, Tensor? positions, int first, "
+      "bool interleaved, float magnitude, bool inverse) -> (Tensor, Tensor)");
+  m.def(
+      "kv_append(Tensor(a!) k_pages, Tensor(b!)? v_pages, Tensor k, Tensor v, Tensor? q, "
+      "Tensor page_table, Tensor starts, Tensor? counts, Tensor? inv_freq, bool interleaved, "
+      "float magnitude) -> Tensor");
+  m.def(
+      "kv_read(Tensor k_pages, Tensor? v_pages, ScalarType dtype, Tensor page_table, "
+      "Tensor lengths, int max_len) -> (Tensor, Tensor)");
+  m.def(
+      "decode(Tensor q, Tensor k_pages, Tensor? v_pages, Tensor page_table, Tensor lengths, "
+      "Tensor? starts, bool causal, float sm_scale, bool need_lse) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(fav, CUDA, m) {
   m.impl("fwd", &fwd_cuda);
   m.impl("bwd", &bwd_cuda);
   m.impl("merge_", &merge_cuda);
+  m.impl("rotary", &rotary_cuda);
+  m.impl("rotary_qk", &rotary_qk_cuda);
+  m.impl("kv_append", &kv_append_cuda);
+  m.impl("kv_read", &kv_read_cuda);
+  m.impl("decode", &decode_cuda);
+}
+
+TORCH_LIBRARY_IMPL(fav, Autograd, m) {
+  m.impl("rotary", &rotary_autograd);
+  m.impl("rotary_qk", &rotary_qk_autograd);
 }

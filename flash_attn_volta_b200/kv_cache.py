@@ -1,0 +1,208 @@
+"""Paged key/value cache: append, read back, and attention over it.
+
+Serving next to ``flash_attn``: a prompt's attention runs in flash_attn while
+``kv_cache_append`` stores its keys and values; then each new token is appended
+(rotated on the way) and ``flash_attn_decode`` attends to everything cached.
+A prompt that arrives in chunks reads its prefix back with ``kv_cache_read`` and
+calls flash_attn(q_chunk, k_all, v_all, causal=True).
+
+A page holds ``page_size`` tokens of one sequence; ``page_table`` (B, W) int32 names
+the page of tokens i * page_size .. of each sequence in column i (entries behind
+a sequence's length are not read).  Lengths and starts are (B,) int32 tensors on
+the device and are never copied to the host, so the calls can be captured in CUDA
+graphs and replayed with other lengths, tables and tokens.  A page id outside the
+cache, or a length beyond the table, sets bit 2 of the status word
+(``check_status``); those tokens are not written, and take no part in reads.
+
+16-bit pages are ordinary tensors (pages, kv heads, page, head_dim).  4-bit pages
+hold groups of 32 dims of a token as 4-bit codes with an fp16 scale and minimum
+(5 bits a value; include/fa_sm100.h, csrc/fa_kv_cache.cuh); the attention
+kernel multiplies the codes themselves.
+
+The reference has no cache (its patched models decode in their own code).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib, ops
+from .rotary import Rotary
+
+BLOCK_TOKENS = 16
+
+
+class PagedKVCache:
+    """Pages of one attention layer, 16-bit (``k_pages``, ``v_pages``) or 4-bit
+    (``PagedKVCache.of_blocks``); ``PagedKVCache.allocate`` makes them."""
+    __slots__ = ("k_pages", "v_pages", "num_pages", "page_size", "n_heads", "head_dim", "dtype",
+                 "bits")
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
+        assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, \
+            "k_pages and v_pages must be (pages, kv heads, page_size, head_dim)"
+        assert k_pages.dtype in (torch.float16, torch.bfloat16) and k_pages.dtype == v_pages.dtype, \
+            "fp16 (or bf16) pages only"
+        assert k_pages.device == v_pages.device, "k_pages and v_pages must be on one device"
+        assert k_pages.shape[3] in (16, 32, 64, 128), \
+            f"unsupported head_dim {k_pages.shape[3]} (allowed: 16,32,64,128)"
+        self._set(k_pages, v_pages, k_pages.shape[2], k_pages.shape[3], k_pages.dtype, 16)
+        assert v_pages.is_contiguous(), "pages must be contiguous"
+
+    def _set(self, k_pages, v_pages, page_size, head_dim, dtype, bits):
+        assert k_pages.is_contiguous(), "pages must be contiguous"
+        assert 16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, \
+            f"page_size {page_size} is not a power of two from 16 to 1024"
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.num_pages, self.n_heads = k_pages.shape[0], k_pages.shape[1]
+        assert self.num_pages > 0 and self.n_heads > 0, "a cache needs pages and heads"
+        assert self.num_pages * self.n_heads * page_size < 2 ** 31, \
+            "pages * heads * page_size must be below 2^31"
+        self.page_size, self.head_dim = page_size, head_dim
+        self.dtype, self.bits = dtype, bits
+
+    @classmethod
+    def of_blocks(cls, blocks: torch.Tensor, head_dim: int,
+                  dtype: torch.dtype = torch.float16) -> "PagedKVCache":
+        """4-bit pages: uint8 (pages, kv heads, page_size / 16, 20 * head_dim);
+        ``dtype`` is that of the keys, values and queries in the calls."""
+        assert head_dim in (32, 64, 128), f"unsupported head_dim {head_dim} at 4 bits (32,64,128)"
+        assert dtype in (torch.float16, torch.bfloat16), "fp16 (or bf16) only"
+        assert blocks.dtype == torch.uint8 and blocks.dim() == 4 \
+            and blocks.shape[3] == 20 * head_dim, \
+            "blocks must be uint8 (pages, kv heads, page_size / 16, 20 * head_dim)"
+        c = cls.__new__(cls)
+        c._set(blocks, None, blocks.shape[2] * BLOCK_TOKENS, head_dim, dtype, 4)
+        return c
+
+    @classmethod
+    def allocate(cls, num_pages: int, page_size: int, n_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.float16, bits: int = 16,
+                 device="cuda") -> "PagedKVCache":
+        """A new cache; what its pages hold is undefined until it is appended."""
+        assert bits in (4, 16), "bits must be 4 or 16"
+        if bits == 4:
+            assert page_size % BLOCK_TOKENS == 0, "page_size must be a multiple of 16"
+            return cls.of_blocks(torch.empty((num_pages, n_heads, page_size // BLOCK_TOKENS,
+                                              20 * head_dim), dtype=torch.uint8, device=device),
+                                 head_dim, dtype)
+        shape = (num_pages, n_heads, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device),
+                   torch.empty(shape, dtype=dtype, device=device))
+
+
+def _check_ints(cache, batch, page_table, **vectors):
+    dev = cache.k_pages.device
+    assert cache.k_pages.is_cuda, "the cache must be on CUDA"
+    assert page_table.dtype == torch.int32 and page_table.dim() == 2 \
+        and page_table.shape[0] == batch and page_table.shape[1] > 0 \
+        and page_table.device == dev, "page_table must be (batch, pages) int32 on the cache's device"
+    for name, t in vectors.items():
+        assert t is None or (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == batch
+                             and t.device == dev), \
+            f"{name} must be (batch,) int32 on the cache's device"
+
+
+def _no_grad(*tensors):
+    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                                for t in tensors)), \
+        "the cache operators are for inference: call them under torch.no_grad()"
+
+
+def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
+                    page_table: torch.Tensor, starts: torch.Tensor,
+                    counts: torch.Tensor | None = None, *, q: torch.Tensor | None = None,
+                    rotary: Rotary | None = None) -> torch.Tensor | None:
+    """Store new tokens: token s of sequence b at position starts[b] + s.
+
+    Args:
+        k, v: (B, S, H_kv, D) of the cache's dtype, any strides.
+        counts: (B,) tokens of each sequence that are new (the rows behind are
+            padding and are not stored); None: all S.
+        rotary: rotates k (and q) at those positions before k is stored.
+        q: (B, S, H, D) queries of the same tokens; returned rotated (copied
+            without ``rotary``), contiguous, padding rows included.
+    No two tokens of one call may go to the same place of the cache.
+    """
+    assert k.dim() == 4 and k.shape == v.shape, f"kv shape mismatch {k.shape} {v.shape}"
+    B, S, Hkv, D = k.shape
+    assert Hkv == cache.n_heads and D == cache.head_dim, \
+        f"k {tuple(k.shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
+    dev = cache.k_pages.device
+    assert k.dtype == v.dtype == cache.dtype, f"k and v must have the cache's dtype {cache.dtype}"
+    assert k.device == v.device == dev, "k and v must be on the cache's device"
+    _check_ints(cache, B, page_table, starts=starts, counts=counts)
+    if q is not None:
+        assert q.dim() == 4 and q.shape[:2] == (B, S) and q.shape[3] == D and q.dtype == k.dtype \
+            and q.device == dev, f"q {tuple(q.shape)} does not fit k {tuple(k.shape)}"
+    if rotary is not None:
+        assert rotary.dim <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
+        assert rotary.inv_freq.device == dev, "inv_freq must be on the cache's device"
+    _no_grad(k, v, q)
+    ops.load()
+    ops.note_device(dev.index)
+    out = torch.ops.fav.kv_append(
+        cache.k_pages, cache.v_pages, k, v, q, page_table, starts, counts,
+        None if rotary is None else rotary.inv_freq,
+        rotary is not None and rotary.interleaved, 1.0 if rotary is None else rotary.magnitude)
+    if _lib.debug_sync():
+        _lib.check_status(dev)
+    return out if q is not None else None
+
+
+def kv_cache_read(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                  max_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The first lengths[b] cached tokens of each sequence as contiguous k and v
+    (B, max_len, H_kv, D) of the cache's dtype; rows behind a length are zero.
+    max_len: default the table's room; longer sequences are cut there."""
+    if max_len is None:
+        max_len = page_table.shape[-1] * cache.page_size
+    assert max_len >= 0, "max_len must not be negative"
+    _check_ints(cache, lengths.shape[0], page_table, lengths=lengths)
+    dev = cache.k_pages.device
+    ops.load()
+    ops.note_device(dev.index)
+    k, v = torch.ops.fav.kv_read(cache.k_pages, cache.v_pages, cache.dtype, page_table, lengths,
+                                 max_len)
+    if _lib.debug_sync():
+        _lib.check_status(dev)
+    return k, v
+
+
+def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor,
+                      lengths: torch.Tensor, causal: bool = True, sm_scale: float | None = None,
+                      return_softmax_lse: bool = False, *, starts: torch.Tensor | None = None):
+    """Attention of one or a few new tokens per sequence over the cache.
+
+    Args:
+        q: (B, S, H, D) of the cache's dtype, H % H_kv == 0 (query head h reads
+            K/V head h // (H // H_kv)).  Any S; built for S * H / H_kv up to a
+            few tens of rows (the cache is read once per 16 of them).
+        lengths: (B,) int32 cached tokens of each sequence, the new ones included.
+        causal: query i of sequence b sees tokens j <= starts[b] + i.
+        starts: (B,) int32 position of each sequence's first query (default
+            lengths - S); for a batch whose sequences have different counts of
+            new tokens, pass what kv_cache_append got.
+        sm_scale, return_softmax_lse: as in flash_attn_forward.
+
+    Returns:
+        out (B, S, H, D), with return_softmax_lse also lse (B, H, S) fp32.  A row
+        that sees no token gets out 0 and lse +inf.
+    """
+    assert q.dim() == 4 and q.shape[3] == cache.head_dim and q.shape[2] > 0 \
+        and q.shape[2] % cache.n_heads == 0, \
+        f"q {tuple(q.shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
+    dev = cache.k_pages.device
+    assert q.dtype == cache.dtype and q.device == dev, "q must have the cache's dtype and device"
+    _check_ints(cache, q.shape[0], page_table, lengths=lengths, starts=starts)
+    _no_grad(q)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(q.shape[3])
+    ops.load()
+    ops.note_device(dev.index)
+    out, lse = torch.ops.fav.decode(q, cache.k_pages, cache.v_pages, page_table, lengths, starts,
+                                    bool(causal), float(sm_scale), bool(return_softmax_lse))
+    if _lib.debug_sync():
+        _lib.check_status(dev)
+    return (out, lse) if return_softmax_lse else out

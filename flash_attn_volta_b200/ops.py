@@ -55,6 +55,31 @@ def _check_qkv(q, k, v):
         raise RuntimeError("the query heads must be a multiple of the key/value heads")
 
 
+def _check_rotary(x, inv_freq, positions):
+    if x.dim() != 4 or inv_freq.dim() != 1 or 2 * inv_freq.shape[0] > x.shape[3]:
+        raise RuntimeError("rotary: (batch, seqlen, heads, head_dim) and at most head_dim / 2 "
+                           "frequencies expected")
+    if positions is not None:
+        _expect(positions, x.shape[1:2] if positions.dim() == 1 else x.shape[:2], "positions")
+
+
+def _cache_dim(k_pages, v_pages):
+    """head_dim of a cache: 16-bit pages, or 4-bit blocks of 20 * head_dim bytes."""
+    if k_pages.dim() != 4:
+        raise RuntimeError("cache pages must be 4-D")
+    if v_pages is None:
+        return k_pages.shape[3] // 20
+    _expect(v_pages, k_pages.shape, "v_pages")
+    return k_pages.shape[3]
+
+
+def _check_ints(batch, page_table, **vectors):
+    _expect(page_table, (batch, page_table.shape[-1]), "page_table")
+    for name, t in vectors.items():
+        if t is not None:
+            _expect(t, (batch,), name)
+
+
 def _register_python_parts() -> None:
     @torch.library.register_fake("fav::fwd")
     def _fwd_fake(q, k, v, causal, sm_scale):
@@ -76,6 +101,49 @@ def _register_python_parts() -> None:
         _expect(lse, (o.shape[0], o.shape[2], o.shape[1]), "lse")
         _expect(acc_lse, lse.shape, "acc_lse")
         return None
+
+    @torch.library.register_fake("fav::rotary")
+    def _rotary_fake(x, inv_freq, positions, first, interleaved, magnitude, inverse):
+        _check_rotary(x, inv_freq, positions)
+        return x.new_empty(x.shape)
+
+    @torch.library.register_fake("fav::rotary_qk")
+    def _rotary_qk_fake(q, k, inv_freq, positions, first, interleaved, magnitude, inverse):
+        _check_rotary(q, inv_freq, positions)
+        _expect(k, (q.shape[0], q.shape[1], k.shape[2], q.shape[3]), "k")
+        return q.new_empty(q.shape), k.new_empty(k.shape)
+
+    @torch.library.register_fake("fav::kv_append")
+    def _kv_append_fake(k_pages, v_pages, k, v, q, page_table, starts, counts, inv_freq,
+                        interleaved, magnitude):
+        heads, dim = k_pages.shape[1], _cache_dim(k_pages, v_pages)
+        _expect(k, (k.shape[0], k.shape[1], heads, dim), "k")
+        _expect(v, k.shape, "v")
+        _check_ints(k.shape[0], page_table, starts=starts, counts=counts)
+        if inv_freq is not None:
+            _check_rotary(k, inv_freq, None)
+        if q is None:
+            return k.new_empty((0,))
+        _expect(q, (k.shape[0], k.shape[1], q.shape[2], dim), "q")
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake("fav::kv_read")
+    def _kv_read_fake(k_pages, v_pages, dtype, page_table, lengths, max_len):
+        B = lengths.shape[0]
+        _check_ints(B, page_table, lengths=lengths)
+        shape = (B, max_len, k_pages.shape[1], _cache_dim(k_pages, v_pages))
+        return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
+
+    @torch.library.register_fake("fav::decode")
+    def _decode_fake(q, k_pages, v_pages, page_table, lengths, starts, causal, sm_scale,
+                     need_lse):
+        B, S, H, _ = q.shape
+        _expect(q, (B, S, H, _cache_dim(k_pages, v_pages)), "q")
+        if H == 0 or H % k_pages.shape[1]:
+            raise RuntimeError("the query heads must be a multiple of the cache's heads")
+        _check_ints(B, page_table, lengths=lengths, starts=starts)
+        lse = (B, H, S) if need_lse else (0,)
+        return q.new_empty(q.shape), q.new_empty(lse, dtype=torch.float32)
 
     def _setup(ctx, inputs, output):
         q, k, v, causal, sm_scale = inputs

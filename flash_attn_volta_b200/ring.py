@@ -41,6 +41,7 @@ import torch.distributed as dist
 from . import ops
 from .backward import flash_attn_backward
 from .forward import flash_attn_forward
+from .rotary import Rotary, rotary_embed_qk
 
 
 def _kernel_block_fwd(q, k, v, causal, scale):
@@ -54,10 +55,19 @@ def _kernel_block_bwd(do, q, k, v, o, lse, causal, scale):
 # The per-block computations; the CPU tests substitute the oracle here.
 block_fwd = _kernel_block_fwd
 block_bwd = _kernel_block_bwd
+rotate = rotary_embed_qk
 
 
 def zigzag_chunk_ids(rank: int, world: int) -> tuple[int, int]:
     return rank, 2 * world - 1 - rank
+
+
+def zigzag_positions(rank: int, world: int, rows: int, device=None) -> torch.Tensor:
+    """Positions in the whole sequence of the `rows` rows of this rank's shard."""
+    C = rows // 2
+    a, b = zigzag_chunk_ids(rank, world)
+    at = torch.arange(C, device=device, dtype=torch.int64)
+    return torch.cat([at + a * C, at + b * C])
 
 
 def zigzag_shard(x: torch.Tensor, rank: int, world: int, dim: int = 1) -> torch.Tensor:
@@ -273,7 +283,8 @@ class _RingFlashAttnFn(torch.autograd.Function):
 
 
 def ring_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = True,
-                    sm_scale: Optional[float] = None, group=None) -> torch.Tensor:
+                    sm_scale: Optional[float] = None, group=None, *,
+                    rotary: Optional[Rotary] = None) -> torch.Tensor:
     """Attention over a sequence sharded across the ranks of `group` (zigzag).
 
     Args:
@@ -284,6 +295,8 @@ def ring_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
         causal: top-left causal mask over the full (unsharded) sequence.
         sm_scale: softmax scale (default 1/sqrt(D)).
         group: process group (default: the world).
+        rotary: rotates the shard's q and k at their positions in the whole
+            sequence first, with gradients.
 
     Returns the rank's shard of the output, same layout; autograd-aware.
     """
@@ -294,4 +307,7 @@ def ring_flash_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: b
         "q and k/v must have the same batch, sequence shard and head_dim"
     assert k.shape[2] > 0 and q.shape[2] % k.shape[2] == 0, \
         "the query heads must be a multiple of the key/value heads"
+    if rotary is not None:
+        rank, world = _world(group)
+        q, k = rotate(q, k, rotary, zigzag_positions(rank, world, q.shape[1], q.device))
     return _RingFlashAttnFn.apply(q, k, v, causal, sm_scale, group)

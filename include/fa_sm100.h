@@ -9,6 +9,8 @@
  * Bit 1 (2): a backward row term was beyond the range the kernel represents
  * and was clamped (fp16: |LSE / sm_scale| or |rowsum(O * dO)| above ~1.3e8;
  * bf16: above its largest finite value); the gradients of those rows are wrong.
+ * Bit 2 (4): a page id or a length was outside the key/value cache; the tokens
+ * behind it were not written, and not read (zeros, or no part in the softmax).
  * Calls are asynchronous and thread-safe.  All of them except
  * fa_sm100_bwd_noalloc keep no state between calls; that one shares a static
  * device array between calls (see its comment below).
@@ -157,6 +159,89 @@ int fa_sm100_bwd_noalloc(const void* dout, const void* q, const void* k, const v
  * No counterpart in the reference (it has no multi-GPU path). */
 int fa_sm100_merge(float* acc_o, float* acc_lse, const void* o, const float* lse, int batch,
                    int seqlen, int nheads, int head_dim, int dtype, int first, void* stream);
+
+/* ---- Rotary positions, and attention over a paged key/value cache.  None of
+ * these has a counterpart in the reference. */
+
+/* Rows of `heads` heads for each token of a (batch, seqlen) grid: element
+ * (b, s, h, d) of `in` is in[b * stride_batch + s * stride_seq + h * stride_head
+ * + d] (strides in elements).  `out` is contiguous (batch, seqlen, heads,
+ * head_dim) and may be NULL where a function writes elsewhere. */
+typedef struct fa_sm100_heads {
+  const void* in;
+  void* out;
+  long long stride_batch, stride_seq, stride_head;
+  int heads;
+} fa_sm100_heads;
+
+/* Rotary positions of q and (if k != NULL) k in one launch.  With
+ * a = position * inv_freq[i] (computed in 64 bits) and M = magnitude, each pair
+ * (x1, x2) of the first rotary_dim dims becomes
+ *   y1 = M (x1 cos a - x2 sin a),  y2 = M (x2 cos a + x1 sin a);
+ * pairs are dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if `interleaved`;
+ * the other dims are copied.  `inverse` turns by -a: the gradient of the
+ * forward call.  inv_freq: rotary_dim / 2 device doubles.  positions: int32, or
+ * int64 if positions_64, of token (b, s) at positions[b * positions_stride + s];
+ * NULL: first + s.  head_dim and rotary_dim are even, rotary_dim <= 8192;
+ * interleaved pairs have to be 4-byte aligned. */
+int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k, const double* inv_freq,
+                    int rotary_dim, int interleaved, float magnitude, int inverse,
+                    const void* positions, int positions_64, long long positions_stride,
+                    long long first, int batch, int seqlen, int head_dim, int dtype, void* stream);
+
+/* A paged key/value cache.  A page holds page_size (a power of two, 16 to 1024)
+ * consecutive tokens of one sequence; page_table[b * table_width + i] names the
+ * page of tokens i * page_size .. of sequence b.
+ * bits = 16: k_pages and v_pages are (num_pages, nheads_kv, page_size, head_dim)
+ *   of `dtype`, head_dim 16, 32, 64 or 128.
+ * bits = 4: k_pages is (num_pages, nheads_kv, page_size / 16) blocks of
+ *   20 * head_dim bytes, each 16 tokens of one head, v_pages is unused,
+ *   head_dim 32, 64 or 128 and `dtype` the type of k, v and q in the calls.  For each group of
+ *   32 dims of a token: m = the smallest value rounded down to fp16, s = (largest
+ *   - m) / 15 rounded up to fp16, code = round((x - m) / s), value m + s * code.
+ *   (The order of the codes in a block: csrc/fa_kv_cache.cuh.)  Values beyond
+ *   +-65504 are clamped; a group that holds a NaN reads back as NaN.
+ * All bases 16-byte aligned; num_pages * nheads_kv * page_size <= 2^31 - 1. */
+typedef struct fa_sm100_kv_cache {
+  void* k_pages;
+  void* v_pages;
+  int num_pages, page_size, nheads_kv, head_dim, dtype, bits;
+} fa_sm100_kv_cache;
+
+/* Appends tokens: token s of sequence b goes to position starts[b] + s, for
+ * s < counts[b] (counts NULL: every s < seqlen).  k and v give the keys and values
+ * (`out` unused).  With inv_freq (as in fa_sm100_rotary, at those positions) k is
+ * rotated before it is stored and q, if given, into q->out; without it q is
+ * copied.  q's rows behind counts[b] are rotated too.  No two tokens of a call
+ * may go to one place. */
+int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100_heads* k,
+                       const fa_sm100_heads* v, const fa_sm100_heads* q, const int* page_table,
+                       int table_width, const int* starts, const int* counts,
+                       const double* inv_freq, int rotary_dim, int interleaved, float magnitude,
+                       int batch, int seqlen, int* status, void* stream);
+
+/* The first min(lengths[b], max_len) tokens of each sequence as contiguous k_out
+ * and v_out (batch, max_len, nheads_kv, head_dim) of the cache's dtype, zeros
+ * behind them.  batch <= 65535. */
+int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_table, int table_width,
+                     const int* lengths, void* k_out, void* v_out, int batch, int max_len,
+                     int* status, void* stream);
+
+/* Attention of seqlen query tokens per sequence over the first lengths[b] cached
+ * tokens: q, out contiguous (batch, seqlen, nheads, head_dim) of the cache's
+ * dtype, query head h reading K/V head h / (nheads / nheads_kv); lse (or NULL)
+ * (batch, nheads, seqlen) as in fa_sm100_fwd.  causal: query i sees tokens
+ * j <= starts[b] + i (starts NULL: lengths[b] - seqlen).  A row that sees no token
+ * gets out = 0, lse = +inf.  Built for a few query tokens: the cache is read once
+ * per 16 rows (query tokens x query heads of a K/V head).
+ * The workspace (caller-owned, 256-byte aligned, not initialised; bytes for the
+ * current device) is used by this call alone. */
+size_t fa_sm100_decode_workspace_bytes(const fa_sm100_kv_cache* cache, int table_width, int batch,
+                                       int seqlen, int nheads);
+int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, void* out, float* lse,
+                    const int* page_table, int table_width, const int* lengths, const int* starts,
+                    void* workspace, size_t workspace_bytes, int batch, int seqlen, int nheads,
+                    float sm_scale, int causal, int* status, void* stream);
 
 /* Upper bound, in nanoseconds, of every on-device wait of later launches
  * (default 4e9).  Process-wide. */

@@ -45,7 +45,9 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kCtasPerSm = 2;
+// A maximum is left as it is while no score is more than 2^kSlack above it (the
+// probabilities then reach 4, and times a scale of at most 8734 stay in fp16).
+constexpr float kSlack = 2.f;
 constexpr float kLn2 = 0.69314718055994531f;
 
 // Per-instantiation constants.
@@ -54,15 +56,15 @@ struct Cfg {
   static constexpr int kU = (BITS == 16 && D == 128) ? 1 : 2;  // blocks of a warp per tile
   static constexpr int kBlockBytes = BITS == 16 ? 64 * D : 20 * D;
   static constexpr int kStageBytes = kU * kBlockBytes;
-  static constexpr int kStages = BITS == 16 ? (D == 128 ? 3 : 3) : (D == 128 ? 4 : 6);
+  static constexpr int kStages = BITS == 16 ? 3 : D == 128 ? 2 : 4;
+  static constexpr int kCtas = BITS == 16 ? 2 : 3;  // per SM
   static constexpr int kTile = kWarps * kU * kBlockTokens;  // tokens
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kJoinStride = D + 4;  // floats of a row in the join buffer
   static constexpr int kJoinBytes = kWarps * 8 * kJoinStride * 4;
   static constexpr int kMiscBytes = 512;         // barriers and small shared variables
-  // two CTAs per SM: 2 x (kSmem + 1 KB) <= 228 KB
   static constexpr int kSmem = kRingBytes + kJoinBytes + kMiscBytes;
-  static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
+  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
   static constexpr int kGroups = D / 32;
 };
 
@@ -75,9 +77,9 @@ struct DecodeParams {
   const int* starts;   // (B) or null: length - Sq
   float* part_o;       // (2 * grid, ROWS, D)
   float2* part_ml;     // (2 * grid, ROWS): maximum (log2 domain), sum
-  int B, Sq, H, group, row_blocks, causal;
-  int grid;
-  float scale_log2;
+  int B, Sq, H, group, row_blocks, causal, page_shift;
+  int grid, negate;
+  float scale_log2;  // |scale| log2 e, above 0; `negate`: the scale is negative (q's sign changes)
   unsigned long long timeout_ns;
 };
 
@@ -137,6 +139,17 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
 }
+// The same with zero to add to.
+template <typename T>
+__device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  static_assert(Elem<T>::kIdescAB == 0, "fp16 operands");
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -152,7 +165,7 @@ __device__ __forceinline__ float low_half(uint32_t w) {
 
 // Position in the tile list.
 struct Cursor {
-  int b, hr, tt, nt, len;  // sequence, K/V head * row_blocks + row block, tile of nt, length
+  int b, h, rb, tt, nt, len;  // sequence, K/V head, row block, tile of nt, length
 };
 
 template <int TILE>
@@ -205,7 +218,7 @@ __device__ __forceinline__ void locate(const DecodeParams& p, int per_tile, long
 }
 
 template <typename T, int D, int BITS, int NT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+__global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
     fa_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<D, BITS>;
@@ -247,14 +260,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     cur.len = p.kv.clamp_length(given);
     cur.nt = tiles_of<C::kTile>(cur.len);
     const long long in = begin - sh.box[2];
-    cur.hr = (int)(in / cur.nt);
+    const int hr = (int)(in / cur.nt);
     cur.tt = (int)(in % cur.nt);
+    cur.h = hr / p.row_blocks;
+    cur.rb = hr % p.row_blocks;
   }
   auto advance = [&](Cursor& c) {
     if (++c.tt < c.nt) return;
     c.tt = 0;
-    if (++c.hr < segs) return;
-    c.hr = 0;
+    if (++c.rb < p.row_blocks) return;
+    c.rb = 0;
+    if (++c.h < p.kv.heads) return;
+    c.h = 0;
     if (++c.b >= p.B) return;
     c.len = p.kv.clamp_length(p.lengths[c.b]);
     c.nt = tiles_of<C::kTile>(c.len);
@@ -273,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     next_id = -2;
     if (lane < U && to_issue > 0) {
       const int tok = block_token(pc, lane);
-      if (tok < pc.len) next_id = p.kv.table[(long long)pc.b * p.kv.table_width + tok / p.kv.page];
+      if (tok < pc.len) next_id = p.kv.table[(long long)pc.b * p.kv.table_width + (tok >> p.page_shift)];
     }
   };
   auto issue = [&](int stage) {
@@ -284,17 +301,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (next_id != -2 && !ok) p.kv.report(kStatusPage);
       ok_bits = ok ? ok_bits | (1u << stage) : ok_bits & ~(1u << stage);
       if (ok) {
-        const int tok = block_token(pc, lane) & (p.kv.page - 1), h = pc.hr / p.row_blocks;
+        // block (16-bit: row) of the cache, below 2^31
+        const int at = (((next_id * p.kv.heads + pc.h) << p.page_shift) |
+                        (block_token(pc, lane) & (p.kv.page - 1)));
         const uint32_t dst = my_ring + stage * C::kStageBytes + lane * C::kBlockBytes;
         mbar_arrive_expect_tx(bar, C::kBlockBytes);
         if constexpr (BITS == 4) {
-          bulk_load(dst, p.kv.k + p.kv.block4(next_id, h, tok), C::kBlockBytes, bar);
+          bulk_load(dst, p.kv.k + (long long)(at / kBlockTokens) * C::kBlockBytes, C::kBlockBytes, bar);
         } else {
-          const int row = (next_id * p.kv.heads + h) * p.kv.page + tok;
 #pragma unroll
           for (int x = 0; x < D; x += 64) {
-            tma_load_2d(dst + x * 32, &tm_k, bar, x, row);
-            tma_load_2d(dst + 32 * D + x * 32, &tm_v, bar, x, row);
+            tma_load_2d(dst + x * 32, &tm_k, bar, x, at);
+            tma_load_2d(dst + 32 * D + x * 32, &tm_v, bar, x, at);
           }
         }
       } else {
@@ -313,10 +331,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   // ---- consumer state
   uint32_t qf[NT][KSTEPS][2];   // q as the second operand of S^T
   uint32_t qsum[NT][2];         // 4-bit: (0, head), (0, tail) of group t's sum
-  float f[NT][2];               // factor of a score to the log2 domain, per column
+  float f[NT][2];               // factor of a score to the log2 domain, per column (above 0)
   int lim[NT][2];               // tokens that a column's query row sees
   int col_q[NT][2];             // query token of a column's row; -1: none
-  float o[KSTEPS][NT][4], om[NT][4], m[NT][2], l[NT][2];
+  float o[KSTEPS][NT][4], om[NT][4], l[NT][2];
+  float mf[NT][2];              // running maximum in the log2 domain
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
 
   auto limit_of = [&](int qpos) {
@@ -326,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   };
 
   auto begin_segment = [&]() {
-    const int h = cur.hr / p.row_blocks, rb = cur.hr % p.row_blocks;
+    const int h = cur.h, rb = cur.rb;
     const int rows = p.Sq * p.group;
     start = p.starts ? p.starts[cur.b] : cur.len - p.Sq;
     qp_first = rb * ROWS / p.group;
@@ -340,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const int rr = rb * ROWS + n * 8 + 2 * t + i;
         lim[n][i] = rr < rows ? limit_of(rr / p.group) : 0;
         col_q[n][i] = rr < rows ? rr / p.group : -1;
-        m[n][i] = -INFINITY;
+        mf[n][i] = -INFINITY;
         l[n][i] = 0.f;
       }
 #pragma unroll
@@ -359,6 +378,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int k = 0; k < KSTEPS; ++k) {
           qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * t) : 0u;
           qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 + 2 * t) : 0u;
+        }
+        if (p.negate) {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            qf[n][k][0] ^= 0x80008000u;
+            qf[n][k][1] ^= 0x80008000u;
+          }
         }
         f[n][0] = f[n][1] = p.scale_log2;
       } else {
@@ -382,6 +408,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
         e = max(-90, min(e, 110));
         const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+        const float turn = p.negate ? -up : up;
         const float down = __uint_as_float((uint32_t)(127 + 10 + e) << 23) * p.scale_log2;  // 2^20 / up
         float mine = 0.f;  // sum of group t
 #pragma unroll
@@ -391,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = Elem<T>::unpack2(ws[i]);
-            const uint32_t h2 = Elem<__half>::pack2(v.x * up, v.y * up);
+            const uint32_t h2 = Elem<__half>::pack2(v.x * turn, v.y * turn);
             const float2 r = Elem<__half>::unpack2(h2);
             sum += r.x + r.y;
             // codes of the first two dims of four stand 4 bits lower: their q is 2^4 larger
@@ -411,25 +438,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     }
   };
 
-  auto step = [&](int stage) {
+  // One tile.  `edge`: some block has no tokens, or tokens that some row does
+  // not see; without it every score counts.
+  auto step = [&](int stage, uint32_t ok_mask, auto edge_tag) {
+    constexpr bool EDGE = decltype(edge_tag)::value;
     const uint32_t base = my_ring + stage * C::kStageBytes;
-    float s[U][NT][4];
-    bool ok[U];
-    float top[NT][2];
+    auto skipped = [&](int u) {
+      return EDGE && !((ok_mask >> u & 1u) && block_token(cur, u) < max_lim);
+    };
+    float s[U][NT][4], top[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) top[n][0] = top[n][1] = -INFINITY;
     // ---- S^T = K Q^T
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int tok0 = block_token(cur, u);
-      ok[u] = ((__shfl_sync(0xffffffffu, ok_bits, u) >> stage) & 1u) && tok0 < max_lim;
-      if (!ok[u]) continue;
+      if (skipped(u)) continue;
       const uint32_t blk = base + u * C::kBlockBytes;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
       if constexpr (BITS == 16) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[u][n][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
           uint32_t a[4];
@@ -443,24 +472,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             mma16816<M>(s[u][n], a[0], a[1], a[2], a[3], qf[n][k][0], qf[n][k][1]);
         }
       } else {
-        const Kv4 lay(D);
+        constexpr Kv4 lay(D);
         uint32_t w0[NG], w1[NG], q0[NG], q1[NG];  // codes and parameters of tokens g, g + 8
-        lds_words<NG>(blk + (g * 4 + t) * NG * 4, w0);
-        lds_words<NG>(blk + ((g + 8) * 4 + t) * NG * 4, w1);
-        lds_words<NG>(blk + lay.k_params() + g * NG * 4, q0);
-        lds_words<NG>(blk + lay.k_params() + (g + 8) * NG * 4, q1);
+        lds_words<NG>(blk + lane * (NG * 4), w0);
+        lds_words<NG>(blk + (32 + lane) * (NG * 4), w1);
+        lds_words<NG>(blk + lay.k_params() + g * (NG * 4), q0);
+        lds_words<NG>(blk + lay.k_params() + (g + 8) * (NG * 4), q1);
         uint32_t p0 = 0, p1 = 0;  // parameters of group t
         if (t < NG) {
           p0 = lds32(blk + lay.k_params() + (g * NG + t) * 4);
           p1 = lds32(blk + lay.k_params() + ((g + 8) * NG + t) * 4);
         }
-        float c[NT][4];
+        float c[4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-          mma16816<M>(c[n], p0, p1, p0, p1, qsum[n][0], qsum[n][1]);
+          mma16816_zero<M>(c, p0, p1, p0, p1, qsum[n][0], qsum[n][1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[u][n][i] = c[n][i] * 0x1p-14f;
+          for (int i = 0; i < 4; ++i) s[u][n][i] = c[i] * 0x1p-14f;
         }
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -468,50 +496,46 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           const float s0 = low_half(q0[grp]), s1 = low_half(q1[grp]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-            mma16816<M>(c[n], w0[grp] & 0x000F000Fu, w1[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
-                        w1[grp] & 0x00F000F0u, qf[n][2 * grp][0], qf[n][2 * grp][1]);
-            mma16816<M>(c[n], x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u,
-                        x1 & 0x00F000F0u, qf[n][2 * grp + 1][0], qf[n][2 * grp + 1][1]);
-            s[u][n][0] = fmaf(s0, c[n][0], s[u][n][0]);
-            s[u][n][1] = fmaf(s0, c[n][1], s[u][n][1]);
-            s[u][n][2] = fmaf(s1, c[n][2], s[u][n][2]);
-            s[u][n][3] = fmaf(s1, c[n][3], s[u][n][3]);
+            mma16816_zero<M>(c, w0[grp] & 0x000F000Fu, w1[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
+                             w1[grp] & 0x00F000F0u, qf[n][2 * grp][0], qf[n][2 * grp][1]);
+            mma16816<M>(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u,
+                        qf[n][2 * grp + 1][0], qf[n][2 * grp + 1][1]);
+            s[u][n][0] = fmaf(s0, c[0], s[u][n][0]);
+            s[u][n][1] = fmaf(s0, c[1], s[u][n][1]);
+            s[u][n][2] = fmaf(s1, c[2], s[u][n][2]);
+            s[u][n][3] = fmaf(s1, c[3], s[u][n][3]);
           }
         }
       }
-      // ---- log2 domain, mask, maximum
-      const bool partial = tok0 + kBlockTokens > min_lim;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        if constexpr (EDGE) {
+          const int tok0 = block_token(cur, u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[u][n][i] *= f[n][i & 1];
-          if (partial && tok0 + g + (i >> 1) * 8 >= lim[n][i & 1]) s[u][n][i] = -INFINITY;
+          for (int i = 0; i < 4; ++i)
+            if (tok0 + g + (i >> 1) * 8 >= lim[n][i & 1]) s[u][n][i] = -INFINITY;
         }
         top[n][0] = fmaxf(top[n][0], fmaxf(s[u][n][0], s[u][n][2]));
         top[n][1] = fmaxf(top[n][1], fmaxf(s[u][n][1], s[u][n][3]));
       }
     }
-    bool any = false;
-#pragma unroll
-    for (int u = 0; u < U; ++u) any |= ok[u];
-    if (!any) return;
     // ---- running maximum; O and the sum follow it
-    float base_m[NT][2];
+    bool above = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + kSlack;
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2)
-          top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], d));
-        const float now = fmaxf(m[n][i], top[n][i]);
-        const float safe = now == -INFINITY ? 0.f : now;  // no token seen yet
-        const float keep = ex2(m[n][i] - safe);
-        m[n][i] = now;
-        base_m[n][i] = safe;
-        if (keep != 1.f) {
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2)
+            top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], d));
+          const float now = fmaxf(mf[n][i], top[n][i] * f[n][i]);
+          const float keep = now == -INFINITY ? 1.f : ex2(mf[n][i] - now);
+          mf[n][i] = now;
           l[n][i] *= keep;
           om[n][i] *= keep;
           om[n][i + 2] *= keep;
@@ -521,19 +545,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             o[k][n][i + 2] *= keep;
           }
         }
-      }
+    }
+    float from[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)  // no token seen yet: every probability is 0
+        from[n][i] = EDGE && mf[n][i] == -INFINITY ? 0.f : mf[n][i];
     // ---- P^T, O^T += V^T P^T
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (!ok[u]) continue;
-      const int tok0 = block_token(cur, u);
+      if (skipped(u)) continue;
       const uint32_t blk = base + u * C::kBlockBytes;
       uint32_t pf[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = ex2(s[u][n][i] - base_m[n][i & 1]);
+        for (int i = 0; i < 4; ++i) e[i] = ex2(fmaf(s[u][n][i], f[n][i & 1], -from[n][i & 1]));
         l[n][0] += e[0] + e[2];
         l[n][1] += e[1] + e[3];
         pf[n][0] = transpose8x8(Elem<M>::pack2(e[0], e[1]));
@@ -543,20 +572,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       // so in a block that some row sees in part, the values behind the limit
       // are set to zero, and where the rows' limits differ, each query token's
       // rows are multiplied apart (`apart`) and the other columns kept.
-      const bool partial = tok0 + kBlockTokens > min_lim;
-      const int passes = partial && p.causal ? qp_last - qp_first + 1 : 1;
+      const int tok0 = block_token(cur, u);
+      const bool apart = EDGE && p.causal && qp_last > qp_first && tok0 + kBlockTokens > min_lim;
+      const int passes = apart ? qp_last - qp_first + 1 : 1;
 #pragma unroll 1
       for (int pass = 0; pass < passes; ++pass) {
         uint32_t keep0 = ~0u, keep1 = ~0u;  // token pairs (2t, 2t + 1), (2t + 8, 2t + 9)
-        const bool apart = passes > 1;
         bool mine[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) mine[n][i] = col_q[n][i] == qp_first + pass;
         auto add = [&](float (&acc)[4], int n, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                        uint32_t b0, uint32_t b1) {
-          if (!apart) {
+          if constexpr (!EDGE) {
             mma16816<M>(acc, a0, a1, a2, a3, b0, b1);
           } else {
             float c[4] = {acc[0], acc[1], acc[2], acc[3]};
@@ -565,11 +590,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             for (int i = 0; i < 4; ++i) acc[i] = mine[n][i & 1] ? c[i] : acc[i];
           }
         };
-        if (partial) {
+        if constexpr (EDGE) {
           const int to = limit_of(qp_first + pass) - tok0;
-          if (to <= 0) continue;
+          if (apart && to <= 0) continue;
           keep0 = (2 * t < to ? 0xFFFFu : 0u) | (2 * t + 1 < to ? 0xFFFF0000u : 0u);
           keep1 = (2 * t + 8 < to ? 0xFFFFu : 0u) | (2 * t + 9 < to ? 0xFFFF0000u : 0u);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) mine[n][i] = !apart || col_q[n][i] == qp_first + pass;
         }
         if constexpr (BITS == 16) {
 #pragma unroll
@@ -581,34 +610,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const int sw = WB == 128 ? (r & 7) : WB == 64 ? (r >> 1 & 3) : (r >> 2 & 1);
             ldsm4_trans(blk + 32 * D + (ch / (WB / 16)) * (16 * WB) + r * WB +
                             ((ch % (WB / 16)) ^ sw) * 16, a);
-            if (partial) {
+            if constexpr (EDGE) {
               a[0] &= keep0;
               a[1] &= keep0;
               a[2] &= keep1;
               a[3] &= keep1;
             }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-              add(o[k][n], n, a[0], a[1], a[2], a[3], pf[n][0], pf[n][1]);
+            for (int n = 0; n < NT; ++n) add(o[k][n], n, a[0], a[1], a[2], a[3], pf[n][0], pf[n][1]);
           }
         } else {
-          const Kv4 lay(D);
+          constexpr Kv4 lay(D);
           uint32_t w0[NG], w1[NG];
-          lds_words<NG>(blk + lay.v_codes() + lane * NG * 4, w0);
-          lds_words<NG>(blk + lay.v_codes() + (32 + lane) * NG * 4, w1);
+          lds_words<NG>(blk + lay.v_codes() + lane * (NG * 4), w0);
+          lds_words<NG>(blk + lay.v_codes() + (32 + lane) * (NG * 4), w1);
           uint2 mm = make_uint2(0, 0);
-          if (g < NG) mm = lds64(blk + lay.v_params() + 32 * NG + (g * 4 + t) * 8);
-          mm.x &= keep0;
-          mm.y &= keep1;
+          if (g < NG) mm = lds64(blk + lay.v_params() + 32 * NG + lane * 8);
+          if constexpr (EDGE) {
+            mm.x &= keep0;
+            mm.y &= keep1;
+          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) add(om[n], n, mm.x, 0u, mm.y, 0u, pf[n][0], pf[n][1]);
 #pragma unroll
           for (int grp = 0; grp < NG; ++grp) {
-            const uint2 sc = lds64(blk + lay.v_params() + (grp * 4 + t) * 8);
+            uint2 sc = lds64(blk + lay.v_params() + (grp * 4 + t) * 8);
+            if constexpr (EDGE) {
+              sc.x &= keep0;
+              sc.y &= keep1;
+            }
             const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint32_t b0 = hmul2(pf[n][0], sc.x & keep0), b1 = hmul2(pf[n][1], sc.y & keep1);
+              const uint32_t b0 = hmul2(pf[n][0], sc.x), b1 = hmul2(pf[n][1], sc.y);
               add(o[2 * grp][n], n, w0[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
                   w1[grp] & 0x000F000Fu, w1[grp] & 0x00F000F0u, b0, b1);
               add(o[2 * grp + 1][n], n, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
@@ -623,14 +657,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   // The warps' results of a segment, joined; `first`: this share holds the
   // segment's first tile, `last`: its last.
   auto end_segment = [&](bool first, bool last) {
-    const int h = cur.hr / p.row_blocks, rb = cur.hr % p.row_blocks, rows = p.Sq * p.group;
+    const int h = cur.h, rb = cur.rb, rows = p.Sq * p.group;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-        if (g == 0) sh.join_ml[warp][2 * t + i] = make_float2(m[n][i], l[n][i]);
+        if (g == 0) sh.join_ml[warp][2 * t + i] = make_float2(mf[n][i], l[n][i]);
         float* dst = join + (warp * 8 + 2 * t + i) * C::kJoinStride;
         if constexpr (BITS == 16) {
 #pragma unroll
@@ -700,12 +734,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if (fresh) {
       first = cur.tt == 0;
       begin_segment();
-      if (first && tid == 0 && cur.hr == 0 && p.kv.bad_length(p.lengths[cur.b])) p.kv.report(kStatusPage);
+      if (first && tid == 0 && cur.h == 0 && cur.rb == 0 && p.kv.bad_length(p.lengths[cur.b])) p.kv.report(kStatusPage);
     }
     const bool here = mbar_wait(my_bars + stage * 8, phase, wait);
     if (here) {
       in_flight &= ~(1u << stage);
-      step(stage);
+      const uint32_t ok = __ballot_sync(0xffffffffu, ok_bits >> stage & 1u) & ((1u << U) - 1u);
+      if (ok == (1u << U) - 1u && block_token(cur, U) <= min_lim)
+        step(stage, ok, std::false_type{});
+      else if (ok != 0)
+        step(stage, ok, std::true_type{});
     }
     __syncwarp();
     if (here) {
@@ -831,13 +869,15 @@ int launch_decode_t(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtens
 
 int tile_tokens(int D, int bits) { return (bits == 16 && D == 128) ? 64 : 128; }
 
+int ctas_per_sm(int D, int bits, int nt) { return bits == 16 || nt > 1 ? 2 : 3; }
+
 struct Plan {
   int nt, row_blocks, grid;
   bool split;
 };
 
-// Rows of 8 (one column block of the matrix instructions) or 16; CTAs for two
-// per SM, fewer when the tables have room for fewer tiles.
+// Rows of 8 (one column block of the matrix instructions) or 16; as many CTAs as
+// the SMs hold, fewer when the tables have room for fewer tiles.
 Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen, int nheads) {
   Plan pl;
   const long long rows = (long long)seqlen * (nheads / c->nheads_kv);
@@ -846,7 +886,7 @@ Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen,
   const int tile = tile_tokens(c->head_dim, c->bits);
   const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
   const long long tiles = (long long)batch * c->nheads_kv * pl.row_blocks * per_seg;
-  const long long most = (long long)sm_count() * kCtasPerSm;
+  const long long most = (long long)sm_count() * ctas_per_sm(c->head_dim, c->bits, pl.nt);
   pl.grid = (int)(tiles < most ? tiles : most);
   pl.split = per_seg > 1;
   return pl;
@@ -916,8 +956,10 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   p.group = nheads / cache->nheads_kv;
   p.row_blocks = pl.row_blocks;
   p.causal = causal ? 1 : 0;
+  while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
   p.grid = pl.grid;
-  p.scale_log2 = sm_scale * 1.44269504088896341f;
+  p.negate = sm_scale < 0.f;
+  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);
   p.timeout_ns = wait_timeout_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return cache->dtype == FA_DTYPE_BF16

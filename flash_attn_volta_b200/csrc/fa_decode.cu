@@ -51,6 +51,9 @@ constexpr float kSlack = 2.f;
 constexpr float kLn2 = 0.69314718055994531f;
 
 // Per-instantiation constants.
+// Column blocks of 8 query rows that a CTA's registers hold.
+constexpr int max_nt(int D) { return D <= 64 ? 4 : 2; }
+
 template <int D, int BITS>
 struct Cfg {
   static constexpr int kU = (BITS == 16 && D == 128) ? 1 : 2;  // blocks of a warp per tile
@@ -77,7 +80,7 @@ struct DecodeParams {
   const int* starts;   // (B) or null: length - Sq
   float* part_o;       // (2 * grid, ROWS, D)
   float2* part_ml;     // (2 * grid, ROWS): maximum (log2 domain), sum
-  int B, Sq, H, group, row_blocks, causal, page_shift;
+  int B, Sq, H, group, row_blocks, causal, page_shift, bf16;
   int grid, negate;
   float scale_log2;  // |scale| log2 e, above 0; `negate`: the scale is negative (q's sign changes)
   unsigned long long timeout_ns;
@@ -217,12 +220,33 @@ __device__ __forceinline__ void locate(const DecodeParams& p, int per_tile, long
   __syncthreads();
 }
 
+// 8 dims of a finished row: out = x / sum, and the row's log-sum-exp.
+template <int D>
+__device__ __forceinline__ void write_row(const DecodeParams& p, int b, int h, int rr, int d,
+                                          float top, float sum, const float (&x)[8]) {
+  const int qpos = rr / p.group, hq = h * p.group + (rr - qpos * p.group);
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    w[j] = p.bf16 ? Elem<__nv_bfloat16>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv)
+                  : Elem<__half>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
+  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
+                            (((long long)b * p.Sq + qpos) * p.H + hq) * D + d) =
+      make_uint4(w[0], w[1], w[2], w[3]);
+  if (p.lse && d == 0)
+    p.lse[((long long)b * p.H + hq) * p.Sq + qpos] =
+        sum == 0.f ? INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// T: the element type of 16-bit pages; 4-bit codes are multiplied as fp16
+// whatever q's type is.
 template <typename T, int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
     fa_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
   using C = Cfg<D, BITS>;
-  using M = typename std::conditional<BITS == 4, __half, T>::type;  // operand type
+  using M = T;  // operand type
   constexpr int U = C::kU, NS = C::kStages, ROWS = 8 * NT, NG = BITS == 4 ? C::kGroups : 1;
   constexpr int KSTEPS = D / 16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -372,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
       const int rr = rb * ROWS + n * 8 + g;
       const bool there = rr < rows;
       const int qpos = there ? rr / p.group : 0, hq = h * p.group + (there ? rr % p.group : 0);
-      const T* src = static_cast<const T*>(p.q) + (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D;
       if constexpr (BITS == 16) {
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
@@ -399,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
           const uint32_t ws[4] = {raw[grp].x, raw[grp].y, raw[grp].z, raw[grp].w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = Elem<T>::unpack2(ws[i]);
+            const float2 v = p.bf16 ? Elem<__nv_bfloat16>::unpack2(ws[i]) : Elem<__half>::unpack2(ws[i]);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
         }
@@ -417,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = Elem<T>::unpack2(ws[i]);
+            const float2 v = p.bf16 ? Elem<__nv_bfloat16>::unpack2(ws[i]) : Elem<__half>::unpack2(ws[i]);
             const uint32_t h2 = Elem<__half>::pack2(v.x * turn, v.y * turn);
             const float2 r = Elem<__half>::unpack2(h2);
             sum += r.x + r.y;
@@ -568,12 +592,25 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
         pf[n][0] = transpose8x8(Elem<M>::pack2(e[0], e[1]));
         pf[n][1] = transpose8x8(Elem<M>::pack2(e[2], e[3]));
       }
-      // Values that a row does not see must not reach its sum even as 0 x NaN,
-      // so in a block that some row sees in part, the values behind the limit
-      // are set to zero, and where the rows' limits differ, each query token's
-      // rows are multiplied apart (`apart`) and the other columns kept.
+      // Values that a row does not see must not reach its sum even as 0 x NaN.
+      // Those that no row of the block sees are set to zero; where the rows'
+      // limits differ and some value is not finite, each query token's rows are
+      // multiplied apart and the other columns kept.
       const int tok0 = block_token(cur, u);
-      const bool apart = EDGE && p.causal && qp_last > qp_first && tok0 + kBlockTokens > min_lim;
+      bool apart = false;
+      if constexpr (EDGE) {
+        if (p.causal && qp_last > qp_first && tok0 + kBlockTokens > min_lim) {
+          constexpr uint32_t EXP = Elem<M>::kIdescAB == 0 ? 0x7C00u : 0x7F80u;
+          // the block's values (4-bit: V's parameters), two to a word
+          constexpr int WORDS = BITS == 16 ? 8 * D : 16 * NG;
+          const uint32_t at = blk + (BITS == 16 ? 32 * D : Kv4(D).v_params());
+          for (int i = lane; i < WORDS; i += 32) {
+            const uint32_t w = lds32(at + 4 * i);
+            apart |= (w & EXP) == EXP || (w >> 16 & EXP) == EXP;
+          }
+          apart = __any_sync(0xffffffffu, apart);
+        }
+      }
       const int passes = apart ? qp_last - qp_first + 1 : 1;
 #pragma unroll 1
       for (int pass = 0; pass < passes; ++pass) {
@@ -591,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
           }
         };
         if constexpr (EDGE) {
-          const int to = limit_of(qp_first + pass) - tok0;
+          const int to = (apart ? limit_of(qp_first + pass) : max_lim) - tok0;
           if (apart && to <= 0) continue;
           keep0 = (2 * t < to ? 0xFFFFu : 0u) | (2 * t + 1 < to ? 0xFFFF0000u : 0u);
           keep1 = (2 * t + 8 < to ? 0xFFFFu : 0u) | (2 * t + 9 < to ? 0xFFFF0000u : 0u);
@@ -702,17 +739,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
         }
         if (rr >= rows) continue;
         if (first && last) {
-          const int qpos = rr / p.group, hq = h * p.group + rr % p.group;
-          const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = Elem<T>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
-                                    (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D + d) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-          if (p.lse && d == 0)
-            p.lse[((long long)cur.b * p.H + hq) * p.Sq + qpos] =
-                sum == 0.f ? INFINITY : (top + log2f(sum)) * kLn2;
+          write_row<D>(p, cur.b, h, rr, d, top, sum, x);
         } else {
           const long long slot = (2LL * blockIdx.x + (first ? 1 : 0)) * ROWS + n * 8 + r;
           float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + d);
@@ -766,63 +793,58 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
 }
 
 // Joins the partial results of the segments that cross shares, in the order of
-// the shares.  One CTA per segment; a thread holds 8 dims of a row.
-template <typename T, int D, int BITS, int NT>
+// the shares.  blockIdx.x is a border between two shares; the border that a
+// segment crosses first does its work, two rows to a CTA (blockIdx.y).  A thread
+// holds 8 dims of a row and takes every P-th share, all loads independent.
+template <int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeParams p) {
   using C = Cfg<D, BITS>;
-  constexpr int ROWS = 8 * NT, PER_ROW = D / 8;
+  constexpr int ROWS = 8 * NT, PER_ROW = D / 8, P = kThreads / 2 / PER_ROW;
   __shared__ long long box[3], warp_sum[kWarps];
-  const int segs = p.kv.heads * p.row_blocks;
-  const int b = blockIdx.x / segs, hr = blockIdx.x % segs;
-  const int h = hr / p.row_blocks, rb = hr % p.row_blocks;
-  locate<C::kTile>(p, segs, box, warp_sum, 0, 1, b);
-  const long long total = box[0];
-  const int nt = tiles_of<C::kTile>(p.kv.clamp_length(p.lengths[b]));
+  __shared__ float4 part_x[2][P][D / 4];
+  __shared__ float2 part_ml[2][P];
+  const int segs = p.kv.heads * p.row_blocks, border = blockIdx.x + 1;
+  locate<C::kTile>(p, segs, box, warp_sum, border, p.grid, -1);
+  const long long total = box[0], at = total * border / p.grid, in = at - box[2];
+  const int b = (int)box[1], nt = tiles_of<C::kTile>(p.kv.clamp_length(p.lengths[b]));
+  const int hr = (int)(in / nt);
   const long long t0 = box[2] + (long long)hr * nt, t1 = t0 + nt - 1;
-  const int c0 = (int)(((t0 + 1) * p.grid - 1) / total), c1 = (int)(((t1 + 1) * p.grid - 1) / total);
   griddep_wait();
   griddep_launch_dependents();
-  if (c0 == c1) return;
-  const int rows = p.Sq * p.group;
-  for (int i = threadIdx.x; i < ROWS * PER_ROW; i += kThreads) {
-    const int r = i / PER_ROW, d = i % PER_ROW * 8, rr = rb * ROWS + r;
-    if (rr >= rows) break;
-    auto slot = [&](int c) { return (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r; };
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c)
-      if (total * (c + 1) / p.grid > total * c / p.grid) top = fmaxf(top, p.part_ml[slot(c)].x);
-    const float safe = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[8] = {};
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
-      const float2 ml = p.part_ml[slot(c)];
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot(c) * D + d);
-      const float4 u = src[0], v = src[1];
-      const float e = ex2(ml.x - safe);
-      sum = fmaf(e, ml.y, sum);
-      x[0] = fmaf(e, u.x, x[0]);
-      x[1] = fmaf(e, u.y, x[1]);
-      x[2] = fmaf(e, u.z, x[2]);
-      x[3] = fmaf(e, u.w, x[3]);
-      x[4] = fmaf(e, v.x, x[4]);
-      x[5] = fmaf(e, v.y, x[5]);
-      x[6] = fmaf(e, v.z, x[6]);
-      x[7] = fmaf(e, v.w, x[7]);
-    }
-    const int qpos = rr / p.group, hq = h * p.group + rr % p.group;
-    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
-    uint32_t w[4];
+  if (at == t0 || total * (border - 1) / p.grid > t0) return;
+  const int c0 = border - 1, c1 = (int)(((t1 + 1) * p.grid - 1) / total);
+  const int h = hr / p.row_blocks, rb = hr % p.row_blocks, rows = p.Sq * p.group;
+  const int half = threadIdx.x / (kThreads / 2), i = threadIdx.x % (kThreads / 2);
+  const int pg = i / PER_ROW, d = i % PER_ROW * 8, r = blockIdx.y * 2 + half, rr = rb * ROWS + r;
+  float top = -INFINITY, sum = 0.f, x[8] = {};
+  auto take = [&](float2 ml, const float (&v)[8]) {
+    const float now = fmaxf(top, ml.x);
+    const float safe = now == -INFINITY ? 0.f : now;
+    const float old = ex2(top - safe), e = ex2(ml.x - safe);
+    top = now;
+    sum = fmaf(e, ml.y, sum * old);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = Elem<T>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) +
-                              (((long long)b * p.Sq + qpos) * p.H + hq) * D + d) =
-        make_uint4(w[0], w[1], w[2], w[3]);
-    if (p.lse && d == 0)
-      p.lse[((long long)b * p.H + hq) * p.Sq + qpos] =
-          sum == 0.f ? INFINITY : (top + log2f(sum)) * kLn2;
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(e, v[j], x[j] * old);
+  };
+#pragma unroll 4
+  for (int c = c0 + pg; c <= c1; c += P) {
+    if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
+    const long long slot = (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r;
+    const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
+    const float4 u = src[0], v = src[1];
+    take(p.part_ml[slot], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
   }
+  part_x[half][pg][d / 4] = make_float4(x[0], x[1], x[2], x[3]);
+  part_x[half][pg][d / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+  if (d == 0) part_ml[half][pg] = make_float2(top, sum);
+  __syncthreads();
+  if (pg != 0 || rr >= rows) return;
+#pragma unroll
+  for (int k = 1; k < P; ++k) {
+    const float4 u = part_x[half][k][d / 4], v = part_x[half][k][d / 4 + 1];
+    take(part_ml[half][k], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
+  }
+  write_row<D>(p, b, h, rr, d, top, sum, x);
 }
 
 template <typename T, int D, int BITS, int NT>
@@ -836,34 +858,44 @@ int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
   if (launch_pdl(kernel, dim3(p.grid), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
     return FA_ERR_LAUNCH;
   if (!split) return FA_OK;
-  const long long segs = (long long)p.B * p.kv.heads * p.row_blocks;
-  return launch_pdl(fa_decode_merge_kernel<T, D, BITS, NT>, dim3((unsigned)segs), dim3(kThreads), 0,
+  return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid - 1, 4 * NT), dim3(kThreads), 0,
                     st, p) == cudaSuccess
              ? FA_OK
              : FA_ERR_LAUNCH;
 }
 
-template <typename T, int D>
+template <typename T, int D, int BITS>
+int launch_decode_nt(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
+                     bool split, cudaStream_t st) {
+  switch (nt) {
+    case 1: return launch_decode<T, D, BITS, 1>(p, tk, tv, split, st);
+    case 2: return launch_decode<T, D, BITS, 2>(p, tk, tv, split, st);
+  }
+  if constexpr (max_nt(D) > 2) {
+    if (nt == 3) return launch_decode<T, D, BITS, 3>(p, tk, tv, split, st);
+    return launch_decode<T, D, BITS, 4>(p, tk, tv, split, st);
+  }
+  return FA_ERR_ARG;
+}
+
+template <int D>
 int launch_decode_d(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
                     bool split, cudaStream_t st) {
   if (p.kv.bits == 4) {
-    if constexpr (D >= 32)
-      return nt == 1 ? launch_decode<T, D, 4, 1>(p, tk, tv, split, st)
-                     : launch_decode<T, D, 4, 2>(p, tk, tv, split, st);
+    if constexpr (D >= 32) return launch_decode_nt<__half, D, 4>(p, nt, tk, tv, split, st);
     return FA_ERR_ARG;
   }
-  return nt == 1 ? launch_decode<T, D, 16, 1>(p, tk, tv, split, st)
-                 : launch_decode<T, D, 16, 2>(p, tk, tv, split, st);
+  return p.bf16 ? launch_decode_nt<__nv_bfloat16, D, 16>(p, nt, tk, tv, split, st)
+                : launch_decode_nt<__half, D, 16>(p, nt, tk, tv, split, st);
 }
 
-template <typename T>
-int launch_decode_t(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
-                    bool split, cudaStream_t st) {
+int launch_decode_any(DecodeParams& p, int nt, const CUtensorMap& tk, const CUtensorMap& tv,
+                      bool split, cudaStream_t st) {
   switch (p.kv.D) {
-    case 16: return launch_decode_d<T, 16>(p, nt, tk, tv, split, st);
-    case 32: return launch_decode_d<T, 32>(p, nt, tk, tv, split, st);
-    case 64: return launch_decode_d<T, 64>(p, nt, tk, tv, split, st);
-    default: return launch_decode_d<T, 128>(p, nt, tk, tv, split, st);
+    case 16: return launch_decode_d<16>(p, nt, tk, tv, split, st);
+    case 32: return launch_decode_d<32>(p, nt, tk, tv, split, st);
+    case 64: return launch_decode_d<64>(p, nt, tk, tv, split, st);
+    default: return launch_decode_d<128>(p, nt, tk, tv, split, st);
   }
 }
 
@@ -876,19 +908,20 @@ struct Plan {
   bool split;
 };
 
-// Rows of 8 (one column block of the matrix instructions) or 16; as many CTAs as
+// Query rows in as few row blocks as the registers allow; as many CTAs as
 // the SMs hold, fewer when the tables have room for fewer tiles.
 Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen, int nheads) {
   Plan pl;
   const long long rows = (long long)seqlen * (nheads / c->nheads_kv);
-  pl.nt = rows <= 8 ? 1 : 2;
-  pl.row_blocks = (int)((rows + 8 * pl.nt - 1) / (8 * pl.nt));
+  const int most_rows = 8 * max_nt(c->head_dim);
+  pl.row_blocks = (int)((rows + most_rows - 1) / most_rows);
+  pl.nt = (int)((rows + 8LL * pl.row_blocks - 1) / (8LL * pl.row_blocks));
   const int tile = tile_tokens(c->head_dim, c->bits);
   const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
   const long long tiles = (long long)batch * c->nheads_kv * pl.row_blocks * per_seg;
   const long long most = (long long)sm_count() * ctas_per_sm(c->head_dim, c->bits, pl.nt);
   pl.grid = (int)(tiles < most ? tiles : most);
-  pl.split = per_seg > 1;
+  pl.split = per_seg > 1 && pl.grid > 1;
   return pl;
 }
 
@@ -959,10 +992,8 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
   p.grid = pl.grid;
   p.negate = sm_scale < 0.f;
+  p.bf16 = cache->dtype == FA_DTYPE_BF16;
   p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);
   p.timeout_ns = wait_timeout_ns();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache->dtype == FA_DTYPE_BF16
-             ? launch_decode_t<__nv_bfloat16>(p, pl.nt, tk, tv, pl.split, st)
-             : launch_decode_t<__half>(p, pl.nt, tk, tv, pl.split, st);
+  return launch_decode_any(p, pl.nt, tk, tv, pl.split, static_cast<cudaStream_t>(stream));
 }

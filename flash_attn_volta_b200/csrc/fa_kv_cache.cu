@@ -59,13 +59,12 @@ struct AppendPart {
 
 struct AppendParams {
   KvView kv;
-  AppendPart q, k, v;
+  AppendPart part[3];  // q, k, v
   void* q_out;
   const int* starts;
-  const int* counts;  // null: every token is new
+  const int* counts;       // null: every token is new
   const double* inv_freq;  // null: no rotation
-  long long tokens;
-  int S, half, per_cta;
+  int S, half, per_cta, per_seq, page_shift, chunk_shift;
   float magnitude;
 };
 
@@ -82,8 +81,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Rounds the 32 values of a group, 8 in each of 4 neighbouring lanes, to codes.
 // Returns (s, m); a group with a NaN reads back as NaN, infinities as the
-// largest fp16.  The division is correctly rounded, so a code is the definition's
-// also where (x - m) / s is half a step.
+// largest fp16.  The quotient (x - m) / s is the correctly rounded one
+// (Markstein: with r = 1/s rounded, q = d r, then q + r (d - q s) in fused
+// steps), so a code is the definition's also where it is half a step; adding
+// 1.5 2^23 rounds it to a whole number, ties to even, in the sum's low bits.
 __device__ __forceinline__ uint32_t quantise(float (&x)[8], uint32_t (&code)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = max_nan(-65504.f, min_nan(x[i], 65504.f));
@@ -101,184 +102,233 @@ __device__ __forceinline__ uint32_t quantise(float (&x)[8], uint32_t (&code)[8])
   const __half m = __float2half_rd(lo);
   const float mf = __half2float(m);
   const __half s = __float2half_ru(__fdiv_rn(hi - mf, 15.f));
-  const float sf = __half2float(s);
+  const float sf = __half2float(s), r = __frcp_rn(sf);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float c = rintf(__fdiv_rn(x[i] - mf, sf));  // 0 / 0 and NaN become 0
-    code[i] = (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
+    const float d = x[i] - mf, q = d * r;
+    const float c = fmaf(fmaf(-q, sf, d), r, q);  // 0 / 0 and NaN become 0 below
+    code[i] = __float_as_uint(fminf(fmaxf(c, 0.f), 15.f) + 12582912.f) & 15u;
   }
   return (uint32_t)__half_as_ushort(s) | ((uint32_t)__half_as_ushort(m) << 16);
 }
 
-// 8 consecutive dims of a row as fp32; VEC elements per load.
-template <typename T, int VEC>
-__device__ __forceinline__ void load8(const T* src, float (&x)[8]) {
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 8; i += VEC) {
-    const Pack16<VEC> p = *reinterpret_cast<const Pack16<VEC>*>(src + i);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) x[i + j] = Elem<T>::value(p.v[j]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem<T>::unpack2(v[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
   }
 }
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]),
+                    Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
+}
 
-// Rotates the 8 dims e.. of a row (the thread's own values in x).
-template <typename T, int VEC, bool INTER>
+// Where the angle of pair i stands: the 8 angles of a thread's dims are `half / 8`
+// apart, so that neighbouring threads read neighbouring words (WIDE: half % 8
+// == 0); interleaved pairs, of which a thread has 4, likewise.
+template <bool INTER, bool WIDE>
+__device__ __forceinline__ int angle_at(int i, int half) {
+  constexpr int N = INTER ? 4 : 8;
+  return WIDE ? i % N * (half / N) + i / N : i;
+}
+
+// Rotates the 8 dims e.. of a row (the thread's own values in x, WIDE: those of
+// the partner dims in y).
+template <typename T, bool INTER, bool WIDE>
 __device__ __forceinline__ void rotate8(const T* row, int e, int half, const float2* cs,
-                                        float (&x)[8]) {
-  if (e >= 2 * half) return;
-  if (INTER) {
+                                        float (&x)[8], float (&y)[8]) {
+  if constexpr (INTER) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      if (e + i < 2 * half) {
-        const float2 w = cs[(e + i) / 2];
+      if (WIDE || e + i < 2 * half) {
+        const float2 w = cs[angle_at<INTER, WIDE>((e + i) / 2, half)];
         const float a = x[i], b = x[i + 1];
         x[i] = a * w.x - b * w.y;
         x[i + 1] = b * w.x + a * w.y;
       }
     }
-    return;
-  }
-  float y[8];
-  if (VEC == 8 && half % 8 == 0) {
-    load8<T, VEC>(row + (e < half ? e + half : e - half), y);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int d = e + i;
-      y[i] = d < 2 * half
-                 ? Elem<T>::value(reinterpret_cast<const uint16_t*>(row)[d < half ? d + half : d - half])
-                 : 0.f;
+      if (!WIDE) {
+        if (d >= 2 * half) break;
+        y[i] = Elem<T>::value(reinterpret_cast<const uint16_t*>(row)[d < half ? d + half : d - half]);
+      }
+      const bool first = d < half;
+      const float2 w = cs[angle_at<INTER, WIDE>(first ? d : d - half, half)];
+      x[i] = x[i] * w.x + (first ? -y[i] : y[i]) * w.y;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = e + i;
-    if (d < half) {
-      const float2 w = cs[d];
-      x[i] = x[i] * w.x - y[i] * w.y;
-    } else if (d < 2 * half) {
-      const float2 w = cs[d - half];
-      x[i] = x[i] * w.x + y[i] * w.y;
-    }
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ Pack16<8> pack8(const float (&x)[8]) {
-  Pack16<8> p;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) p.v[i] = Elem<T>::bits(x[i]);
-  return p;
 }
 
 // New tokens into the cache.  Bound by HBM for prompts (every input is read
 // once, every output written once) and by latency for single tokens: one
 // launch does the rotation of q and k, the page lookup and both writes.
-// A CTA takes whole tokens, whose cosines and sines it makes once for all
-// heads; an item is 8 consecutive dims of a head of q, k or v (the half layout
-// reads the partner dims a second time, from L1).  The item ranges of q, k and
-// v start at multiples of 32, so a warp works on one of them, and the 4 lanes
-// that hold a group of 32 dims reduce its minimum and maximum by shuffles.
-template <typename T, int VEC, bool INTER, int BITS>
-__global__ void __launch_bounds__(kThreads) fa_kv_append_kernel(const AppendParams p) {
+// A CTA takes whole tokens of one sequence; it makes their cosines and sines
+// and finds their places in the cache once for all heads.  The rows are the
+// heads of q, k and v of each token, D/8 threads to a row; a thread holds 8
+// consecutive dims (the half layout reads the partner dims a second time, from
+// L1) and steps down the rows with additions alone.  The 4 lanes that hold a
+// group of 32 dims reduce its minimum and maximum by shuffles.
+// WIDE: 16-byte loads, and rotated dims that end at a thread's border.
+template <typename T, bool INTER, int BITS, bool WIDE>
+__global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendParams p) {
   extern __shared__ float2 cs[];
   griddep_wait();
   griddep_launch_dependents();
   const KvView& kv = p.kv;
-  const int D = kv.D, chunks = D / 8;
-  const long long tok0 = (long long)blockIdx.x * p.per_cta;
-  const int ntok = (int)min((long long)p.per_cta, p.tokens - tok0);
-  const int nq = ntok * p.q.heads * chunks, nk = ntok * kv.heads * chunks;
-  const int k0 = (nq + 31) & ~31, v0 = k0 + ((nk + 31) & ~31), end = v0 + ((nk + 31) & ~31);
-  if (p.half > 0) {
-    for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
-      const long long t = tok0 + i / p.half;
-      const long long pos = p.starts[t / p.S] + t % p.S;
-      cs[i] = rotary_cos_sin((double)pos, p.inv_freq[i % p.half], p.magnitude);
+  const int b = blockIdx.x / p.per_seq, s0 = (blockIdx.x - b * p.per_seq) * p.per_cta;
+  const int ntok = min(p.per_cta, p.S - s0);
+  int* places = reinterpret_cast<int*>(cs + p.per_cta * p.half);  // row of head 0, or -1
+  const int hq = p.part[0].heads, hk = kv.heads, heads = hq + 2 * hk;
+  const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), e = c * 8;
+  const int row = threadIdx.x >> p.chunk_shift, step = kThreads >> p.chunk_shift;
+  const int step_tok = step / heads, step_h = step - step_tok * heads;
+  int tok = row / heads, h = row - tok * heads;
+  const bool turning = e < 2 * p.half;
+
+  const long long first = (long long)p.starts[b] + s0;
+  for (int i = threadIdx.x; i < ntok; i += kThreads) {
+    int at = -1;
+    if (p.counts == nullptr || s0 + i < p.counts[b]) {
+      const long long pos = first + i;
+      const int id = kv.page_of(b, pos, p.page_shift);
+      if (id < 0)
+        kv.report(kStatusPage);
+      else
+        at = ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
     }
-    __syncthreads();
+    places[i] = at;
   }
-  for (int it = threadIdx.x; it < end; it += kThreads) {
-    const int part = it < k0 ? 0 : it < v0 ? 1 : 2;  // the same in all lanes of a warp
-    const int i = it - (part == 0 ? 0 : part == 1 ? k0 : v0);
-    const bool there = i < (part == 0 ? nq : nk);
-    const int heads = part == 0 ? p.q.heads : kv.heads;
-    const int c = i % chunks, th = i / chunks, h = th % heads;
-    const int tok = there ? th / heads : 0;
-    const long long t = tok0 + tok;
-    const int b = (int)(t / p.S), s = (int)(t % p.S);
-    const AppendPart& src = part == 0 ? p.q : part == 1 ? p.k : p.v;
-    float x[8] = {};
-    const T* row = static_cast<const T*>(src.in) + b * src.sb + s * src.ss + (there ? h : 0) * src.sh;
-    if (there) {
-      load8<T, VEC>(row + c * 8, x);
-      if (part < 2 && p.half > 0) rotate8<T, VEC, INTER>(row, c * 8, p.half, cs + tok * p.half, x);
-    }
-    if (part == 0) {
-      if (there)
-        *reinterpret_cast<Pack16<8>*>(static_cast<T*>(p.q_out) + (t * heads + h) * D + c * 8) = pack8<T>(x);
-      continue;
-    }
-    const bool is_new = there && (p.counts == nullptr || s < p.counts[b]);
-    const long long pos = (long long)p.starts[b] + s;
-    const int id = is_new ? kv.page_of(b, pos) : -1;
-    if (is_new && id < 0) kv.report(kStatusPage);
-    const int token = (int)(pos & (kv.page - 1));
-    if (BITS == 16) {
-      if (id >= 0)
-        *reinterpret_cast<Pack16<8>*>((part == 1 ? kv.k : kv.v) + kv.row16(id, h, token) + c * 16) =
-            pack8<T>(x);
-      continue;
-    }
-    uint32_t code[8];
-    const uint32_t sm = quantise(x, code);
-    if (id < 0) continue;
-    const Kv4 lay(D);
-    const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = token % kBlockTokens;
-    uint8_t* blk = kv.k + kv.block4(id, h, token);
-    if (part == 1) {
-      const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 |
-                         code[3] << 20 | code[5] << 24 | code[7] << 28;
-      reinterpret_cast<uint32_t*>(blk)[(r * 4 + t4) * NG + grp] = w;
-      if (t4 == 0) reinterpret_cast<uint32_t*>(blk + lay.k_params())[r * NG + grp] = sm;
-    } else {
-      const int tp = r / 8, tt = r % 8 / 2, hi = r % 2;
+
+  bool filled = false;
+  // the same number of rounds for all lanes of a warp: the warp's first row leads
+  int lead_tok = (int)((threadIdx.x & ~31u) >> p.chunk_shift) / heads;
+  int lead_h = (int)((threadIdx.x & ~31u) >> p.chunk_shift) - lead_tok * heads;
+  while (lead_tok < ntok || !filled) {
+    uint4 own[2], other[2];
+    int rt[2], rh[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int g = 2 * t4 + n;
-        const uint32_t w = code[4 * n] | code[4 * n + 1] << 4 | code[4 * n + 2] << 8 | code[4 * n + 3] << 12;
-        reinterpret_cast<uint16_t*>(blk + lay.v_codes())[(((tp * 8 + g) * 4 + tt) * NG + grp) * 2 + hi] =
-            (uint16_t)w;
+    for (int u = 0; u < 2; ++u) {
+      rt[u] = tok;
+      rh[u] = h;
+      if (WIDE && tok < ntok) {
+        const int part = h < hq ? 0 : h < hq + hk ? 1 : 2;
+        const AppendPart& src = p.part[part];
+        const T* at = static_cast<const T*>(src.in) + b * src.sb + (s0 + tok) * src.ss +
+                      (h - (part == 0 ? 0 : part == 1 ? hq : hq + hk)) * src.sh;
+        own[u] = *reinterpret_cast<const uint4*>(at + e);
+        if (!INTER && turning && part < 2)
+          other[u] = *reinterpret_cast<const uint4*>(at + (e < p.half ? e + p.half : e - p.half));
       }
-      if (t4 == 0) {
-        uint16_t* vp = reinterpret_cast<uint16_t*>(blk + lay.v_params());
-        const int at = (grp * 4 + tt) * 4 + tp * 2 + hi;
-        vp[at] = (uint16_t)sm;
-        vp[at + 16 * NG] = (uint16_t)(sm >> 16);
+      tok += step_tok;
+      h += step_h;
+      if (h >= heads) {
+        h -= heads;
+        ++tok;
+      }
+      lead_tok += step_tok;
+      lead_h += step_h;
+      if (lead_h >= heads) {
+        lead_h -= heads;
+        ++lead_tok;
+      }
+    }
+    if (!filled) {
+      for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
+        const int at = i / p.half, f = i - at * p.half;
+        cs[at * p.half + angle_at<INTER, WIDE>(f, p.half)] =
+            rotary_cos_sin((double)(first + at), p.inv_freq[f], p.magnitude);
+      }
+      __syncthreads();
+      filled = true;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool there = rt[u] < ntok;
+      const int part = rh[u] < hq ? 0 : rh[u] < hq + hk ? 1 : 2;
+      const int hp = rh[u] - (part == 0 ? 0 : part == 1 ? hq : hq + hk);
+      float x[8] = {}, y[8];
+      if (there) {
+        const AppendPart& src = p.part[part];
+        const T* at = static_cast<const T*>(src.in) + b * src.sb + (s0 + rt[u]) * src.ss + hp * src.sh;
+        if (WIDE) {
+          unpack8<T>(own[u], x);
+          if (!INTER && turning) unpack8<T>(other[u], y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = Elem<T>::value(reinterpret_cast<const uint16_t*>(at)[e + i]);
+        }
+        if (part < 2 && turning) rotate8<T, INTER, WIDE>(at, e, p.half, cs + rt[u] * p.half, x, y);
+        if (part == 0)
+          *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) +
+                                    (((long long)b * p.S + s0 + rt[u]) * hq + hp) * kv.D + e) = pack8<T>(x);
+      }
+      const int place = there && part > 0 ? places[rt[u]] : -1;
+      const int at = place + (hp << p.page_shift);  // row of the cache
+      if (BITS == 16) {
+        if (place >= 0)
+          *reinterpret_cast<uint4*>((part == 1 ? kv.k : kv.v) + ((long long)at * kv.D + e) * 2) = pack8<T>(x);
+        continue;
+      }
+      if (!__any_sync(0xffffffffu, place >= 0)) continue;
+      uint32_t code[8];
+      const uint32_t sm = quantise(x, code);
+      if (place < 0) continue;
+      const Kv4 lay(kv.D);
+      const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = at % kBlockTokens;
+      uint8_t* blk = kv.k + (long long)(at / kBlockTokens) * lay.bytes();
+      if (part == 1) {
+        const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 |
+                           code[3] << 20 | code[5] << 24 | code[7] << 28;
+        reinterpret_cast<uint32_t*>(blk)[(r * 4 + t4) * NG + grp] = w;
+        if (t4 == 0) reinterpret_cast<uint32_t*>(blk + lay.k_params())[r * NG + grp] = sm;
+      } else {
+        const int tp = r / 8, tt = r % 8 / 2, hi = r % 2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const int g = 2 * t4 + n;
+          const uint32_t w =
+              code[4 * n] | code[4 * n + 1] << 4 | code[4 * n + 2] << 8 | code[4 * n + 3] << 12;
+          reinterpret_cast<uint16_t*>(blk + lay.v_codes())[(((tp * 8 + g) * 4 + tt) * NG + grp) * 2 + hi] =
+              (uint16_t)w;
+        }
+        if (t4 == 0) {
+          uint16_t* vp = reinterpret_cast<uint16_t*>(blk + lay.v_params());
+          const int i = (grp * 4 + tt) * 4 + tp * 2 + hi;
+          vp[i] = (uint16_t)sm;
+          vp[i + 16 * NG] = (uint16_t)(sm >> 16);
+        }
       }
     }
   }
 }
 
-template <typename T, int VEC, int BITS>
+template <typename T, int BITS, bool WIDE>
 int launch_append(const AppendParams& p, bool interleaved, unsigned grid, size_t smem,
                   cudaStream_t st) {
   const cudaError_t e =
-      interleaved ? launch_pdl(fa_kv_append_kernel<T, VEC, true, BITS>, dim3(grid), dim3(kThreads),
+      interleaved ? launch_pdl(fa_kv_append_kernel<T, true, BITS, WIDE>, dim3(grid), dim3(kThreads),
                                smem, st, p)
-                  : launch_pdl(fa_kv_append_kernel<T, VEC, false, BITS>, dim3(grid), dim3(kThreads),
+                  : launch_pdl(fa_kv_append_kernel<T, false, BITS, WIDE>, dim3(grid), dim3(kThreads),
                                smem, st, p);
   return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 template <typename T>
-int launch_append_t(const AppendParams& p, int vec, bool interleaved, unsigned grid, size_t smem,
+int launch_append_t(const AppendParams& p, bool is_wide, bool interleaved, unsigned grid, size_t smem,
                     cudaStream_t st) {
   if (p.kv.bits == 16)
-    return vec == 8 ? launch_append<T, 8, 16>(p, interleaved, grid, smem, st)
-                    : launch_append<T, 1, 16>(p, interleaved, grid, smem, st);
-  return vec == 8 ? launch_append<T, 8, 4>(p, interleaved, grid, smem, st)
-                  : launch_append<T, 1, 4>(p, interleaved, grid, smem, st);
+    return is_wide ? launch_append<T, 16, true>(p, interleaved, grid, smem, st)
+                   : launch_append<T, 16, false>(p, interleaved, grid, smem, st);
+  return is_wide ? launch_append<T, 4, true>(p, interleaved, grid, smem, st)
+                 : launch_append<T, 4, false>(p, interleaved, grid, smem, st);
 }
 
 // ---------------------------------------------------------------- read
@@ -287,12 +337,14 @@ struct ReadParams {
   const int* lengths;
   void* k_out;  // (batch, max_len, heads, D)
   void* v_out;
-  int max_len;
+  int max_len, page_shift, chunk_shift;
 };
 
-__device__ __forceinline__ float2 params_of(uint32_t sm) {
-  return make_float2(__half2float(__ushort_as_half((uint16_t)sm)),
-                     __half2float(__ushort_as_half((uint16_t)(sm >> 16))));
+// 4-bit codes to values: a nibble pair masked out of its word is two fp16
+// subnormals (c 2^-24 from bits 0..3, c 2^-20 from bits 4..7), which convert
+// exactly; `s24` and `s20` are the scale times 2^24 and 2^20.
+__device__ __forceinline__ float2 pair_of(uint32_t masked) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&masked));
 }
 
 // The cached tokens as contiguous K and V, rows behind a sequence's length
@@ -305,75 +357,135 @@ __global__ void __launch_bounds__(kThreads) fa_kv_read_kernel(const ReadParams p
   griddep_wait();
   griddep_launch_dependents();
   const KvView& kv = p.kv;
-  const int D = kv.D, chunks = D / 8, b = blockIdx.y, first = blockIdx.x * kBlockTokens;
+  const int D = kv.D, b = blockIdx.y, first = blockIdx.x * kBlockTokens;
   const int given = p.lengths[b], len = min(kv.clamp_length(given), p.max_len);
   if (kv.bad_length(given) && blockIdx.x == 0 && threadIdx.x == 0) kv.report(kStatusPage);
   const int there = max(0, min(len - first, kBlockTokens));  // tokens of the block to copy
   const int rows = min(p.max_len - first, kBlockTokens);     // tokens of the block to write
   int id = -1;
   if (there > 0) {
-    id = kv.page_of(b, first);
+    id = kv.page_of(b, first, p.page_shift);
     if (id < 0 && threadIdx.x == 0) kv.report(kStatusPage);
   }
-  const int token0 = first & (kv.page - 1);
   const int copied = id < 0 ? 0 : there;
-  T* k_out = static_cast<T*>(p.k_out) + ((long long)b * p.max_len + first) * kv.heads * D;
-  T* v_out = static_cast<T*>(p.v_out) + ((long long)b * p.max_len + first) * kv.heads * D;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  const int per_token = kv.heads * chunks;
+  uint4* k_out = reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + ((long long)b * p.max_len + first) * kv.heads * D);
+  uint4* v_out = reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + ((long long)b * p.max_len + first) * kv.heads * D);
+  const int per_token = kv.heads << p.chunk_shift;
   if (copied < rows) {  // zero the rest
+    const uint4 zero = make_uint4(0, 0, 0, 0);
     for (int i = copied * per_token + threadIdx.x; i < rows * per_token; i += kThreads) {
-      reinterpret_cast<uint4*>(k_out)[i] = zero;
-      reinterpret_cast<uint4*>(v_out)[i] = zero;
+      k_out[i] = zero;
+      v_out[i] = zero;
     }
   }
+  // row of the cache: head 0, the block's first token
+  const int at0 = id < 0 ? 0 : ((id * kv.heads) << p.page_shift) | (first & (kv.page - 1));
+  const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), row = threadIdx.x >> p.chunk_shift;
+  const int step = kThreads >> p.chunk_shift;
+  const int step_tok = step / kv.heads, step_h = step - step_tok * kv.heads;
+  const int tok0 = row / kv.heads, h0 = row - tok0 * kv.heads;
+  auto next = [&](int& tok, int& h) {
+    tok += step_tok;
+    h += step_h;
+    if (h >= kv.heads) {
+      h -= kv.heads;
+      ++tok;
+    }
+  };
+  auto out_at = [&](int tok, int h) { return tok * per_token + (h << p.chunk_shift) + c; };
   if (BITS == 16) {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < copied * per_token; i += kThreads) {
-      const int c = i % chunks, h = i / chunks % kv.heads, r = i / per_token;
-      const long long at = kv.row16(id, h, token0 + r) + c * 16;
-      reinterpret_cast<uint4*>(k_out)[i] = *reinterpret_cast<const uint4*>(kv.k + at);
-      reinterpret_cast<uint4*>(v_out)[i] = *reinterpret_cast<const uint4*>(kv.v + at);
+    const uint4* ks = reinterpret_cast<const uint4*>(kv.k);
+    const uint4* vs = reinterpret_cast<const uint4*>(kv.v);
+    int tok = tok0, h = h0;
+    while (tok < copied) {
+      uint4 x[4], y[4];
+      int o[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        o[u] = -1;
+        if (tok < copied) {
+          const long long at = ((long long)(at0 + (h << p.page_shift) + tok) << p.chunk_shift) + c;
+          x[u] = ks[at];
+          y[u] = vs[at];
+          o[u] = out_at(tok, h);
+        }
+        next(tok, h);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (o[u] >= 0) {
+          k_out[o[u]] = x[u];
+          v_out[o[u]] = y[u];
+        }
     }
     return;
   }
   const Kv4 lay(D);
-  const int NG = lay.groups();
-  for (int i = threadIdx.x; i < copied * per_token; i += kThreads) {
-    const int c = i % chunks, h = i / chunks % kv.heads, r = i / per_token;
-    const int grp = c / 4, t4 = c % 4;
-    const uint8_t* blk = kv.k + kv.block4(id, h, token0);
-    const uint32_t w = reinterpret_cast<const uint32_t*>(blk)[(r * 4 + t4) * NG + grp];
-    const float2 sm = params_of(reinterpret_cast<const uint32_t*>(blk + lay.k_params())[r * NG + grp]);
-    float x[8];
+  const int NG = lay.groups(), grp = c / 4, t4 = c % 4;
+  auto block = [&](int h) {
+    return kv.k + (long long)((at0 + (h << p.page_shift)) / kBlockTokens) * lay.bytes();
+  };
+  {
+    int r = tok0, h = h0;
+    while (r < copied) {
+      uint32_t w[2], sm[2];
+      int o[2];
 #pragma unroll
-    for (int d = 0; d < 8; ++d)
-      x[d] = fmaf(sm.x, (float)(w >> (d / 2 * 4 + d % 2 * 16) & 15u), sm.y);
-    *reinterpret_cast<Pack16<8>*>(k_out + (long long)i * 8) = pack8<T>(x);
+      for (int u = 0; u < 2; ++u) {
+        o[u] = -1;
+        if (r < copied) {
+          const uint8_t* blk = block(h);
+          w[u] = reinterpret_cast<const uint32_t*>(blk)[(r * 4 + t4) * NG + grp];
+          sm[u] = reinterpret_cast<const uint32_t*>(blk + lay.k_params())[r * NG + grp];
+          o[u] = out_at(r, h);
+        }
+        next(r, h);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (o[u] < 0) continue;
+        const float2 par = pair_of(sm[u]);
+        const float s24 = par.x * 0x1p24f, s20 = par.x * 0x1p20f;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = pair_of((i < 2 ? w[u] : w[u] >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
+          x[2 * i] = fmaf(i % 2 ? s20 : s24, f.x, par.y);
+          x[2 * i + 1] = fmaf(i % 2 ? s20 : s24, f.y, par.y);
+        }
+        k_out[o[u]] = pack8<T>(x);
+      }
+    }
   }
-  const int pairs = (copied + 1) / 2;
-  for (int i = threadIdx.x; i < pairs * per_token; i += kThreads) {
-    const int c = i % chunks, h = i / chunks % kv.heads, rp = i / per_token;
-    const int grp = c / 4, g = c % 4 * 2, tp = rp / 4, tt = rp % 4;
-    const uint8_t* blk = kv.k + kv.block4(id, h, token0);
+  const int pairs = (copied + 1) / 2, g = t4 * 2;
+  int rp = tok0, h = h0;
+  while (rp < pairs) {
+    const uint8_t* blk = block(h);
+    const int tp = rp / 4, tt = rp % 4;
     const uint32_t* vc = reinterpret_cast<const uint32_t*>(blk + lay.v_codes());
     const uint32_t w0 = vc[((tp * 8 + g) * 4 + tt) * NG + grp];
     const uint32_t w1 = vc[((tp * 8 + g + 1) * 4 + tt) * NG + grp];
-    const uint16_t* vp = reinterpret_cast<const uint16_t*>(blk + lay.v_params());
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + lay.v_params()) + (grp * 4 + tt) * 2 + tp;
+    const float2 s = pair_of(vp[0]), m = pair_of(vp[8 * NG]);  // of both tokens
+    const int o = out_at(2 * rp, h);
+    float x[2][8];
 #pragma unroll
-    for (int hi = 0; hi < 2; ++hi) {
-      if (2 * rp + hi >= copied) break;
-      const int at = (grp * 4 + tt) * 4 + tp * 2 + hi;
-      const float s = __half2float(__ushort_as_half(vp[at]));
-      const float m = __half2float(__ushort_as_half(vp[at + 16 * NG]));
-      float x[8];
-#pragma unroll
-      for (int d = 0; d < 8; ++d)
-        x[d] = fmaf(s, (float)((d < 4 ? w0 : w1) >> (hi * 16 + d % 4 * 4) & 15u), m);
-      *reinterpret_cast<Pack16<8>*>(v_out + ((long long)(2 * rp + hi) * per_token + h * chunks + c) * 8) =
-          pack8<T>(x);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = i < 4 ? w0 : w1;
+      const float2 f = pair_of((i % 4 < 2 ? w : w >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
+      x[0][i] = fmaf(s.x * (i % 2 ? 0x1p20f : 0x1p24f), f.x, m.x);
+      x[1][i] = fmaf(s.y * (i % 2 ? 0x1p20f : 0x1p24f), f.y, m.y);
     }
+    v_out[o] = pack8<T>(x[0]);
+    if (2 * rp + 1 < copied) v_out[o + per_token] = pack8<T>(x[1]);
+    next(rp, h);
   }
+}
+
+int log2_of(int x) {
+  int n = 0;
+  while ((1 << n) < x) ++n;
+  return n;
 }
 
 bool bad_append_part(const fa_sm100_heads& x) {
@@ -409,31 +521,35 @@ extern "C" int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100
   if (inv_freq && (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > cache->head_dim)) return FA_ERR_ARG;
   AppendParams p = {};
   p.kv = kv_view(cache, page_table, table_width, status);
-  if (q) p.q = {q->in, q->stride_batch, q->stride_seq, q->stride_head, q->heads};
-  p.k = {k->in, k->stride_batch, k->stride_seq, k->stride_head, k->heads};
-  p.v = {v->in, v->stride_batch, v->stride_seq, v->stride_head, v->heads};
+  if (q) p.part[0] = {q->in, q->stride_batch, q->stride_seq, q->stride_head, q->heads};
+  p.part[1] = {k->in, k->stride_batch, k->stride_seq, k->stride_head, k->heads};
+  p.part[2] = {v->in, v->stride_batch, v->stride_seq, v->stride_head, v->heads};
   p.q_out = q ? q->out : nullptr;
   p.starts = starts;
   p.counts = counts;
   p.inv_freq = inv_freq;
   p.half = inv_freq ? rotary_dim / 2 : 0;
-  p.tokens = (long long)batch * seqlen;
   p.S = seqlen;
   p.magnitude = magnitude;
-  const int vec = wide(*k) && wide(*v) && (!q || wide(*q)) ? 8 : 1;
-  // whole tokens until every thread has two items
-  const long long per_token = (long long)(p.q.heads + 2 * p.k.heads) * (cache->head_dim / 8);
-  long long per_cta = 2 * kThreads / per_token;
+  p.page_shift = log2_of(cache->page_size);
+  p.chunk_shift = log2_of(cache->head_dim / 8);
+  const bool is_wide = wide(*k) && wide(*v) && (!q || wide(*q)) &&
+                       (interleaved ? p.half % 4 : p.half % 8) == 0;
+  // whole tokens until every thread has four items
+  const long long per_token = (long long)(p.part[0].heads + 2 * k->heads) * (cache->head_dim / 8);
+  long long per_cta = 4 * kThreads / per_token;
   if (p.half > 0 && per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
+  if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
   p.per_cta = (int)per_cta;
-  const long long grid = (p.tokens + per_cta - 1) / per_cta;
+  p.per_seq = (int)((seqlen + per_cta - 1) / per_cta);
+  const long long grid = (long long)p.per_seq * batch;
   if (grid > 2147483647LL) return FA_ERR_ARG;
-  const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
+  const size_t smem = (size_t)per_cta * (p.half * sizeof(float2) + sizeof(int));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return cache->dtype == FA_DTYPE_BF16
-             ? launch_append_t<__nv_bfloat16>(p, vec, interleaved != 0, (unsigned)grid, smem, st)
-             : launch_append_t<__half>(p, vec, interleaved != 0, (unsigned)grid, smem, st);
+             ? launch_append_t<__nv_bfloat16>(p, is_wide, interleaved != 0, (unsigned)grid, smem, st)
+             : launch_append_t<__half>(p, is_wide, interleaved != 0, (unsigned)grid, smem, st);
 }
 
 extern "C" int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_table,
@@ -455,6 +571,8 @@ extern "C" int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_
   p.k_out = k_out;
   p.v_out = v_out;
   p.max_len = max_len;
+  p.page_shift = log2_of(cache->page_size);
+  p.chunk_shift = log2_of(cache->head_dim / 8);
   const dim3 grid((unsigned)(((long long)max_len + kBlockTokens - 1) / kBlockTokens), (unsigned)batch);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;

@@ -48,8 +48,8 @@ struct KvView {  // a cache as the kernels take it
     if (status) atomicOr(status, bit);
   }
   // Page id of token `pos` of sequence b, or -1.
-  __device__ __forceinline__ int page_of(int b, long long pos) const {
-    const long long i = pos / page;
+  __device__ __forceinline__ int page_of(int b, long long pos, int page_shift) const {
+    const long long i = pos >> page_shift;
     if (pos < 0 || i >= table_width) return -1;
     const int id = table[(long long)b * table_width + i];
     return bad_page(id) ? -1 : id;
@@ -61,15 +61,6 @@ struct KvView {  // a cache as the kernels take it
   }
   __device__ __forceinline__ bool bad_length(int n) const {
     return n < 0 || n > (long long)table_width * page;
-  }
-  // Byte offset of a 16-bit row (page, head, token).
-  __device__ __forceinline__ long long row16(int id, int head, int token) const {
-    return (((long long)id * heads + head) * page + token) * D * 2;
-  }
-  // Byte offset of the 4-bit block that holds (page, head, token).
-  __device__ __forceinline__ long long block4(int id, int head, int token) const {
-    return (((long long)id * heads + head) * (page / kBlockTokens) + token / kBlockTokens) *
-           Kv4(D).bytes();
   }
 };
 

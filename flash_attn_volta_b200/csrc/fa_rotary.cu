@@ -38,89 +38,104 @@ struct RotaryParams {
   const void* positions;  // int32 or int64 (pos64), or null
   long long pos_sb;       // its batch stride
   long long first;        // position of token 0 without `positions`
-  long long tokens;       // batch * seqlen
-  int S, D, half, per_cta, pos64;
+  int S, D, half, per_cta, pos64;  // per_cta: tokens of a CTA, all of one sequence
+  int per_seq, per_head, width;    // CTAs of a sequence, items of a head, items of a row of threads
   float magnitude, sign;
 };
 
-// One thread's share of a head: a vector of VEC first halves and the VEC
-// second halves of the same pairs (half), or VEC elements = VEC/2 pairs
-// (interleaved), or VEC elements behind R.
+// One thread's share of a head (an item): a vector of VEC first halves and the
+// VEC second halves of the same pairs (half), or VEC elements = VEC/2 pairs
+// (interleaved), or VEC elements behind R.  The threads stand as `rows` rows of
+// `width` items; a row is one head of one token, and each thread steps down the
+// rows with additions alone.  A vector's i-th cosine and sine are `turning`
+// apart in shared memory, so the lanes of a row read neighbouring words.
 template <typename T, int VEC, bool INTER>
-__global__ void __launch_bounds__(kThreads) fa_rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, 4) fa_rotary_kernel(const RotaryParams p) {
   extern __shared__ float2 cs[];
   griddep_wait();
   griddep_launch_dependents();
   using V = Pack16<VEC>;
-  const unsigned half = p.half, D = p.D;
-  const unsigned turning = INTER ? 2 * half / VEC : half / VEC;  // items of a head that rotate
-  const unsigned per_head = turning + (D - 2 * half) / VEC;
-  const unsigned heads = p.q.heads + p.k.heads, per_token = heads * per_head;
-  const long long tok0 = (long long)blockIdx.x * p.per_cta;
-  const int ntok = (int)min((long long)p.per_cta, p.tokens - tok0);
-  const unsigned total = ntok * per_token;
+  constexpr int PAIRS = INTER ? VEC / 2 : VEC;
+  const int half = p.half, turning = half / PAIRS;  // items of a head that rotate
+  const int heads = p.q.heads + p.k.heads;
+  const int b = blockIdx.x / p.per_seq, s0 = (blockIdx.x - b * p.per_seq) * p.per_cta;
+  const int ntok = min(p.per_cta, p.S - s0);
+  const int row = threadIdx.x / p.width, col = threadIdx.x - row * p.width;
+  const int step = kThreads / p.width, step_tok = step / heads, step_h = step - step_tok * heads;
+  int tok = row < step ? row / heads : ntok, h = row - row / heads * heads;
 
-  for (unsigned base = 0; base < total || base == 0; base += kThreads * kItems) {
-    V a[kItems], b[kItems];
-    T* dst[kItems];
-    unsigned where[kItems];  // angle index; ~0u: copied
-#pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      const unsigned it = base + u * kThreads + threadIdx.x;
-      dst[u] = nullptr;
-      if (it >= total) continue;
-      const unsigned tok = it / per_token, rem = it % per_token;
-      unsigned h = rem / per_head;
-      const unsigned j = rem % per_head;
-      const bool is_k = h >= (unsigned)p.q.heads;
-      const RotaryPart& part = is_k ? p.k : p.q;
-      if (is_k) h -= p.q.heads;
-      const long long t = tok0 + tok, bt = t / p.S, s = t % p.S;
-      const T* src = static_cast<const T*>(part.in) + bt * part.sb + s * part.ss + h * part.sh;
-      T* out = static_cast<T*>(part.out) + (t * part.heads + h) * (long long)D;
+  auto fill = [&]() {
+    for (int i = threadIdx.x; i < ntok * half; i += kThreads) {
+      const int at = i / half, f = i - at * half;
+      const long long s = s0 + at, where = b * p.pos_sb + s;
+      const long long pos = p.positions == nullptr ? p.first + s
+                            : p.pos64 ? static_cast<const long long*>(p.positions)[where]
+                                      : static_cast<const int*>(p.positions)[where];
+      float2 c = rotary_cos_sin((double)pos, p.inv_freq[f], p.magnitude);
+      c.y *= p.sign;
+      cs[at * half + f % PAIRS * turning + f / PAIRS] = c;
+    }
+    __syncthreads();
+  };
+  bool filled = false;
+  while (tok < ntok || !filled) {
+    for (int j = col; j < p.per_head || !filled; j += p.width) {
+      V a[kItems], o[kItems];
+      T* dst[kItems];
+      const float2* w[kItems];  // null: copied
       const bool turns = j < turning;
-      const unsigned e = turns ? j * VEC : 2 * half + (j - turning) * VEC;
-      a[u] = *reinterpret_cast<const V*>(src + e);
-      if (!INTER && turns) b[u] = *reinterpret_cast<const V*>(src + e + half);
-      dst[u] = out + e;
-      where[u] = turns ? tok * half + (INTER ? e / 2 : e) : ~0u;
-    }
-    if (base == 0) {
-      for (unsigned i = threadIdx.x; i < ntok * half; i += kThreads) {
-        const long long t = tok0 + i / half, bt = t / p.S, s = t % p.S;
-        const long long at = bt * p.pos_sb + s;
-        const long long pos = p.positions == nullptr ? p.first + s
-                              : p.pos64 ? static_cast<const long long*>(p.positions)[at]
-                                        : static_cast<const int*>(p.positions)[at];
-        float2 c = rotary_cos_sin((double)pos, p.inv_freq[i % half], p.magnitude);
-        c.y *= p.sign;
-        cs[i] = c;
-      }
-      __syncthreads();
-    }
+      const int e = turns ? j * VEC : 2 * half + (j - turning) * VEC;
+      int t = tok, hh = h;
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      if (dst[u] == nullptr) continue;
-      if (where[u] != ~0u) {
-        const float2* w = cs + where[u];
-        if (INTER) {
-#pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) {
-            const float x = Elem<T>::value(a[u].v[2 * i]), y = Elem<T>::value(a[u].v[2 * i + 1]);
-            a[u].v[2 * i] = Elem<T>::bits(x * w[i].x - y * w[i].y);
-            a[u].v[2 * i + 1] = Elem<T>::bits(y * w[i].x + x * w[i].y);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float x = Elem<T>::value(a[u].v[i]), y = Elem<T>::value(b[u].v[i]);
-            a[u].v[i] = Elem<T>::bits(x * w[i].x - y * w[i].y);
-            b[u].v[i] = Elem<T>::bits(y * w[i].x + x * w[i].y);
-          }
-          *reinterpret_cast<V*>(dst[u] + half) = b[u];
+      for (int u = 0; u < kItems; ++u) {
+        dst[u] = nullptr;
+        if (t < ntok && j < p.per_head) {
+          const bool is_k = hh >= p.q.heads;
+          const RotaryPart& part = is_k ? p.k : p.q;
+          const int hp = is_k ? hh - p.q.heads : hh;
+          const T* src = static_cast<const T*>(part.in) + b * part.sb + (s0 + t) * part.ss + hp * part.sh + e;
+          dst[u] = static_cast<T*>(part.out) + (((long long)b * p.S + s0 + t) * part.heads + hp) * p.D + e;
+          w[u] = turns ? cs + t * half + j : nullptr;
+          a[u] = *reinterpret_cast<const V*>(src);
+          if (!INTER && turns) o[u] = *reinterpret_cast<const V*>(src + half);
+        }
+        t += step_tok;
+        hh += step_h;
+        if (hh >= heads) {
+          hh -= heads;
+          ++t;
         }
       }
-      *reinterpret_cast<V*>(dst[u]) = a[u];
+      if (!filled) {
+        filled = true;
+        fill();
+      }
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        if (dst[u] == nullptr) continue;
+        if (w[u] != nullptr) {
+#pragma unroll
+          for (int i = 0; i < PAIRS; ++i) {
+            const float2 c = w[u][i * turning];
+            uint16_t& lo = INTER ? a[u].v[2 * i] : a[u].v[i];
+            uint16_t& hi = INTER ? a[u].v[2 * i + (VEC > 1)] : o[u].v[i];
+            const float x = Elem<T>::value(lo), y = Elem<T>::value(hi);
+            lo = Elem<T>::bits(x * c.x - y * c.y);
+            hi = Elem<T>::bits(y * c.x + x * c.y);
+          }
+          if (!INTER) *reinterpret_cast<V*>(dst[u] + half) = o[u];
+        }
+        *reinterpret_cast<V*>(dst[u]) = a[u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      tok += step_tok;
+      h += step_h;
+      if (h >= heads) {
+        h -= heads;
+        ++tok;
+      }
     }
   }
 }
@@ -186,7 +201,6 @@ extern "C" int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k,
   p.pos_sb = positions_stride;
   p.pos64 = positions_64;
   p.first = first;
-  p.tokens = (long long)batch * seqlen;
   p.S = seqlen;
   p.D = head_dim;
   p.half = rotary_dim / 2;
@@ -198,15 +212,17 @@ extern "C" int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k,
   const int unit = interleaved ? rotary_dim : rotary_dim / 2;
   while (vec > 1 && (unit % vec || head_dim % vec || rotary_dim % vec)) vec /= 2;
   if (interleaved && vec == 1) return FA_ERR_ARG;  // a pair has to be 4-byte aligned
-  const int per_head = (interleaved ? head_dim : head_dim - p.half) / vec;
-  const long long per_token = (long long)(p.q.heads + p.k.heads) * per_head;
-  // whole tokens until each thread has kItems vectors: 2 measured against 1 and 4 at
-  // 8 x 2048 tokens of 16 + 16 heads of 128 (see the timing below)
-  long long per_cta = (long long)kThreads * kItems / per_token;
+  p.per_head = (interleaved ? head_dim : head_dim - p.half) / vec;
+  p.width = p.per_head < kThreads ? p.per_head : kThreads;
+  const long long per_token = (long long)(p.q.heads + p.k.heads) * p.per_head;
+  // whole tokens until each thread has two rounds of kItems vectors
+  long long per_cta = 2LL * kThreads * kItems / per_token;
   if (per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
+  if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
   p.per_cta = (int)per_cta;
-  const long long grid = (p.tokens + per_cta - 1) / per_cta;
+  p.per_seq = (int)((seqlen + per_cta - 1) / per_cta);
+  const long long grid = (long long)p.per_seq * batch;
   if (grid > 2147483647LL) return FA_ERR_ARG;
   const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

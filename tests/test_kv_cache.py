@@ -377,6 +377,8 @@ DECODE = [  # bits, B lengths, S, H, Hkv, D, page
     (16, [70, 19], 17, 3, 1, 128, 16), (4, [70, 19], 17, 3, 1, 128, 16),
     (4, [2500, 1], 2, 16, 2, 128, 256), (16, [2500, 1], 2, 16, 2, 64, 1024),
     (4, [600], 3, 32, 4, 32, 64), (16, [600], 3, 32, 4, 16, 64),
+    (4, [500, 77], 7, 12, 3, 64, 32), (16, [500, 77], 7, 12, 3, 64, 32),
+    (4, [290, 3], 9, 8, 2, 32, 16), (16, [290, 3], 9, 8, 2, 32, 16),
 ]
 
 

@@ -54,17 +54,28 @@ constexpr float kLn2 = 0.69314718055994531f;
 // Column blocks of 8 query rows that a CTA's registers hold.
 constexpr int max_nt(int D) { return D <= 64 ? 4 : 2; }
 
-template <int D, int BITS>
+// Blocks of a warp per tile, stages of its ring, CTAs per SM.
+constexpr int blocks_of(int D, int bits, int nt) {
+  return bits == 16 ? (D == 128 ? 1 : 2) : nt == 1 ? 4 : 2;
+}
+constexpr int stages_of(int D, int bits, int nt) {
+  return bits == 16 ? 3 : D == 128 ? (nt == 1 ? 2 : 4) : 4;
+}
+constexpr int kCtas = 2;
+
+template <int D, int BITS, int NT>
 struct Cfg {
-  static constexpr int kU = (BITS == 16 && D == 128) ? 1 : 2;  // blocks of a warp per tile
+  static constexpr int kU = blocks_of(D, BITS, NT);
   static constexpr int kBlockBytes = BITS == 16 ? 64 * D : 20 * D;
   static constexpr int kStageBytes = kU * kBlockBytes;
-  static constexpr int kStages = BITS == 16 ? 3 : D == 128 ? 2 : 4;
-  static constexpr int kCtas = BITS == 16 ? 2 : 3;  // per SM
+  static constexpr int kStages = stages_of(D, BITS, NT);
   static constexpr int kTile = kWarps * kU * kBlockTokens;  // tokens
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kJoinStride = D + 4;  // floats of a row in the join buffer
-  static constexpr int kJoinBytes = kWarps * 8 * kJoinStride * 4;
+  // The warps join all 8 rows of a column block at once, or 4 where there is no room.
+  static constexpr int kJoinRows =
+      kCtas * (kRingBytes + kWarps * 8 * kJoinStride * 4 + 512 + 1024) <= 228 * 1024 ? 8 : 4;
+  static constexpr int kJoinBytes = kWarps * kJoinRows * kJoinStride * 4;
   static constexpr int kMiscBytes = 512;         // barriers and small shared variables
   static constexpr int kSmem = kRingBytes + kJoinBytes + kMiscBytes;
   static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
@@ -81,33 +92,26 @@ struct DecodeParams {
   float* part_o;       // (2 * grid, ROWS, D)
   float2* part_ml;     // (2 * grid, ROWS): maximum (log2 domain), sum
   int B, Sq, H, group, row_blocks, causal, page_shift, bf16;
-  int grid, negate;
+  int grid, negate, whole;  // whole: CTA i computes segment i
   float scale_log2;  // |scale| log2 e, above 0; `negate`: the scale is negative (q's sign changes)
   unsigned long long timeout_ns;
 };
 
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
+// N words of shared memory as one load.
 template <int N>
-__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[N]) {
+__device__ __forceinline__ void load_words(const uint8_t* at, uint32_t (&w)[N]) {
   if constexpr (N == 4) {
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(a));
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
   } else if constexpr (N == 2) {
-    const uint2 v = lds64(a);
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
     w[0] = v.x;
     w[1] = v.y;
   } else {
-    w[0] = lds32(a);
+    w[0] = *reinterpret_cast<const uint32_t*>(at);
   }
 }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
@@ -129,13 +133,13 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(T) == 2 && Elem<T>::kIdescAB == 0) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   } else {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -147,7 +151,7 @@ template <typename T>
 __device__ __forceinline__ void mma16816_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                               uint32_t a3, uint32_t b0, uint32_t b1) {
   static_assert(Elem<T>::kIdescAB == 0, "fp16 operands");
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -168,8 +172,13 @@ __device__ __forceinline__ float low_half(uint32_t w) {
 
 // Position in the tile list.
 struct Cursor {
-  int b, h, rb, tt, nt, len;  // sequence, K/V head, row block, tile of nt, length
+  int b, h, rb, tt, nt, len;  // sequence, K/V head, row block, tile of nt (nt: behind them), length
 };
+
+// The start and end of a segment (its q, the join of the warps) take a CTA about
+// as long as kSegmentCost tiles, so the list has that many empty places behind
+// each segment's tiles and shares with many short segments hold fewer tiles.
+constexpr int kSegmentCost = 4;
 
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) {
@@ -177,19 +186,18 @@ __device__ __forceinline__ int tiles_of(int len) {
   return n < 1 ? 1 : n;  // a sequence without tokens has one tile, which writes its zeros
 }
 
-// Sums the tile counts of all sequences (`total`) and, for one position `want`
-// of the list, finds the sequence that holds it and the tiles before that
-// sequence.  All threads of the CTA take part.
+// Sums the places of all sequences in the list (box[0]) and finds the sequence
+// that holds the first place of a share (box[1]) and the places before that
+// sequence (box[2]).  All threads of the CTA take part.
 template <int TILE>
-__device__ __forceinline__ void locate(const DecodeParams& p, int per_tile, long long (&box)[3],
-                                       long long* warp_sum, long long want_num, long long want_den,
-                                       int want_b) {
+__device__ __forceinline__ void locate(const DecodeParams& p, int segs, long long (&box)[3],
+                                       long long* warp_sum, int share) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int chunk = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
   long long mine = 0;
   for (int b = b0; b < b1; ++b)
-    mine += (long long)tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) * per_tile;
+    mine += (long long)(tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) + kSegmentCost) * segs;
   long long before = mine;  // inclusive scan
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
@@ -205,13 +213,12 @@ __device__ __forceinline__ void locate(const DecodeParams& p, int per_tile, long
     total += warp_sum[i];
   }
   before -= mine;
-  // want_b >= 0: the tiles before that sequence; else the position total * num / den
-  const long long want = want_b >= 0 ? 0 : total * want_num / want_den;
+  const long long want = total * share / p.grid;
   if (tid == 0) box[0] = total;
   long long at = before;
   for (int b = b0; b < b1; ++b) {
-    const long long n = (long long)tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) * per_tile;
-    if (want_b >= 0 ? b == want_b : (want >= at && want < at + n)) {
+    const long long n = (long long)(tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) + kSegmentCost) * segs;
+    if (want >= at && want < at + n) {
       box[1] = b;
       box[2] = at;
     }
@@ -242,10 +249,10 @@ __device__ __forceinline__ void write_row(const DecodeParams& p, int b, int h, i
 // T: the element type of 16-bit pages; 4-bit codes are multiplied as fp16
 // whatever q's type is.
 template <typename T, int D, int BITS, int NT>
-__global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
+__global__ void __launch_bounds__(kThreads, kCtas)
     fa_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v) {
-  using C = Cfg<D, BITS>;
+  using C = Cfg<D, BITS, NT>;
   using M = T;  // operand type
   constexpr int U = C::kU, NS = C::kStages, ROWS = 8 * NT, NG = BITS == 4 ? C::kGroups : 1;
   constexpr int KSTEPS = D / 16;
@@ -271,39 +278,57 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
   griddep_launch_dependents();
 
   const int segs = p.kv.heads * p.row_blocks;  // segments of a sequence
-  locate<C::kTile>(p, segs, sh.box, sh.warp_sum, blockIdx.x, p.grid, -1);  // ends with __syncthreads
-  const long long total = sh.box[0];
-  const long long begin = total * blockIdx.x / p.grid, end = total * (blockIdx.x + 1) / p.grid;
-  if (begin >= end) return;
   const WaitCtx wait{&sh.abort_flag, p.kv.status, p.timeout_ns};
-
   Cursor cur;
-  {
+  long long left;
+  if (p.whole) {
+    cur.b = blockIdx.x / segs;
+    const int hr = blockIdx.x - cur.b * segs;
+    cur.len = p.kv.clamp_length(p.lengths[cur.b]);
+    cur.nt = tiles_of<C::kTile>(cur.len);
+    cur.tt = 0;
+    cur.h = hr / p.row_blocks;
+    cur.rb = hr - cur.h * p.row_blocks;
+    left = cur.nt;
+    __syncthreads();
+  } else {
+    locate<C::kTile>(p, segs, sh.box, sh.warp_sum, blockIdx.x);  // ends with __syncthreads
+    const long long total = sh.box[0];
+    const long long begin = total * blockIdx.x / p.grid, end = total * (blockIdx.x + 1) / p.grid;
+    if (begin >= end) return;
     cur.b = (int)sh.box[1];
-    const int given = p.lengths[cur.b];
-    cur.len = p.kv.clamp_length(given);
+    cur.len = p.kv.clamp_length(p.lengths[cur.b]);
     cur.nt = tiles_of<C::kTile>(cur.len);
     const long long in = begin - sh.box[2];
-    const int hr = (int)(in / cur.nt);
-    cur.tt = (int)(in % cur.nt);
+    const int places = cur.nt + kSegmentCost, hr = (int)(in / places);
+    cur.tt = (int)(in % places);
     cur.h = hr / p.row_blocks;
     cur.rb = hr % p.row_blocks;
+    left = end - begin;
   }
+  // To the next tile; returns the places of the list that this takes.
   auto advance = [&](Cursor& c) {
-    if (++c.tt < c.nt) return;
+    if (++c.tt < c.nt) return 1;
+    const int places = 1 + kSegmentCost + c.nt - c.tt;
     c.tt = 0;
-    if (++c.rb < p.row_blocks) return;
+    if (++c.rb < p.row_blocks) return places;
     c.rb = 0;
-    if (++c.h < p.kv.heads) return;
+    if (++c.h < p.kv.heads) return places;
     c.h = 0;
-    if (++c.b >= p.B) return;
+    if (++c.b >= p.B) return places;
     c.len = p.kv.clamp_length(p.lengths[c.b]);
     c.nt = tiles_of<C::kTile>(c.len);
+    return places;
   };
+  if (cur.tt >= cur.nt) {  // the share begins behind a segment's tiles
+    const int over = cur.tt - cur.nt;
+    cur.tt = cur.nt - 1;
+    left -= advance(cur) - 1 - over;
+  }
 
   // ---- producer: lane u < U brings block u of the warp's share of a tile
   Cursor pc = cur;
-  long long to_issue = end - begin;
+  long long to_issue = left;
   int next_id = -1;
   uint32_t ok_bits = 0;  // this lane's block of each stage holds tokens
   uint32_t in_flight = 0;  // stages whose copies have not been waited for
@@ -344,8 +369,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
       }
     }
     in_flight |= 1u << stage;
-    advance(pc);
-    --to_issue;
+    to_issue -= advance(pc);
     look_up();
   };
   look_up();
@@ -467,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
   auto step = [&](int stage, uint32_t ok_mask, auto edge_tag) {
     constexpr bool EDGE = decltype(edge_tag)::value;
     const uint32_t base = my_ring + stage * C::kStageBytes;
+    const uint8_t* bytes = smem_raw + (warp * NS + stage) * C::kStageBytes;
     auto skipped = [&](int u) {
       return EDGE && !((ok_mask >> u & 1u) && block_token(cur, u) < max_lim);
     };
@@ -497,37 +522,41 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
         }
       } else {
         constexpr Kv4 lay(D);
+        const uint8_t* at = bytes + u * C::kBlockBytes;
         uint32_t w0[NG], w1[NG], q0[NG], q1[NG];  // codes and parameters of tokens g, g + 8
-        lds_words<NG>(blk + lane * (NG * 4), w0);
-        lds_words<NG>(blk + (32 + lane) * (NG * 4), w1);
-        lds_words<NG>(blk + lay.k_params() + g * (NG * 4), q0);
-        lds_words<NG>(blk + lay.k_params() + (g + 8) * (NG * 4), q1);
-        uint32_t p0 = 0, p1 = 0;  // parameters of group t
+        load_words<NG>(at + lane * (NG * 4), w0);
+        load_words<NG>(at + (32 + lane) * (NG * 4), w1);
+        load_words<NG>(at + lay.k_params() + g * (NG * 4), q0);
+        load_words<NG>(at + lay.k_params() + (g + 8) * (NG * 4), q1);
+        uint32_t p0[1] = {0}, p1[1] = {0};  // parameters of group t
         if (t < NG) {
-          p0 = lds32(blk + lay.k_params() + (g * NG + t) * 4);
-          p1 = lds32(blk + lay.k_params() + ((g + 8) * NG + t) * 4);
+          load_words<1>(at + lay.k_params() + (g * NG + t) * 4, p0);
+          load_words<1>(at + lay.k_params() + ((g + 8) * NG + t) * 4, p1);
         }
-        float c[4];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma16816_zero<M>(c, p0, p1, p0, p1, qsum[n][0], qsum[n][1]);
+          // the groups' first halves, then their second ones: no product waits
+          // for the one before it
+          float c[NG][4], cm[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[u][n][i] = c[i] * 0x1p-14f;
-        }
+          for (int grp = 0; grp < NG; ++grp)
+            mma16816_zero<M>(c[grp], w0[grp] & 0x000F000Fu, w1[grp] & 0x000F000Fu,
+                             w0[grp] & 0x00F000F0u, w1[grp] & 0x00F000F0u, qf[n][2 * grp][0],
+                             qf[n][2 * grp][1]);
+          mma16816_zero<M>(cm, p0[0], p1[0], p0[0], p1[0], qsum[n][0], qsum[n][1]);
 #pragma unroll
-        for (int grp = 0; grp < NG; ++grp) {
-          const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
-          const float s0 = low_half(q0[grp]), s1 = low_half(q1[grp]);
+          for (int grp = 0; grp < NG; ++grp) {
+            const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
+            mma16816<M>(c[grp], x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u,
+                        x1 & 0x00F000F0u, qf[n][2 * grp + 1][0], qf[n][2 * grp + 1][1]);
+          }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma16816_zero<M>(c, w0[grp] & 0x000F000Fu, w1[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
-                             w1[grp] & 0x00F000F0u, qf[n][2 * grp][0], qf[n][2 * grp][1]);
-            mma16816<M>(c, x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u,
-                        qf[n][2 * grp + 1][0], qf[n][2 * grp + 1][1]);
-            s[u][n][0] = fmaf(s0, c[0], s[u][n][0]);
-            s[u][n][1] = fmaf(s0, c[1], s[u][n][1]);
-            s[u][n][2] = fmaf(s1, c[2], s[u][n][2]);
-            s[u][n][3] = fmaf(s1, c[3], s[u][n][3]);
+          for (int i = 0; i < 4; ++i) s[u][n][i] = cm[i] * 0x1p-14f;
+#pragma unroll
+          for (int grp = 0; grp < NG; ++grp) {
+            const float s0 = low_half(q0[grp]), s1 = low_half(q1[grp]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[u][n][i] = fmaf(i < 2 ? s0 : s1, c[grp][i], s[u][n][i]);
           }
         }
       }
@@ -603,9 +632,10 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
           constexpr uint32_t EXP = Elem<M>::kIdescAB == 0 ? 0x7C00u : 0x7F80u;
           // the block's values (4-bit: V's parameters), two to a word
           constexpr int WORDS = BITS == 16 ? 8 * D : 16 * NG;
-          const uint32_t at = blk + (BITS == 16 ? 32 * D : Kv4(D).v_params());
+          const uint32_t* at = reinterpret_cast<const uint32_t*>(
+              bytes + u * C::kBlockBytes + (BITS == 16 ? 32 * D : Kv4(D).v_params()));
           for (int i = lane; i < WORDS; i += 32) {
-            const uint32_t w = lds32(at + 4 * i);
+            const uint32_t w = at[i];
             apart |= (w & EXP) == EXP || (w >> 16 & EXP) == EXP;
           }
           apart = __any_sync(0xffffffffu, apart);
@@ -618,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
         bool mine[NT][2];
         auto add = [&](float (&acc)[4], int n, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                        uint32_t b0, uint32_t b1) {
-          if constexpr (!EDGE) {
+          if (!EDGE || !apart) {
             mma16816<M>(acc, a0, a1, a2, a3, b0, b1);
           } else {
             float c[4] = {acc[0], acc[1], acc[2], acc[3]};
@@ -658,28 +688,29 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
           }
         } else {
           constexpr Kv4 lay(D);
-          uint32_t w0[NG], w1[NG];
-          lds_words<NG>(blk + lay.v_codes() + lane * (NG * 4), w0);
-          lds_words<NG>(blk + lay.v_codes() + (32 + lane) * (NG * 4), w1);
-          uint2 mm = make_uint2(0, 0);
-          if (g < NG) mm = lds64(blk + lay.v_params() + 32 * NG + lane * 8);
+          const uint8_t* at = bytes + u * C::kBlockBytes;
+          uint32_t w0[NG], w1[NG], mm[2] = {0, 0};
+          load_words<NG>(at + lay.v_codes() + lane * (NG * 4), w0);
+          load_words<NG>(at + lay.v_codes() + (32 + lane) * (NG * 4), w1);
+          if (g < NG) load_words<2>(at + lay.v_params() + 32 * NG + lane * 8, mm);
           if constexpr (EDGE) {
-            mm.x &= keep0;
-            mm.y &= keep1;
+            mm[0] &= keep0;
+            mm[1] &= keep1;
           }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) add(om[n], n, mm.x, 0u, mm.y, 0u, pf[n][0], pf[n][1]);
+          for (int n = 0; n < NT; ++n) add(om[n], n, mm[0], 0u, mm[1], 0u, pf[n][0], pf[n][1]);
 #pragma unroll
           for (int grp = 0; grp < NG; ++grp) {
-            uint2 sc = lds64(blk + lay.v_params() + (grp * 4 + t) * 8);
+            uint32_t sc[2];
+            load_words<2>(at + lay.v_params() + (grp * 4 + t) * 8, sc);
             if constexpr (EDGE) {
-              sc.x &= keep0;
-              sc.y &= keep1;
+              sc[0] &= keep0;
+              sc[1] &= keep1;
             }
             const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint32_t b0 = hmul2(pf[n][0], sc.x), b1 = hmul2(pf[n][1], sc.y);
+              const uint32_t b0 = hmul2(pf[n][0], sc[0]), b1 = hmul2(pf[n][1], sc[1]);
               add(o[2 * grp][n], n, w0[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
                   w1[grp] & 0x000F000Fu, w1[grp] & 0x00F000F0u, b0, b1);
               add(o[2 * grp + 1][n], n, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
@@ -698,11 +729,13 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i) {  // the column block's even rows, then its odd ones
+        constexpr int JR = C::kJoinRows, EACH = JR / 4;
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
-        if (g == 0) sh.join_ml[warp][2 * t + i] = make_float2(mf[n][i], l[n][i]);
-        float* dst = join + (warp * 8 + 2 * t + i) * C::kJoinStride;
+        const int place = t * EACH + (EACH == 2 ? i : 0);
+        if (g == 0) sh.join_ml[warp][place] = make_float2(mf[n][i], l[n][i]);
+        float* dst = join + (warp * JR + place) * C::kJoinStride;
         if constexpr (BITS == 16) {
 #pragma unroll
           for (int k = 0; k < KSTEPS; ++k) {
@@ -719,36 +752,38 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
                             fmaf(o[2 * grp + 1][n][i + 2], 0x1p20f, mm));
           }
         }
-      }
-      __syncthreads();
-      constexpr int PER_ROW = D / 8;
-      for (int i = tid; i < 8 * PER_ROW; i += kThreads) {
-        const int r = i / PER_ROW, d = i % PER_ROW * 8, rr = rb * ROWS + n * 8 + r;
-        float top = -INFINITY, sum = 0.f, x[8] = {};
+        if (EACH == 2 && i == 0) continue;
+        __syncthreads();
+        constexpr int PER_ROW = D / 8;
+        for (int j = tid; j < JR * PER_ROW; j += kThreads) {
+          const int tr = j / PER_ROW, d = j % PER_ROW * 8, r = n * 8 + (EACH == 2 ? tr : 2 * tr + i);
+          const int rr = rb * ROWS + r;
+          float top = -INFINITY, sum = 0.f, x[8] = {};
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.join_ml[w][r].x);
-        const float safe = top == -INFINITY ? 0.f : top;
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sh.join_ml[w][tr].x);
+          const float safe = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 ml = sh.join_ml[w][r];
-          const float e = ex2(ml.x - safe);
-          sum = fmaf(e, ml.y, sum);
-          const float* src = join + (w * 8 + r) * C::kJoinStride + d;
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = sh.join_ml[w][tr];
+            const float e = ex2(ml.x - safe);
+            sum = fmaf(e, ml.y, sum);
+            const float* src = join + (w * JR + tr) * C::kJoinStride + d;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = fmaf(e, src[j], x[j]);
+            for (int k = 0; k < 8; ++k) x[k] = fmaf(e, src[k], x[k]);
+          }
+          if (rr >= rows) continue;
+          if (first && last) {
+            write_row<D>(p, cur.b, h, rr, d, top, sum, x);
+          } else {
+            const long long slot = (2LL * blockIdx.x + (first ? 1 : 0)) * ROWS + r;
+            float4* to = reinterpret_cast<float4*>(p.part_o + slot * D + d);
+            to[0] = make_float4(x[0], x[1], x[2], x[3]);
+            to[1] = make_float4(x[4], x[5], x[6], x[7]);
+            if (d == 0) p.part_ml[slot] = make_float2(top, sum);
+          }
         }
-        if (rr >= rows) continue;
-        if (first && last) {
-          write_row<D>(p, cur.b, h, rr, d, top, sum, x);
-        } else {
-          const long long slot = (2LL * blockIdx.x + (first ? 1 : 0)) * ROWS + n * 8 + r;
-          float4* dst = reinterpret_cast<float4*>(p.part_o + slot * D + d);
-          dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-          dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-          if (d == 0) p.part_ml[slot] = make_float2(top, sum);
-        }
+        __syncthreads();
       }
-      __syncthreads();
     }
   };
 
@@ -757,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
   uint32_t phase = 0;
   bool fresh = true, first = false;
 #pragma unroll 1
-  for (long long left = end - begin; left > 0; --left) {
+  while (left > 0) {
     if (fresh) {
       first = cur.tt == 0;
       begin_segment();
@@ -781,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
     const bool last = cur.tt + 1 == cur.nt;
     if (last || left == 1) end_segment(first, last);
     fresh = last;
-    advance(cur);
+    left -= advance(cur);
     if (++stage == NS) {
       stage = 0;
       phase ^= 1;
@@ -795,62 +830,68 @@ __global__ void __launch_bounds__(kThreads, (NT == 1 ? Cfg<D, BITS>::kCtas : 2))
 // Joins the partial results of the segments that cross shares, in the order of
 // the shares.  blockIdx.x is a border between two shares; the border that a
 // segment crosses first does its work, two rows to a CTA (blockIdx.y).  A thread
-// holds 8 dims of a row and takes every P-th share, all loads independent.
+// holds 8 dims of a row and takes every P-th share, all loads independent;
+// blockIdx.y takes every gridDim.y-th pair of rows.
 template <int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeParams p) {
-  using C = Cfg<D, BITS>;
+  using C = Cfg<D, BITS, NT>;
   constexpr int ROWS = 8 * NT, PER_ROW = D / 8, P = kThreads / 2 / PER_ROW;
   __shared__ long long box[3], warp_sum[kWarps];
   __shared__ float4 part_x[2][P][D / 4];
   __shared__ float2 part_ml[2][P];
   const int segs = p.kv.heads * p.row_blocks, border = blockIdx.x + 1;
-  locate<C::kTile>(p, segs, box, warp_sum, border, p.grid, -1);
+  locate<C::kTile>(p, segs, box, warp_sum, border);
   const long long total = box[0], at = total * border / p.grid, in = at - box[2];
   const int b = (int)box[1], nt = tiles_of<C::kTile>(p.kv.clamp_length(p.lengths[b]));
-  const int hr = (int)(in / nt);
-  const long long t0 = box[2] + (long long)hr * nt, t1 = t0 + nt - 1;
+  const int places = nt + kSegmentCost, hr = (int)(in / places);
+  const long long t0 = box[2] + (long long)hr * places, t1 = t0 + nt - 1;
   griddep_wait();
   griddep_launch_dependents();
-  if (at == t0 || total * (border - 1) / p.grid > t0) return;
+  if (at == t0 || at > t1 || total * (border - 1) / p.grid > t0) return;
   const int c0 = border - 1, c1 = (int)(((t1 + 1) * p.grid - 1) / total);
   const int h = hr / p.row_blocks, rb = hr % p.row_blocks, rows = p.Sq * p.group;
   const int half = threadIdx.x / (kThreads / 2), i = threadIdx.x % (kThreads / 2);
-  const int pg = i / PER_ROW, d = i % PER_ROW * 8, r = blockIdx.y * 2 + half, rr = rb * ROWS + r;
-  float top = -INFINITY, sum = 0.f, x[8] = {};
-  auto take = [&](float2 ml, const float (&v)[8]) {
-    const float now = fmaxf(top, ml.x);
-    const float safe = now == -INFINITY ? 0.f : now;
-    const float old = ex2(top - safe), e = ex2(ml.x - safe);
-    top = now;
-    sum = fmaf(e, ml.y, sum * old);
+  const int pg = i / PER_ROW, d = i % PER_ROW * 8;
+  for (int pair = blockIdx.y; pair < ROWS / 2; pair += gridDim.y) {
+    const int r = pair * 2 + half, rr = rb * ROWS + r;
+    float top = -INFINITY, sum = 0.f, x[8] = {};
+    auto take = [&](float2 ml, const float (&v)[8]) {
+      const float now = fmaxf(top, ml.x);
+      const float safe = now == -INFINITY ? 0.f : now;
+      const float old = ex2(top - safe), e = ex2(ml.x - safe);
+      top = now;
+      sum = fmaf(e, ml.y, sum * old);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = fmaf(e, v[j], x[j] * old);
-  };
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(e, v[j], x[j] * old);
+    };
 #pragma unroll 4
-  for (int c = c0 + pg; c <= c1; c += P) {
-    if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
-    const long long slot = (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r;
-    const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
-    const float4 u = src[0], v = src[1];
-    take(p.part_ml[slot], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
-  }
-  part_x[half][pg][d / 4] = make_float4(x[0], x[1], x[2], x[3]);
-  part_x[half][pg][d / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
-  if (d == 0) part_ml[half][pg] = make_float2(top, sum);
-  __syncthreads();
-  if (pg != 0 || rr >= rows) return;
+    for (int c = c0 + pg; c <= c1; c += P) {
+      if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
+      const long long slot = (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r;
+      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
+      const float4 u = src[0], v = src[1];
+      take(p.part_ml[slot], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
+    }
+    part_x[half][pg][d / 4] = make_float4(x[0], x[1], x[2], x[3]);
+    part_x[half][pg][d / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+    if (d == 0) part_ml[half][pg] = make_float2(top, sum);
+    __syncthreads();
+    if (pg == 0 && rr < rows) {
 #pragma unroll
-  for (int k = 1; k < P; ++k) {
-    const float4 u = part_x[half][k][d / 4], v = part_x[half][k][d / 4 + 1];
-    take(part_ml[half][k], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
+      for (int k = 1; k < P; ++k) {
+        const float4 u = part_x[half][k][d / 4], v = part_x[half][k][d / 4 + 1];
+        take(part_ml[half][k], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
+      }
+      write_row<D>(p, b, h, rr, d, top, sum, x);
+    }
+    __syncthreads();
   }
-  write_row<D>(p, b, h, rr, d, top, sum, x);
 }
 
 template <typename T, int D, int BITS, int NT>
 int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv, bool split,
                   cudaStream_t st) {
-  using C = Cfg<D, BITS>;
+  using C = Cfg<D, BITS, NT>;
   auto kernel = fa_decode_kernel<T, D, BITS, NT>;
   constexpr int kTag = 1000 + ((sizeof(T) == 2 && Elem<T>::kIdescAB == 0) ? 0 : 1) + 2 * NT +
                        8 * (BITS == 4) + 16 * D;
@@ -858,8 +899,11 @@ int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
   if (launch_pdl(kernel, dim3(p.grid), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
     return FA_ERR_LAUNCH;
   if (!split) return FA_OK;
-  return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid - 1, 4 * NT), dim3(kThreads), 0,
-                    st, p) == cudaSuccess
+  // Many shares to a segment (few segments): its rows are spread over CTAs, too.
+  const long long segs = (long long)p.B * p.kv.heads * p.row_blocks;
+  const unsigned y = p.grid > 8 * segs ? 4 * NT : NT;
+  return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid - 1, y), dim3(kThreads), 0, st,
+                    p) == cudaSuccess
              ? FA_OK
              : FA_ERR_LAUNCH;
 }
@@ -899,13 +943,12 @@ int launch_decode_any(DecodeParams& p, int nt, const CUtensorMap& tk, const CUte
   }
 }
 
-int tile_tokens(int D, int bits) { return (bits == 16 && D == 128) ? 64 : 128; }
-
-int ctas_per_sm(int D, int bits, int nt) { return bits == 16 || nt > 1 ? 2 : 3; }
+// Tokens up to which a segment is not split.
+constexpr int kWholeTokens = 1024;
 
 struct Plan {
   int nt, row_blocks, grid;
-  bool split;
+  bool split;  // segments may cross shares: a second launch joins them
 };
 
 // Query rows in as few row blocks as the registers allow; as many CTAs as
@@ -916,12 +959,15 @@ Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen,
   const int most_rows = 8 * max_nt(c->head_dim);
   pl.row_blocks = (int)((rows + most_rows - 1) / most_rows);
   pl.nt = (int)((rows + 8LL * pl.row_blocks - 1) / (8LL * pl.row_blocks));
-  const int tile = tile_tokens(c->head_dim, c->bits);
+  const int tile = kWarps * kBlockTokens * blocks_of(c->head_dim, c->bits, pl.nt);
   const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
   const long long tiles = (long long)batch * c->nheads_kv * pl.row_blocks * per_seg;
-  const long long most = (long long)sm_count() * ctas_per_sm(c->head_dim, c->bits, pl.nt);
-  pl.grid = (int)(tiles < most ? tiles : most);
-  pl.split = per_seg > 1 && pl.grid > 1;
+  const long long most = (long long)sm_count() * kCtas;
+  // Short tables: a CTA per segment, no join.
+  const long long segs = tiles / per_seg;
+  pl.split = (long long)table_width * c->page_size > kWholeTokens || segs > (1LL << 30);
+  pl.grid = (int)(!pl.split ? segs : tiles < most ? tiles : most);
+  if (pl.grid == 1) pl.split = false;
   return pl;
 }
 
@@ -991,6 +1037,7 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   p.causal = causal ? 1 : 0;
   while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
   p.grid = pl.grid;
+  p.whole = !pl.split && pl.grid > 1;
   p.negate = sm_scale < 0.f;
   p.bf16 = cache->dtype == FA_DTYPE_BF16;
   p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);

@@ -64,7 +64,8 @@ struct AppendParams {
   const int* starts;
   const int* counts;       // null: every token is new
   const double* inv_freq;  // null: no rotation
-  int S, half, per_cta, per_seq, page_shift, chunk_shift;
+  FastDiv per_seq, q_heads, k_heads;  // CTAs of a sequence, heads of q (0 without q), of k and v
+  int S, half, per_cta, page_shift, chunk_shift;
   float magnitude;
 };
 
@@ -128,41 +129,47 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                     Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
 }
 
-// Where the angle of pair i stands: the 8 angles of a thread's dims are `half / 8`
-// apart, so that neighbouring threads read neighbouring words (WIDE: half % 8
-// == 0); interleaved pairs, of which a thread has 4, likewise.
-template <bool INTER, bool WIDE>
-__device__ __forceinline__ int angle_at(int i, int half) {
-  constexpr int N = INTER ? 4 : 8;
-  return WIDE ? i % N * (half / N) + i / N : i;
-}
-
-// Rotates the 8 dims e.. of a row (the thread's own values in x, WIDE: those of
-// the partner dims in y).
-template <typename T, bool INTER, bool WIDE>
-__device__ __forceinline__ void rotate8(const T* row, int e, int half, const float2* cs,
-                                        float (&x)[8], float (&y)[8]) {
+// Rotates the 8 dims e.. of a row whose own values are x.  WIDE: the thread's
+// angles stand `stride` apart from `w` on (neighbouring lanes read neighbouring
+// words), the partner dims' values are y, and `sign` is -1 in the first halves.
+// Otherwise `w` holds the angles in order and partner dims are read from `row`.
+template <bool INTER>
+__device__ __forceinline__ void rotate_wide(const float2* w, int stride, float sign, float (&x)[8],
+                                            const float (&y)[8]) {
   if constexpr (INTER) {
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
-      if (WIDE || e + i < 2 * half) {
-        const float2 w = cs[angle_at<INTER, WIDE>((e + i) / 2, half)];
-        const float a = x[i], b = x[i + 1];
-        x[i] = a * w.x - b * w.y;
-        x[i + 1] = b * w.x + a * w.y;
-      }
+      const float2 c = w[i / 2 * stride];
+      const float a = x[i], b = x[i + 1];
+      x[i] = a * c.x - b * c.y;
+      x[i + 1] = b * c.x + a * c.y;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int d = e + i;
-      if (!WIDE) {
-        if (d >= 2 * half) break;
-        y[i] = Elem<T>::value(reinterpret_cast<const uint16_t*>(row)[d < half ? d + half : d - half]);
-      }
+      const float2 c = w[i * stride];
+      x[i] = x[i] * c.x + sign * y[i] * c.y;
+    }
+  }
+}
+template <typename T, bool INTER>
+__device__ __forceinline__ void rotate_any(const uint16_t* row, int e, int half, const float2* w,
+                                           float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = e + i;
+    if (d >= 2 * half) break;
+    if constexpr (INTER) {
+      if (i % 2) continue;
+      const float2 c = w[d / 2];
+      const float a = x[i], b = x[i + 1];
+      x[i] = a * c.x - b * c.y;
+      x[i + 1] = b * c.x + a * c.y;
+    } else {
       const bool first = d < half;
-      const float2 w = cs[angle_at<INTER, WIDE>(first ? d : d - half, half)];
-      x[i] = x[i] * w.x + (first ? -y[i] : y[i]) * w.y;
+      const float2 c = w[first ? d : d - half];
+      const float y = Elem<T>::value(row[first ? d + half : d - half]);
+      x[i] = x[i] * c.x + (first ? -y : y) * c.y;
     }
   }
 }
@@ -171,119 +178,114 @@ __device__ __forceinline__ void rotate8(const T* row, int e, int half, const flo
 // once, every output written once) and by latency for single tokens: one
 // launch does the rotation of q and k, the page lookup and both writes.
 // A CTA takes whole tokens of one sequence; it makes their cosines and sines
-// and finds their places in the cache once for all heads.  The rows are the
-// heads of q, k and v of each token, D/8 threads to a row; a thread holds 8
-// consecutive dims (the half layout reads the partner dims a second time, from
-// L1) and steps down the rows with additions alone.  The 4 lanes that hold a
-// group of 32 dims reduce its minimum and maximum by shuffles.
-// WIDE: 16-byte loads, and rotated dims that end at a thread's border.
+// and finds their places in the cache once for all heads.  An item is 8
+// consecutive dims of a head of q, k or v (the half layout reads the partner
+// dims a second time, from L1).  The items of q, k and v start at multiples of
+// 32, so a warp works on one of them, and the 4 lanes that hold a group of 32
+// dims reduce its minimum and maximum by shuffles.
+// WIDE: 16-byte loads at 32-bit offsets, and rotated dims that end at an item's
+// border.
 template <typename T, bool INTER, int BITS, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendParams p) {
   extern __shared__ float2 cs[];
   griddep_wait();
   griddep_launch_dependents();
   const KvView& kv = p.kv;
-  const int b = blockIdx.x / p.per_seq, s0 = (blockIdx.x - b * p.per_seq) * p.per_cta;
+  const int b = p.per_seq.div(blockIdx.x), s0 = (blockIdx.x - b * p.per_seq.d) * p.per_cta;
   const int ntok = min(p.per_cta, p.S - s0);
   int* places = reinterpret_cast<int*>(cs + p.per_cta * p.half);  // row of head 0, or -1
-  const int hq = p.part[0].heads, hk = kv.heads, heads = hq + 2 * hk;
-  const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), e = c * 8;
-  const int row = threadIdx.x >> p.chunk_shift, step = kThreads >> p.chunk_shift;
-  const int step_tok = step / heads, step_h = step - step_tok * heads;
-  int tok = row / heads, h = row - tok * heads;
-  const bool turning = e < 2 * p.half;
-
+  const int hk = kv.heads;
   const long long first = (long long)p.starts[b] + s0;
-  for (int i = threadIdx.x; i < ntok; i += kThreads) {
-    int at = -1;
-    if (p.counts == nullptr || s0 + i < p.counts[b]) {
-      const long long pos = first + i;
-      const int id = kv.page_of(b, pos, p.page_shift);
-      if (id < 0)
-        kv.report(kStatusPage);
-      else
-        at = ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
-    }
-    places[i] = at;
+  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, p.counts[b] - s0));  // tokens to store
+  const int nq = (ntok * (int)p.q_heads.d) << p.chunk_shift, nk = (fresh * hk) << p.chunk_shift;
+  const int k0 = (nq + 31) & ~31, v0 = k0 + ((nk + 31) & ~31), end = v0 + ((nk + 31) & ~31);
+  for (int i = threadIdx.x; i < fresh; i += kThreads) {
+    const long long pos = first + i;
+    const int id = kv.page_of(b, pos, p.page_shift);
+    if (id < 0) kv.report(kStatusPage);
+    places[i] = id < 0 ? -1 : ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
   }
+  const int mask = (1 << p.chunk_shift) - 1;
+  T* q_out = static_cast<T*>(p.q_out) + ((((long long)b * p.S + s0) * p.q_heads.d) << (p.chunk_shift + 3));
 
-  bool filled = false;
-  // the same number of rounds for all lanes of a warp: the warp's first row leads
-  int lead_tok = (int)((threadIdx.x & ~31u) >> p.chunk_shift) / heads;
-  int lead_h = (int)((threadIdx.x & ~31u) >> p.chunk_shift) - lead_tok * heads;
-  while (lead_tok < ntok || !filled) {
+  for (int base = threadIdx.x; base < end || base < kThreads; base += 2 * kThreads) {
     uint4 own[2], other[2];
-    int rt[2], rh[2];
+    const T* at[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      rt[u] = tok;
-      rh[u] = h;
-      if (WIDE && tok < ntok) {
-        const int part = h < hq ? 0 : h < hq + hk ? 1 : 2;
-        const AppendPart& src = p.part[part];
-        const T* at = static_cast<const T*>(src.in) + b * src.sb + (s0 + tok) * src.ss +
-                      (h - (part == 0 ? 0 : part == 1 ? hq : hq + hk)) * src.sh;
-        own[u] = *reinterpret_cast<const uint4*>(at + e);
-        if (!INTER && turning && part < 2)
-          other[u] = *reinterpret_cast<const uint4*>(at + (e < p.half ? e + p.half : e - p.half));
-      }
-      tok += step_tok;
-      h += step_h;
-      if (h >= heads) {
-        h -= heads;
-        ++tok;
-      }
-      lead_tok += step_tok;
-      lead_h += step_h;
-      if (lead_h >= heads) {
-        lead_h -= heads;
-        ++lead_tok;
+      const int it = base + u * kThreads;
+      const int part = it < k0 ? 0 : it < v0 ? 1 : 2;  // the same in all lanes of a warp
+      const int i = it - (part == 0 ? 0 : part == 1 ? k0 : v0);
+      const AppendPart& src = p.part[part];
+      const int row = i >> p.chunk_shift, e = (i & mask) * 8;
+      const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
+      const int tok = heads.div(row), h = row - tok * heads.d;
+      const T* from = static_cast<const T*>(src.in) + b * src.sb + s0 * src.ss;
+      if (WIDE) {
+        at[u] = from + (tok * (int)src.ss + h * (int)src.sh);
+        if (i < (part == 0 ? nq : nk) && it < end) {
+          own[u] = *reinterpret_cast<const uint4*>(at[u] + e);
+          if (!INTER && part < 2 && e < 2 * p.half)
+            other[u] = *reinterpret_cast<const uint4*>(at[u] + (e < p.half ? e + p.half : e - p.half));
+        }
+      } else {
+        at[u] = from + (tok * src.ss + h * src.sh);
       }
     }
-    if (!filled) {
+    if (base < kThreads) {
+      constexpr int N = INTER ? 4 : 8;  // pairs of an item
       for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
-        const int at = i / p.half, f = i - at * p.half;
-        cs[at * p.half + angle_at<INTER, WIDE>(f, p.half)] =
-            rotary_cos_sin((double)(first + at), p.inv_freq[f], p.magnitude);
+        const int tok = i / p.half, f = i - tok * p.half;
+        cs[tok * p.half + (WIDE ? f % N * (p.half / N) + f / N : f)] =
+            rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
       }
       __syncthreads();
-      filled = true;
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const bool there = rt[u] < ntok;
-      const int part = rh[u] < hq ? 0 : rh[u] < hq + hk ? 1 : 2;
-      const int hp = rh[u] - (part == 0 ? 0 : part == 1 ? hq : hq + hk);
-      float x[8] = {}, y[8];
+      const int it = base + u * kThreads;
+      if (it >= end) break;  // whole warps
+      const int part = it < k0 ? 0 : it < v0 ? 1 : 2;
+      const int i = it - (part == 0 ? 0 : part == 1 ? k0 : v0);
+      const bool there = i < (part == 0 ? nq : nk);
+      const int row = i >> p.chunk_shift, c = i & mask, e = c * 8;
+      const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
+      const int tok = there ? heads.div(row) : 0, h = row - tok * heads.d;
+      float x[8] = {};
       if (there) {
-        const AppendPart& src = p.part[part];
-        const T* at = static_cast<const T*>(src.in) + b * src.sb + (s0 + rt[u]) * src.ss + hp * src.sh;
+        const bool turns = part < 2 && e < 2 * p.half;
+        const float2* w = cs + tok * p.half;
         if (WIDE) {
           unpack8<T>(own[u], x);
-          if (!INTER && turning) unpack8<T>(other[u], y);
+          if (turns) {
+            float y[8];
+            if (!INTER) unpack8<T>(other[u], y);
+            const bool lower = e < p.half;
+            rotate_wide<INTER>(w + (INTER || lower ? c : c - p.half / 8), p.half / (INTER ? 4 : 8),
+                               lower ? -1.f : 1.f, x, y);
+          }
         } else {
+          const uint16_t* raw = reinterpret_cast<const uint16_t*>(at[u]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = Elem<T>::value(reinterpret_cast<const uint16_t*>(at)[e + i]);
+          for (int k = 0; k < 8; ++k) x[k] = Elem<T>::value(raw[e + k]);
+          if (turns) rotate_any<T, INTER>(raw, e, p.half, w, x);
         }
-        if (part < 2 && turning) rotate8<T, INTER, WIDE>(at, e, p.half, cs + rt[u] * p.half, x, y);
-        if (part == 0)
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) +
-                                    (((long long)b * p.S + s0 + rt[u]) * hq + hp) * kv.D + e) = pack8<T>(x);
+        if (part == 0) *reinterpret_cast<uint4*>(q_out + (long long)i * 8) = pack8<T>(x);
       }
-      const int place = there && part > 0 ? places[rt[u]] : -1;
-      const int at = place + (hp << p.page_shift);  // row of the cache
+      if (part == 0) continue;
+      const int place = there ? places[tok] : -1;
+      const int to = place + (h << p.page_shift);  // row of the cache
       if (BITS == 16) {
         if (place >= 0)
-          *reinterpret_cast<uint4*>((part == 1 ? kv.k : kv.v) + ((long long)at * kv.D + e) * 2) = pack8<T>(x);
+          *reinterpret_cast<uint4*>((part == 1 ? kv.k : kv.v) + ((long long)to * kv.D + e) * 2) = pack8<T>(x);
         continue;
       }
-      if (!__any_sync(0xffffffffu, place >= 0)) continue;
       uint32_t code[8];
       const uint32_t sm = quantise(x, code);
       if (place < 0) continue;
       const Kv4 lay(kv.D);
-      const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = at % kBlockTokens;
-      uint8_t* blk = kv.k + (long long)(at / kBlockTokens) * lay.bytes();
+      const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = to % kBlockTokens;
+      uint8_t* blk = kv.k + (long long)(to / kBlockTokens) * lay.bytes();
       if (part == 1) {
         const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 |
                            code[3] << 20 | code[5] << 24 | code[7] << 28;
@@ -301,9 +303,9 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
         }
         if (t4 == 0) {
           uint16_t* vp = reinterpret_cast<uint16_t*>(blk + lay.v_params());
-          const int i = (grp * 4 + tt) * 4 + tp * 2 + hi;
-          vp[i] = (uint16_t)sm;
-          vp[i + 16 * NG] = (uint16_t)(sm >> 16);
+          const int k = (grp * 4 + tt) * 4 + tp * 2 + hi;
+          vp[k] = (uint16_t)sm;
+          vp[k + 16 * NG] = (uint16_t)(sm >> 16);
         }
       }
     }
@@ -337,148 +339,174 @@ struct ReadParams {
   const int* lengths;
   void* k_out;  // (batch, max_len, heads, D)
   void* v_out;
-  int max_len, page_shift, chunk_shift;
+  int max_len, page_shift;
 };
 
 // 4-bit codes to values: a nibble pair masked out of its word is two fp16
 // subnormals (c 2^-24 from bits 0..3, c 2^-20 from bits 4..7), which convert
-// exactly; `s24` and `s20` are the scale times 2^24 and 2^20.
+// exactly.
 __device__ __forceinline__ float2 pair_of(uint32_t masked) {
   return __half22float2(*reinterpret_cast<const __half2*>(&masked));
 }
+template <int N>
+__device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = *at;
+  }
+}
 
 // The cached tokens as contiguous K and V, rows behind a sequence's length
-// zero.  Bound by HBM: the cache is read once, K and V written once.  A CTA
-// takes one 16-token block of a sequence, all heads; an item is 8 dims of one
-// token (of two neighbouring tokens for 4-bit V, whose words hold both), so
-// stores are 16 bytes wide and contiguous over a token's heads.
-template <typename T, int BITS>
+// zero.  Bound by HBM: the cache is read once, K and V written once.  A warp
+// takes one 16-token block of one head and has all its loads in flight at
+// once.  4-bit: lane (g, t) = (lane / 4, lane % 4) reads the words that it
+// would read in the attention kernel, each once: 8 dims of each group of tokens
+// g and g + 8 (K), 4 dims of each group of tokens 2 t, 2 t + 1 and the two 8
+// further (V); a store instruction writes whole 32-byte sectors.
+template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kThreads) fa_kv_read_kernel(const ReadParams p) {
   griddep_wait();
   griddep_launch_dependents();
   const KvView& kv = p.kv;
-  const int D = kv.D, b = blockIdx.y, first = blockIdx.x * kBlockTokens;
+  const int b = blockIdx.y, first = blockIdx.x * kBlockTokens, lane = threadIdx.x % 32;
+  const int h = blockIdx.z * (kThreads / 32) + threadIdx.x / 32;
   const int given = p.lengths[b], len = min(kv.clamp_length(given), p.max_len);
-  if (kv.bad_length(given) && blockIdx.x == 0 && threadIdx.x == 0) kv.report(kStatusPage);
-  const int there = max(0, min(len - first, kBlockTokens));  // tokens of the block to copy
-  const int rows = min(p.max_len - first, kBlockTokens);     // tokens of the block to write
+  const bool speaks = lane == 0 && h == 0;
+  if (kv.bad_length(given) && blockIdx.x == 0 && speaks) kv.report(kStatusPage);
+  if (h >= kv.heads) return;
+  const int rows = min(p.max_len - first, kBlockTokens);  // tokens of the block to write
+  int copied = max(0, min(len - first, kBlockTokens));    // and to copy
   int id = -1;
-  if (there > 0) {
+  if (copied > 0) {
     id = kv.page_of(b, first, p.page_shift);
-    if (id < 0 && threadIdx.x == 0) kv.report(kStatusPage);
+    if (id < 0 && speaks) kv.report(kStatusPage);
   }
-  const int copied = id < 0 ? 0 : there;
-  uint4* k_out = reinterpret_cast<uint4*>(static_cast<T*>(p.k_out) + ((long long)b * p.max_len + first) * kv.heads * D);
-  uint4* v_out = reinterpret_cast<uint4*>(static_cast<T*>(p.v_out) + ((long long)b * p.max_len + first) * kv.heads * D);
-  const int per_token = kv.heads << p.chunk_shift;
-  if (copied < rows) {  // zero the rest
+  if (id < 0) copied = 0;
+  constexpr int CHUNKS = D / 8;
+  // of token 0 of the block, in 16-byte vectors; a token is `pitch` further
+  const int pitch = kv.heads * CHUNKS;
+  const long long out = (((long long)b * p.max_len + first) * kv.heads + h) * CHUNKS;
+  uint4* k_out = static_cast<uint4*>(p.k_out) + out;
+  uint4* v_out = static_cast<uint4*>(p.v_out) + out;
+  const int at = id < 0 ? 0 : (((id * kv.heads + h) << p.page_shift) | (first & (kv.page - 1)));
+  if (copied < rows) {
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int i = copied * per_token + threadIdx.x; i < rows * per_token; i += kThreads) {
-      k_out[i] = zero;
-      v_out[i] = zero;
+    for (int i = copied * CHUNKS + lane; i < rows * CHUNKS; i += 32) {
+      const int o = i / CHUNKS * pitch + i % CHUNKS;
+      k_out[o] = zero;
+      v_out[o] = zero;
     }
+    if (copied == 0) return;
   }
-  // row of the cache: head 0, the block's first token
-  const int at0 = id < 0 ? 0 : ((id * kv.heads) << p.page_shift) | (first & (kv.page - 1));
-  const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), row = threadIdx.x >> p.chunk_shift;
-  const int step = kThreads >> p.chunk_shift;
-  const int step_tok = step / kv.heads, step_h = step - step_tok * kv.heads;
-  const int tok0 = row / kv.heads, h0 = row - tok0 * kv.heads;
-  auto next = [&](int& tok, int& h) {
-    tok += step_tok;
-    h += step_h;
-    if (h >= kv.heads) {
-      h -= kv.heads;
-      ++tok;
-    }
-  };
-  auto out_at = [&](int tok, int h) { return tok * per_token + (h << p.chunk_shift) + c; };
-  if (BITS == 16) {
-    const uint4* ks = reinterpret_cast<const uint4*>(kv.k);
-    const uint4* vs = reinterpret_cast<const uint4*>(kv.v);
-    int tok = tok0, h = h0;
-    while (tok < copied) {
-      uint4 x[4], y[4];
-      int o[4];
+  if constexpr (BITS == 16) {
+    constexpr int N = (16 * CHUNKS + 31) / 32;  // vectors of a lane
+    const uint4* ks = reinterpret_cast<const uint4*>(kv.k) + (long long)at * CHUNKS;
+    const uint4* vs = reinterpret_cast<const uint4*>(kv.v) + (long long)at * CHUNKS;
+    uint4 x[N], y[N];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        o[u] = -1;
-        if (tok < copied) {
-          const long long at = ((long long)(at0 + (h << p.page_shift) + tok) << p.chunk_shift) + c;
-          x[u] = ks[at];
-          y[u] = vs[at];
-          o[u] = out_at(tok, h);
-        }
-        next(tok, h);
+    for (int u = 0; u < N; ++u)
+      if (u * 32 + lane < copied * CHUNKS) {
+        x[u] = ks[u * 32 + lane];
+        y[u] = vs[u * 32 + lane];
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (o[u] >= 0) {
-          k_out[o[u]] = x[u];
-          v_out[o[u]] = y[u];
-        }
-    }
-    return;
-  }
-  const Kv4 lay(D);
-  const int NG = lay.groups(), grp = c / 4, t4 = c % 4;
-  auto block = [&](int h) {
-    return kv.k + (long long)((at0 + (h << p.page_shift)) / kBlockTokens) * lay.bytes();
-  };
-  {
-    int r = tok0, h = h0;
-    while (r < copied) {
-      uint32_t w[2], sm[2];
-      int o[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        o[u] = -1;
-        if (r < copied) {
-          const uint8_t* blk = block(h);
-          w[u] = reinterpret_cast<const uint32_t*>(blk)[(r * 4 + t4) * NG + grp];
-          sm[u] = reinterpret_cast<const uint32_t*>(blk + lay.k_params())[r * NG + grp];
-          o[u] = out_at(r, h);
-        }
-        next(r, h);
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (o[u] < 0) continue;
-        const float2 par = pair_of(sm[u]);
-        const float s24 = par.x * 0x1p24f, s20 = par.x * 0x1p20f;
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = pair_of((i < 2 ? w[u] : w[u] >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
-          x[2 * i] = fmaf(i % 2 ? s20 : s24, f.x, par.y);
-          x[2 * i + 1] = fmaf(i % 2 ? s20 : s24, f.y, par.y);
-        }
-        k_out[o[u]] = pack8<T>(x);
+    for (int u = 0; u < N; ++u) {
+      const int i = u * 32 + lane;
+      if (i < copied * CHUNKS) {
+        k_out[i / CHUNKS * pitch + i % CHUNKS] = x[u];
+        v_out[i / CHUNKS * pitch + i % CHUNKS] = y[u];
       }
     }
-  }
-  const int pairs = (copied + 1) / 2, g = t4 * 2;
-  int rp = tok0, h = h0;
-  while (rp < pairs) {
-    const uint8_t* blk = block(h);
-    const int tp = rp / 4, tt = rp % 4;
+  } else {
+    constexpr Kv4 lay(D);
+    constexpr int NG = lay.groups();
+    const int g = lane / 4, t = lane % 4;
+    const uint8_t* blk = kv.k + (long long)(at / kBlockTokens) * lay.bytes();
+    const uint32_t* kc = reinterpret_cast<const uint32_t*>(blk);
+    const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + lay.k_params());
     const uint32_t* vc = reinterpret_cast<const uint32_t*>(blk + lay.v_codes());
-    const uint32_t w0 = vc[((tp * 8 + g) * 4 + tt) * NG + grp];
-    const uint32_t w1 = vc[((tp * 8 + g + 1) * 4 + tt) * NG + grp];
-    const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + lay.v_params()) + (grp * 4 + tt) * 2 + tp;
-    const float2 s = pair_of(vp[0]), m = pair_of(vp[8 * NG]);  // of both tokens
-    const int o = out_at(2 * rp, h);
-    float x[2][8];
+    const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + lay.v_params());
+    uint32_t k[2][NG], kq[2][NG], v[2][NG], vs[2 * NG], vm[2 * NG];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t w = i < 4 ? w0 : w1;
-      const float2 f = pair_of((i % 4 < 2 ? w : w >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
-      x[0][i] = fmaf(s.x * (i % 2 ? 0x1p20f : 0x1p24f), f.x, m.x);
-      x[1][i] = fmaf(s.y * (i % 2 ? 0x1p20f : 0x1p24f), f.y, m.y);
+    for (int n = 0; n < 2; ++n) {
+      load_words<NG>(kc + (n * 32 + lane) * NG, k[n]);
+      load_words<NG>(kp + (n * 8 + g) * NG, kq[n]);
+      load_words<NG>(vc + (n * 32 + lane) * NG, v[n]);
     }
-    v_out[o] = pack8<T>(x[0]);
-    if (2 * rp + 1 < copied) v_out[o + per_token] = pack8<T>(x[1]);
-    next(rp, h);
+#pragma unroll
+    for (int grp = 0; grp < NG; ++grp) {  // the four tokens' scales and minima
+      const uint2 s = *reinterpret_cast<const uint2*>(vp + (grp * 4 + t) * 2);
+      const uint2 m = *reinterpret_cast<const uint2*>(vp + 8 * NG + (grp * 4 + t) * 2);
+      vs[2 * grp] = s.x;
+      vs[2 * grp + 1] = s.y;
+      vm[2 * grp] = m.x;
+      vm[2 * grp + 1] = m.y;
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int r = n * 8 + g;
+      if (r < copied) {
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          const float2 sm = pair_of(kq[n][grp]);
+          const float s24 = sm.x * 0x1p24f, s20 = sm.x * 0x1p20f;
+          float x[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = pair_of((i < 2 ? k[n][grp] : k[n][grp] >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
+            x[2 * i] = fmaf(i % 2 ? s20 : s24, c.x, sm.y);
+            x[2 * i + 1] = fmaf(i % 2 ? s20 : s24, c.y, sm.y);
+          }
+          k_out[r * pitch + grp * 4 + t] = pack8<T>(x);
+        }
+      }
+      const int r0 = n * 8 + 2 * t;
+      if (r0 < copied) {
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          const float2 s = pair_of(vs[2 * grp + n]), m = pair_of(vm[2 * grp + n]);  // of both tokens
+          float2 c[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            c[i] = pair_of((i < 2 ? v[n][grp] : v[n][grp] >> 8) & (i % 2 ? 0x00F000F0u : 0x000F000Fu));
+          float x[4], y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = fmaf(s.x * (i % 2 ? 0x1p20f : 0x1p24f), c[i].x, m.x);
+            y[i] = fmaf(s.y * (i % 2 ? 0x1p20f : 0x1p24f), c[i].y, m.y);
+          }
+          uint2* to = reinterpret_cast<uint2*>(v_out + r0 * pitch) + grp * 8 + g;
+          to[0] = make_uint2(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]));
+          if (r0 + 1 < copied)
+            to[2 * pitch] = make_uint2(Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]));
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int D>
+cudaError_t launch_read(const ReadParams& p, dim3 grid, cudaStream_t st) {
+  if (p.kv.bits == 16) return launch_pdl(fa_kv_read_kernel<T, D, 16>, grid, dim3(kThreads), 0, st, p);
+  if constexpr (D >= 32) return launch_pdl(fa_kv_read_kernel<T, D, 4>, grid, dim3(kThreads), 0, st, p);
+  return cudaErrorInvalidValue;
+}
+template <typename T>
+cudaError_t launch_read_d(const ReadParams& p, dim3 grid, cudaStream_t st) {
+  switch (p.kv.D) {
+    case 16: return launch_read<T, 16>(p, grid, st);
+    case 32: return launch_read<T, 32>(p, grid, st);
+    case 64: return launch_read<T, 64>(p, grid, st);
+    default: return launch_read<T, 128>(p, grid, st);
   }
 }
 
@@ -491,9 +519,12 @@ int log2_of(int x) {
 bool bad_append_part(const fa_sm100_heads& x) {
   return !x.in || x.heads < 1 || (reinterpret_cast<uintptr_t>(x.in) & 1u);
 }
-bool wide(const fa_sm100_heads& x) {
+// 16-byte vectors, and a CTA's tokens within 2^31 elements.
+bool wide(const fa_sm100_heads& x, long long tokens) {
+  const double reach = (double)tokens * (x.stride_seq < 0 ? -x.stride_seq : x.stride_seq) +
+                       (double)x.heads * (x.stride_head < 0 ? -x.stride_head : x.stride_head);
   return !(reinterpret_cast<uintptr_t>(x.in) & 15u) &&
-         !((x.stride_batch | x.stride_seq | x.stride_head) & 7);
+         !((x.stride_batch | x.stride_seq | x.stride_head) & 7) && reach < 2147480000.0;
 }
 
 }  // namespace
@@ -533,17 +564,19 @@ extern "C" int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100
   p.magnitude = magnitude;
   p.page_shift = log2_of(cache->page_size);
   p.chunk_shift = log2_of(cache->head_dim / 8);
-  const bool is_wide = wide(*k) && wide(*v) && (!q || wide(*q)) &&
-                       (interleaved ? p.half % 4 : p.half % 8) == 0;
-  // whole tokens until every thread has four items
-  const long long per_token = (long long)(p.part[0].heads + 2 * k->heads) * (cache->head_dim / 8);
-  long long per_cta = 4 * kThreads / per_token;
+  // whole tokens until every thread has two items: one round
+  const long long per_token = (long long)((q ? q->heads : 0) + 2 * k->heads) * (cache->head_dim / 8);
+  long long per_cta = 2 * kThreads / per_token;
   if (p.half > 0 && per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
   if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
   p.per_cta = (int)per_cta;
-  p.per_seq = (int)((seqlen + per_cta - 1) / per_cta);
-  const long long grid = (long long)p.per_seq * batch;
+  const bool is_wide = wide(*k, per_cta) && wide(*v, per_cta) && (!q || wide(*q, per_cta)) &&
+                       (interleaved ? p.half % 4 : p.half % 8) == 0;
+  p.per_seq = FastDiv((unsigned)((seqlen + per_cta - 1) / per_cta));
+  p.k_heads = FastDiv((unsigned)k->heads);
+  if (q) p.q_heads = FastDiv((unsigned)q->heads);
+  const long long grid = (long long)p.per_seq.d * batch;
   if (grid > 2147483647LL) return FA_ERR_ARG;
   const size_t smem = (size_t)per_cta * (p.half * sizeof(float2) + sizeof(int));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -572,16 +605,11 @@ extern "C" int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_
   p.v_out = v_out;
   p.max_len = max_len;
   p.page_shift = log2_of(cache->page_size);
-  p.chunk_shift = log2_of(cache->head_dim / 8);
-  const dim3 grid((unsigned)(((long long)max_len + kBlockTokens - 1) / kBlockTokens), (unsigned)batch);
+  constexpr int kWarps = kThreads / 32;
+  const dim3 grid((unsigned)(((long long)max_len + kBlockTokens - 1) / kBlockTokens), (unsigned)batch,
+                  (unsigned)((cache->nheads_kv + kWarps - 1) / kWarps));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e;
-  if (cache->dtype == FA_DTYPE_BF16)
-    e = cache->bits == 16
-            ? launch_pdl(fa_kv_read_kernel<__nv_bfloat16, 16>, grid, dim3(kThreads), 0, st, p)
-            : launch_pdl(fa_kv_read_kernel<__nv_bfloat16, 4>, grid, dim3(kThreads), 0, st, p);
-  else
-    e = cache->bits == 16 ? launch_pdl(fa_kv_read_kernel<__half, 16>, grid, dim3(kThreads), 0, st, p)
-                          : launch_pdl(fa_kv_read_kernel<__half, 4>, grid, dim3(kThreads), 0, st, p);
+  const cudaError_t e = cache->dtype == FA_DTYPE_BF16 ? launch_read_d<__nv_bfloat16>(p, grid, st)
+                                                      : launch_read_d<__half>(p, grid, st);
   return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }

@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "fa_kernels.h"
 #include "fa_rotary.cuh"
 #include "sm100_ptx.cuh"
@@ -22,7 +24,8 @@ namespace fa_sm100 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 2;          // vectors (pairs of vectors) in flight per thread
+// Vectors (half: pairs of vectors) in flight per thread: 64 bytes of loads.
+__host__ __device__ constexpr int items_of(bool interleaved) { return interleaved ? 4 : 2; }
 constexpr int kMaxAngles = 4096;   // cosines and sines of a CTA: 32 KB
 
 struct RotaryPart {
@@ -39,125 +42,112 @@ struct RotaryParams {
   long long pos_sb;       // its batch stride
   long long first;        // position of token 0 without `positions`
   int S, D, half, per_cta, pos64;  // per_cta: tokens of a CTA, all of one sequence
-  int per_seq, per_head, width;    // CTAs of a sequence, items of a head, items of a row of threads
+  FastDiv per_seq, per_head, heads;  // CTAs of a sequence, items of a head, heads of q and k
   float magnitude, sign;
 };
 
 // One thread's share of a head (an item): a vector of VEC first halves and the
 // VEC second halves of the same pairs (half), or VEC elements = VEC/2 pairs
-// (interleaved), or VEC elements behind R.  The threads stand as `rows` rows of
-// `width` items; a row is one head of one token, and each thread steps down the
-// rows with additions alone.  A vector's i-th cosine and sine are `turning`
-// apart in shared memory, so the lanes of a row read neighbouring words.
-template <typename T, int VEC, bool INTER>
+// (interleaved), or VEC elements behind R.  A vector's i-th cosine and sine are
+// `turning` apart in shared memory, so neighbouring lanes read neighbouring
+// words.  Addresses inside a CTA's tokens are 32-bit offsets from 64-bit bases
+// where the strides allow it (SMALL).
+template <typename T, int VEC, bool INTER, bool SMALL>
 __global__ void __launch_bounds__(kThreads, 4) fa_rotary_kernel(const RotaryParams p) {
   extern __shared__ float2 cs[];
   griddep_wait();
   griddep_launch_dependents();
   using V = Pack16<VEC>;
-  constexpr int PAIRS = INTER ? VEC / 2 : VEC;
+  using Off = typename std::conditional<SMALL, int, long long>::type;
+  constexpr int PAIRS = INTER ? VEC / 2 : VEC, ITEMS = items_of(INTER);
   const int half = p.half, turning = half / PAIRS;  // items of a head that rotate
-  const int heads = p.q.heads + p.k.heads;
-  const int b = blockIdx.x / p.per_seq, s0 = (blockIdx.x - b * p.per_seq) * p.per_cta;
+  const int b = p.per_seq.div(blockIdx.x), s0 = (blockIdx.x - b * p.per_seq.d) * p.per_cta;
   const int ntok = min(p.per_cta, p.S - s0);
-  const int row = threadIdx.x / p.width, col = threadIdx.x - row * p.width;
-  const int step = kThreads / p.width, step_tok = step / heads, step_h = step - step_tok * heads;
-  int tok = row < step ? row / heads : ntok, h = row - row / heads * heads;
+  const int total = ntok * (int)(p.heads.d * p.per_head.d);
+  const T* in_q = static_cast<const T*>(p.q.in) + b * p.q.sb + s0 * p.q.ss;
+  const T* in_k = static_cast<const T*>(p.k.in) + b * p.k.sb + s0 * p.k.ss;
+  T* out_q = static_cast<T*>(p.q.out) + ((long long)b * p.S + s0) * p.q.heads * p.D;
+  T* out_k = static_cast<T*>(p.k.out) + ((long long)b * p.S + s0) * p.k.heads * p.D;
 
-  auto fill = [&]() {
-    for (int i = threadIdx.x; i < ntok * half; i += kThreads) {
-      const int at = i / half, f = i - at * half;
-      const long long s = s0 + at, where = b * p.pos_sb + s;
-      const long long pos = p.positions == nullptr ? p.first + s
-                            : p.pos64 ? static_cast<const long long*>(p.positions)[where]
-                                      : static_cast<const int*>(p.positions)[where];
-      float2 c = rotary_cos_sin((double)pos, p.inv_freq[f], p.magnitude);
-      c.y *= p.sign;
-      cs[at * half + f % PAIRS * turning + f / PAIRS] = c;
-    }
-    __syncthreads();
-  };
-  bool filled = false;
-  while (tok < ntok || !filled) {
-    for (int j = col; j < p.per_head || !filled; j += p.width) {
-      V a[kItems], o[kItems];
-      T* dst[kItems];
-      const float2* w[kItems];  // null: copied
-      const bool turns = j < turning;
+  for (int base = 0; base < total; base += kThreads * ITEMS) {
+    V a[ITEMS], o[ITEMS];
+    T* dst[ITEMS];
+    int w[ITEMS];  // first angle; -1: copied
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int it = base + u * kThreads + threadIdx.x;
+      dst[u] = nullptr;
+      if (it >= total) continue;
+      const int row = p.per_head.div(it), j = it - row * p.per_head.d;
+      const int tok = p.heads.div(row), h = row - tok * p.heads.d;
+      const bool turns = j < turning, is_k = h >= p.q.heads;
       const int e = turns ? j * VEC : 2 * half + (j - turning) * VEC;
-      int t = tok, hh = h;
-#pragma unroll
-      for (int u = 0; u < kItems; ++u) {
-        dst[u] = nullptr;
-        if (t < ntok && j < p.per_head) {
-          const bool is_k = hh >= p.q.heads;
-          const RotaryPart& part = is_k ? p.k : p.q;
-          const int hp = is_k ? hh - p.q.heads : hh;
-          const T* src = static_cast<const T*>(part.in) + b * part.sb + (s0 + t) * part.ss + hp * part.sh + e;
-          dst[u] = static_cast<T*>(part.out) + (((long long)b * p.S + s0 + t) * part.heads + hp) * p.D + e;
-          w[u] = turns ? cs + t * half + j : nullptr;
-          a[u] = *reinterpret_cast<const V*>(src);
-          if (!INTER && turns) o[u] = *reinterpret_cast<const V*>(src + half);
-        }
-        t += step_tok;
-        hh += step_h;
-        if (hh >= heads) {
-          hh -= heads;
-          ++t;
-        }
+      const T* src;
+      if (is_k) {
+        const int hp = h - p.q.heads;
+        src = in_k + ((Off)tok * (Off)p.k.ss + (Off)hp * (Off)p.k.sh + e);
+        dst[u] = out_k + ((Off)(tok * p.k.heads + hp) * p.D + e);
+      } else {
+        src = in_q + ((Off)tok * (Off)p.q.ss + (Off)h * (Off)p.q.sh + e);
+        dst[u] = out_q + ((Off)(tok * p.q.heads + h) * p.D + e);
       }
-      if (!filled) {
-        filled = true;
-        fill();
+      w[u] = turns ? tok * half + j : -1;
+      a[u] = *reinterpret_cast<const V*>(src);
+      if (!INTER && turns) o[u] = *reinterpret_cast<const V*>(src + half);
+    }
+    if (base == 0) {
+      for (int i = threadIdx.x; i < ntok * half; i += kThreads) {
+        const int at = i / half, f = i - at * half;
+        const long long s = s0 + at, where = b * p.pos_sb + s;
+        const long long pos = p.positions == nullptr ? p.first + s
+                              : p.pos64 ? static_cast<const long long*>(p.positions)[where]
+                                        : static_cast<const int*>(p.positions)[where];
+        float2 c = rotary_cos_sin((double)pos, p.inv_freq[f], p.magnitude);
+        c.y *= p.sign;
+        cs[at * half + f % PAIRS * turning + f / PAIRS] = c;
       }
-#pragma unroll
-      for (int u = 0; u < kItems; ++u) {
-        if (dst[u] == nullptr) continue;
-        if (w[u] != nullptr) {
-#pragma unroll
-          for (int i = 0; i < PAIRS; ++i) {
-            const float2 c = w[u][i * turning];
-            uint16_t& lo = INTER ? a[u].v[2 * i] : a[u].v[i];
-            uint16_t& hi = INTER ? a[u].v[2 * i + (VEC > 1)] : o[u].v[i];
-            const float x = Elem<T>::value(lo), y = Elem<T>::value(hi);
-            lo = Elem<T>::bits(x * c.x - y * c.y);
-            hi = Elem<T>::bits(y * c.x + x * c.y);
-          }
-          if (!INTER) *reinterpret_cast<V*>(dst[u] + half) = o[u];
-        }
-        *reinterpret_cast<V*>(dst[u]) = a[u];
-      }
+      __syncthreads();
     }
 #pragma unroll
-    for (int u = 0; u < kItems; ++u) {
-      tok += step_tok;
-      h += step_h;
-      if (h >= heads) {
-        h -= heads;
-        ++tok;
+    for (int u = 0; u < ITEMS; ++u) {
+      if (dst[u] == nullptr) continue;
+      if (w[u] >= 0) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const float2 c = cs[w[u] + i * turning];
+          uint16_t& lo = INTER ? a[u].v[2 * i] : a[u].v[i];
+          uint16_t& hi = INTER ? a[u].v[2 * i + (VEC > 1)] : o[u].v[i];
+          const float x = Elem<T>::value(lo), y = Elem<T>::value(hi);
+          lo = Elem<T>::bits(x * c.x - y * c.y);
+          hi = Elem<T>::bits(y * c.x + x * c.y);
+        }
+        if (!INTER) *reinterpret_cast<V*>(dst[u] + half) = o[u];
       }
+      *reinterpret_cast<V*>(dst[u]) = a[u];
     }
   }
 }
 
 template <typename T, int VEC>
-int launch(const RotaryParams& p, bool interleaved, unsigned grid, size_t smem, cudaStream_t st) {
-  const cudaError_t e =
-      interleaved
-          ? launch_pdl(fa_rotary_kernel<T, (VEC > 1 ? VEC : 2), true>, dim3(grid), dim3(kThreads),
-                       smem, st, p)
-          : launch_pdl(fa_rotary_kernel<T, VEC, false>, dim3(grid), dim3(kThreads), smem, st, p);
-  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+int launch(const RotaryParams& p, bool interleaved, bool small, unsigned grid, size_t smem,
+           cudaStream_t st) {
+  constexpr int IV = VEC > 1 ? VEC : 2;
+  auto kernel = interleaved ? (small ? fa_rotary_kernel<T, IV, true, true>
+                                     : fa_rotary_kernel<T, IV, true, false>)
+                            : (small ? fa_rotary_kernel<T, VEC, false, true>
+                                     : fa_rotary_kernel<T, VEC, false, false>);
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p) == cudaSuccess ? FA_OK
+                                                                                    : FA_ERR_LAUNCH;
 }
 
 template <typename T>
-int launch_vec(const RotaryParams& p, int vec, bool interleaved, unsigned grid, size_t smem,
-               cudaStream_t st) {
+int launch_vec(const RotaryParams& p, int vec, bool interleaved, bool small, unsigned grid,
+               size_t smem, cudaStream_t st) {
   switch (vec) {
-    case 8: return launch<T, 8>(p, interleaved, grid, smem, st);
-    case 4: return launch<T, 4>(p, interleaved, grid, smem, st);
-    case 2: return launch<T, 2>(p, interleaved, grid, smem, st);
-    default: return launch<T, 1>(p, interleaved, grid, smem, st);
+    case 8: return launch<T, 8>(p, interleaved, small, grid, smem, st);
+    case 4: return launch<T, 4>(p, interleaved, small, grid, smem, st);
+    case 2: return launch<T, 2>(p, interleaved, small, grid, smem, st);
+    default: return launch<T, 1>(p, interleaved, small, grid, smem, st);
   }
 }
 
@@ -168,6 +158,14 @@ int part_vec(const fa_sm100_heads& x) {
                                (unsigned long long)x.stride_batch |
                                (unsigned long long)x.stride_seq | (unsigned long long)x.stride_head;
   return (m & 1) ? 1 : (m & 2) ? 2 : (m & 4) ? 4 : 8;
+}
+
+// Every element of a CTA's tokens is within 2^31 of the first one.
+bool small_offsets(const fa_sm100_heads& x, long long tokens, int D) {
+  const double reach = (double)tokens * (x.stride_seq < 0 ? -x.stride_seq : x.stride_seq) +
+                       (double)x.heads * (x.stride_head < 0 ? -x.stride_head : x.stride_head) +
+                       (double)tokens * x.heads * D + D;
+  return reach < 2147483647.0;
 }
 
 bool bad_part(const fa_sm100_heads& x) {
@@ -212,21 +210,25 @@ extern "C" int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k,
   const int unit = interleaved ? rotary_dim : rotary_dim / 2;
   while (vec > 1 && (unit % vec || head_dim % vec || rotary_dim % vec)) vec /= 2;
   if (interleaved && vec == 1) return FA_ERR_ARG;  // a pair has to be 4-byte aligned
-  p.per_head = (interleaved ? head_dim : head_dim - p.half) / vec;
-  p.width = p.per_head < kThreads ? p.per_head : kThreads;
-  const long long per_token = (long long)(p.q.heads + p.k.heads) * p.per_head;
-  // whole tokens until each thread has two rounds of kItems vectors
-  long long per_cta = 2LL * kThreads * kItems / per_token;
+  const int per_head = (interleaved ? head_dim : head_dim - p.half) / vec;
+  const int heads = q->heads + (k ? k->heads : 0);
+  // whole tokens until the threads have their vectors: one round, so that CTAs
+  // in different phases overlap (two rounds: 95 against 87 us at 40009 tokens of
+  // 32 heads of 64)
+  long long per_cta = (long long)kThreads * items_of(interleaved != 0) / ((long long)heads * per_head);
   if (per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
   if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
   p.per_cta = (int)per_cta;
-  p.per_seq = (int)((seqlen + per_cta - 1) / per_cta);
-  const long long grid = (long long)p.per_seq * batch;
+  p.per_head = FastDiv(per_head);
+  p.heads = FastDiv(heads);
+  p.per_seq = FastDiv((unsigned)((seqlen + per_cta - 1) / per_cta));
+  const long long grid = (long long)p.per_seq.d * batch;
   if (grid > 2147483647LL) return FA_ERR_ARG;
+  const bool small = small_offsets(*q, per_cta, head_dim) && (!k || small_offsets(*k, per_cta, head_dim));
   const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FA_DTYPE_BF16
-             ? launch_vec<__nv_bfloat16>(p, vec, interleaved != 0, (unsigned)grid, smem, st)
-             : launch_vec<__half>(p, vec, interleaved != 0, (unsigned)grid, smem, st);
+             ? launch_vec<__nv_bfloat16>(p, vec, interleaved != 0, small, (unsigned)grid, smem, st)
+             : launch_vec<__half>(p, vec, interleaved != 0, small, (unsigned)grid, smem, st);
 }

@@ -6,7 +6,7 @@
 //   torch.ops.fav.status(device) -> the device's int32 status word
 //   torch.ops.fav.merge_(acc_o, acc_lse, o, lse, first)  (ring: in-place LSE merge)
 //   torch.ops.fav.rotary, rotary_qk                      (rotary positions, with gradients)
-//   torch.ops.fav.kv_append, kv_read, decode             (paged key/value cache)
+//   torch.ops.fav.kv_append, kv_read, decode, decode_lse (paged key/value cache)
 //
 // These are the only callers of the C core on the Python side
 // (flash_attn_volta_b200/forward.py, backward.py, autograd.py): the
@@ -250,7 +250,6 @@ void rotary_launch(const at::Tensor& q_in, const at::Tensor* k_in, at::Tensor& q
   if (B * S == 0) return;
   const bool no_q = q.size(2) == 0, no_k = !k_in || k.size(2) == 0;
   if (no_q && no_k) return;
-  c10::cuda::CUDAGuard guard(q.device());
   fa_sm100_heads hq, hk;
   if (!no_q) hq = heads_of(q, &q_out);
   if (!no_k) hk = heads_of(k, k_out);
@@ -498,11 +497,11 @@ std::tuple<at::Tensor, at::Tensor> kv_read_cuda(const at::Tensor& k_pages, const
   return {k, v};
 }
 
-std::tuple<at::Tensor, at::Tensor> decode_cuda(const at::Tensor& q_in, const at::Tensor& k_pages,
-                                               const OptTensor& v_pages, const at::Tensor& table_in,
-                                               const at::Tensor& lengths_in,
-                                               const OptTensor& starts_in, bool causal,
-                                               double sm_scale, bool need_lse) {
+// out, and lse if it is not null.
+at::Tensor decode_launch(const at::Tensor& q_in, const at::Tensor& k_pages,
+                         const OptTensor& v_pages, const at::Tensor& table_in,
+                         const at::Tensor& lengths_in, const OptTensor& starts_in, bool causal,
+                         double sm_scale, at::Tensor* lse) {
   const at::Tensor q = kernel_input(q_in, "q");
   const fa_sm100_kv_cache cache = cache_of(k_pages, v_pages, dtype_code(q));
   const int64_t B = q.size(0), S = q.size(1), H = q.size(2);
@@ -515,20 +514,36 @@ std::tuple<at::Tensor, at::Tensor> decode_cuda(const at::Tensor& q_in, const at:
   if (starts_in) starts = int_input(*starts_in, 1, B, k_pages, "starts");
   c10::cuda::CUDAGuard guard(q.device());
   at::Tensor out = at::empty(q.sizes(), q.options());
-  at::Tensor lse = at::empty(need_lse ? std::vector<int64_t>{B, H, S} : std::vector<int64_t>{0},
-                             q.options().dtype(at::kFloat));
-  if (B * S == 0) return {out, lse};
+  if (lse) *lse = at::empty({B, H, S}, q.options().dtype(at::kFloat));
+  if (B * S == 0) return out;
   const size_t nbytes = fa_sm100_decode_workspace_bytes(&cache, (int)table.size(1), (int)B, (int)S, (int)H);
   TORCH_CHECK(nbytes > 0, "fa_sm100_decode: unsupported shape");
-  at::Tensor ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
+  // 256 bytes mean that the shape needs none
+  at::Tensor ws;
+  if (nbytes > 256) ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
   at::Tensor st = status_word(q.get_device());
   const int rc = fa_sm100_decode(
-      &cache, q.data_ptr(), out.data_ptr(), need_lse ? lse.data_ptr<float>() : nullptr,
+      &cache, q.data_ptr(), out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
       table.data_ptr<int>(), (int)table.size(1), lengths.data_ptr<int>(),
-      starts.defined() ? starts.data_ptr<int>() : nullptr, ws.data_ptr(), nbytes, (int)B, (int)S,
+      starts.defined() ? starts.data_ptr<int>() : nullptr,
+      ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? nbytes : 0, (int)B, (int)S,
       (int)H, (float)sm_scale, causal ? 1 : 0, st.data_ptr<int>(),
       at::cuda::getCurrentCUDAStream().stream());
   check_rc(rc, "fa_sm100_decode");
+  return out;
+}
+
+at::Tensor decode_cuda(const at::Tensor& q, const at::Tensor& k_pages, const OptTensor& v_pages,
+                       const at::Tensor& table, const at::Tensor& lengths, const OptTensor& starts,
+                       bool causal, double sm_scale) {
+  return decode_launch(q, k_pages, v_pages, table, lengths, starts, causal, sm_scale, nullptr);
+}
+std::tuple<at::Tensor, at::Tensor> decode_lse_cuda(const at::Tensor& q, const at::Tensor& k_pages,
+                                                   const OptTensor& v_pages, const at::Tensor& table,
+                                                   const at::Tensor& lengths, const OptTensor& starts,
+                                                   bool causal, double sm_scale) {
+  at::Tensor lse;
+  at::Tensor out = decode_launch(q, k_pages, v_pages, table, lengths, starts, causal, sm_scale, &lse);
   return {out, lse};
 }
 
@@ -556,7 +571,10 @@ TORCH_LIBRARY(fav, m) {
       "Tensor lengths, int max_len) -> (Tensor, Tensor)");
   m.def(
       "decode(Tensor q, Tensor k_pages, Tensor? v_pages, Tensor page_table, Tensor lengths, "
-      "Tensor? starts, bool causal, float sm_scale, bool need_lse) -> (Tensor, Tensor)");
+      "Tensor? starts, bool causal, float sm_scale) -> Tensor");
+  m.def(
+      "decode_lse(Tensor q, Tensor k_pages, Tensor? v_pages, Tensor page_table, Tensor lengths, "
+      "Tensor? starts, bool causal, float sm_scale) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(fav, CUDA, m) {
@@ -568,6 +586,7 @@ TORCH_LIBRARY_IMPL(fav, CUDA, m) {
   m.impl("kv_append", &kv_append_cuda);
   m.impl("kv_read", &kv_read_cuda);
   m.impl("decode", &decode_cuda);
+  m.impl("decode_lse", &decode_lse_cuda);
 }
 
 TORCH_LIBRARY_IMPL(fav, Autograd, m) {

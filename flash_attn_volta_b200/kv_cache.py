@@ -37,30 +37,32 @@ class PagedKVCache:
     """Pages of one attention layer, 16-bit (``k_pages``, ``v_pages``) or 4-bit
     (``PagedKVCache.of_blocks``); ``PagedKVCache.allocate`` makes them."""
     __slots__ = ("k_pages", "v_pages", "num_pages", "page_size", "n_heads", "head_dim", "dtype",
-                 "bits")
+                 "bits", "device")
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor):
-        assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, \
+        shape, dtype = k_pages.shape, k_pages.dtype
+        assert len(shape) == 4 and v_pages.shape == shape, \
             "k_pages and v_pages must be (pages, kv heads, page_size, head_dim)"
-        assert k_pages.dtype in (torch.float16, torch.bfloat16) and k_pages.dtype == v_pages.dtype, \
+        assert dtype in (torch.float16, torch.bfloat16) and v_pages.dtype == dtype, \
             "fp16 (or bf16) pages only"
         assert k_pages.device == v_pages.device, "k_pages and v_pages must be on one device"
-        assert k_pages.shape[3] in (16, 32, 64, 128), \
-            f"unsupported head_dim {k_pages.shape[3]} (allowed: 16,32,64,128)"
-        self._set(k_pages, v_pages, k_pages.shape[2], k_pages.shape[3], k_pages.dtype, 16)
+        assert shape[3] in (16, 32, 64, 128), \
+            f"unsupported head_dim {shape[3]} (allowed: 16,32,64,128)"
         assert v_pages.is_contiguous(), "pages must be contiguous"
+        self._set(k_pages, v_pages, shape, shape[2], shape[3], dtype, 16)
 
-    def _set(self, k_pages, v_pages, page_size, head_dim, dtype, bits):
+    def _set(self, k_pages, v_pages, shape, page_size, head_dim, dtype, bits):
         assert k_pages.is_contiguous(), "pages must be contiguous"
         assert 16 <= page_size <= 1024 and page_size & (page_size - 1) == 0, \
             f"page_size {page_size} is not a power of two from 16 to 1024"
-        self.k_pages, self.v_pages = k_pages, v_pages
-        self.num_pages, self.n_heads = k_pages.shape[0], k_pages.shape[1]
-        assert self.num_pages > 0 and self.n_heads > 0, "a cache needs pages and heads"
-        assert self.num_pages * self.n_heads * page_size < 2 ** 31, \
+        num_pages, n_heads = shape[0], shape[1]
+        assert num_pages > 0 and n_heads > 0, "a cache needs pages and heads"
+        assert num_pages * n_heads * page_size < 2 ** 31, \
             "pages * heads * page_size must be below 2^31"
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.num_pages, self.n_heads = num_pages, n_heads
         self.page_size, self.head_dim = page_size, head_dim
-        self.dtype, self.bits = dtype, bits
+        self.dtype, self.bits, self.device = dtype, bits, k_pages.device
 
     @classmethod
     def of_blocks(cls, blocks: torch.Tensor, head_dim: int,
@@ -69,11 +71,11 @@ class PagedKVCache:
         ``dtype`` is that of the keys, values and queries in the calls."""
         assert head_dim in (32, 64, 128), f"unsupported head_dim {head_dim} at 4 bits (32,64,128)"
         assert dtype in (torch.float16, torch.bfloat16), "fp16 (or bf16) only"
-        assert blocks.dtype == torch.uint8 and blocks.dim() == 4 \
-            and blocks.shape[3] == 20 * head_dim, \
+        shape = blocks.shape
+        assert blocks.dtype == torch.uint8 and len(shape) == 4 and shape[3] == 20 * head_dim, \
             "blocks must be uint8 (pages, kv heads, page_size / 16, 20 * head_dim)"
         c = cls.__new__(cls)
-        c._set(blocks, None, blocks.shape[2] * BLOCK_TOKENS, head_dim, dtype, 4)
+        c._set(blocks, None, shape, shape[2] * BLOCK_TOKENS, head_dim, dtype, 4)
         return c
 
     @classmethod
@@ -92,22 +94,19 @@ class PagedKVCache:
                    torch.empty(shape, dtype=dtype, device=device))
 
 
-def _check_ints(cache, batch, page_table, **vectors):
-    dev = cache.k_pages.device
-    assert cache.k_pages.is_cuda, "the cache must be on CUDA"
-    assert page_table.dtype == torch.int32 and page_table.dim() == 2 \
-        and page_table.shape[0] == batch and page_table.shape[1] > 0 \
-        and page_table.device == dev, "page_table must be (batch, pages) int32 on the cache's device"
-    for name, t in vectors.items():
-        assert t is None or (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == batch
-                             and t.device == dev), \
-            f"{name} must be (batch,) int32 on the cache's device"
+def _check_table(page_table, batch, dev):
+    shape = page_table.shape
+    assert len(shape) == 2 and shape[0] == batch and shape[1] > 0 \
+        and page_table.dtype == torch.int32 and page_table.device == dev, \
+        "page_table must be (batch, pages) int32 on the cache's device"
 
 
-def _no_grad(*tensors):
-    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                                for t in tensors)), \
-        "the cache operators are for inference: call them under torch.no_grad()"
+def _check_vector(t, batch, dev, name):
+    assert t.shape == (batch,) and t.dtype == torch.int32 and t.device == dev, \
+        f"{name} must be (batch,) int32 on the cache's device"
+
+
+_INFERENCE = "the cache operators are for inference: call them under torch.no_grad()"
 
 
 def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
@@ -125,27 +124,36 @@ def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
             without ``rotary``), contiguous, padding rows included.
     No two tokens of one call may go to the same place of the cache.
     """
-    assert k.dim() == 4 and k.shape == v.shape, f"kv shape mismatch {k.shape} {v.shape}"
-    B, S, Hkv, D = k.shape
+    shape = k.shape
+    assert len(shape) == 4 and v.shape == shape, f"kv shape mismatch {shape} {v.shape}"
+    B, S, Hkv, D = shape
     assert Hkv == cache.n_heads and D == cache.head_dim, \
-        f"k {tuple(k.shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
-    dev = cache.k_pages.device
-    assert k.dtype == v.dtype == cache.dtype, f"k and v must have the cache's dtype {cache.dtype}"
-    assert k.device == v.device == dev, "k and v must be on the cache's device"
-    _check_ints(cache, B, page_table, starts=starts, counts=counts)
+        f"k {tuple(shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
+    dev, dtype = cache.device, cache.dtype
+    assert dev.type == "cuda", "the cache must be on CUDA"
+    assert k.dtype == dtype and v.dtype == dtype, f"k and v must have the cache's dtype {dtype}"
+    assert k.device == dev and v.device == dev, "k and v must be on the cache's device"
+    _check_table(page_table, B, dev)
+    _check_vector(starts, B, dev, "starts")
+    if counts is not None:
+        _check_vector(counts, B, dev, "counts")
+    grad = k.requires_grad or v.requires_grad
     if q is not None:
-        assert q.dim() == 4 and q.shape[:2] == (B, S) and q.shape[3] == D and q.dtype == k.dtype \
-            and q.device == dev, f"q {tuple(q.shape)} does not fit k {tuple(k.shape)}"
-    if rotary is not None:
-        assert rotary.dim <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
-        assert rotary.inv_freq.device == dev, "inv_freq must be on the cache's device"
-    _no_grad(k, v, q)
+        qs = q.shape
+        assert len(qs) == 4 and qs[0] == B and qs[1] == S and qs[3] == D and q.dtype == dtype \
+            and q.device == dev, f"q {tuple(qs)} does not fit k {tuple(shape)}"
+        grad = grad or q.requires_grad
+    assert not (grad and torch.is_grad_enabled()), _INFERENCE
+    if rotary is None:
+        freq, interleaved, magnitude = None, False, 1.0
+    else:
+        freq, interleaved, magnitude = rotary.inv_freq, rotary.interleaved, rotary.magnitude
+        assert 2 * freq.shape[0] <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
+        assert freq.device == dev, "inv_freq must be on the cache's device"
     ops.load()
     ops.note_device(dev.index)
-    out = torch.ops.fav.kv_append(
-        cache.k_pages, cache.v_pages, k, v, q, page_table, starts, counts,
-        None if rotary is None else rotary.inv_freq,
-        rotary is not None and rotary.interleaved, 1.0 if rotary is None else rotary.magnitude)
+    out = torch.ops.fav.kv_append(cache.k_pages, cache.v_pages, k, v, q, page_table, starts, counts,
+                                  freq, interleaved, magnitude)
     if _lib.debug_sync():
         _lib.check_status(dev)
     return out if q is not None else None
@@ -159,8 +167,10 @@ def kv_cache_read(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.
     if max_len is None:
         max_len = page_table.shape[-1] * cache.page_size
     assert max_len >= 0, "max_len must not be negative"
-    _check_ints(cache, lengths.shape[0], page_table, lengths=lengths)
-    dev = cache.k_pages.device
+    dev, B = cache.device, lengths.shape[0]
+    assert dev.type == "cuda", "the cache must be on CUDA"
+    _check_table(page_table, B, dev)
+    _check_vector(lengths, B, dev, "lengths")
     ops.load()
     ops.note_device(dev.index)
     k, v = torch.ops.fav.kv_read(cache.k_pages, cache.v_pages, cache.dtype, page_table, lengths,
@@ -190,19 +200,23 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
         out (B, S, H, D), with return_softmax_lse also lse (B, H, S) fp32.  A row
         that sees no token gets out 0 and lse +inf.
     """
-    assert q.dim() == 4 and q.shape[3] == cache.head_dim and q.shape[2] > 0 \
-        and q.shape[2] % cache.n_heads == 0, \
-        f"q {tuple(q.shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
-    dev = cache.k_pages.device
+    shape, H = q.shape, cache.n_heads
+    assert len(shape) == 4 and shape[3] == cache.head_dim and shape[2] > 0 and shape[2] % H == 0, \
+        f"q {tuple(shape)} does not fit a cache of {H} heads of {cache.head_dim}"
+    dev, B = cache.device, shape[0]
+    assert dev.type == "cuda", "the cache must be on CUDA"
     assert q.dtype == cache.dtype and q.device == dev, "q must have the cache's dtype and device"
-    _check_ints(cache, q.shape[0], page_table, lengths=lengths, starts=starts)
-    _no_grad(q)
+    _check_table(page_table, B, dev)
+    _check_vector(lengths, B, dev, "lengths")
+    if starts is not None:
+        _check_vector(starts, B, dev, "starts")
+    assert not (q.requires_grad and torch.is_grad_enabled()), _INFERENCE
     if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(q.shape[3])
+        sm_scale = 1.0 / math.sqrt(shape[3])
     ops.load()
     ops.note_device(dev.index)
-    out, lse = torch.ops.fav.decode(q, cache.k_pages, cache.v_pages, page_table, lengths, starts,
-                                    bool(causal), float(sm_scale), bool(return_softmax_lse))
+    fn = torch.ops.fav.decode_lse if return_softmax_lse else torch.ops.fav.decode
+    out = fn(q, cache.k_pages, cache.v_pages, page_table, lengths, starts, causal, sm_scale)
     if _lib.debug_sync():
         _lib.check_status(dev)
-    return (out, lse) if return_softmax_lse else out
+    return out

@@ -135,15 +135,18 @@ def _register_python_parts() -> None:
         return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
     @torch.library.register_fake("fav::decode")
-    def _decode_fake(q, k_pages, v_pages, page_table, lengths, starts, causal, sm_scale,
-                     need_lse):
+    def _decode_fake(q, k_pages, v_pages, page_table, lengths, starts, causal, sm_scale):
         B, S, H, _ = q.shape
         _expect(q, (B, S, H, _cache_dim(k_pages, v_pages)), "q")
         if H == 0 or H % k_pages.shape[1]:
             raise RuntimeError("the query heads must be a multiple of the cache's heads")
         _check_ints(B, page_table, lengths=lengths, starts=starts)
-        lse = (B, H, S) if need_lse else (0,)
-        return q.new_empty(q.shape), q.new_empty(lse, dtype=torch.float32)
+        return q.new_empty(q.shape)
+
+    @torch.library.register_fake("fav::decode_lse")
+    def _decode_lse_fake(q, *args):
+        B, S, H, _ = q.shape
+        return _decode_fake(q, *args), q.new_empty((B, H, S), dtype=torch.float32)
 
     def _setup(ctx, inputs, output):
         q, k, v, causal, sm_scale = inputs
@@ -180,7 +183,7 @@ def note_device(index: int) -> None:
     status word), so that check_status() without a device looks there.  Not
     recorded inside torch.compile tracing (a side effect dynamo refuses); the
     word still exists and check_status(device) finds it."""
-    if not torch.compiler.is_compiling():
+    if index not in _status_devices and not torch.compiler.is_compiling():
         _status_devices.add(index)
 
 

@@ -80,16 +80,17 @@ class Rotary:
 
 
 def _check(x: torch.Tensor, rotary: Rotary, positions) -> None:
-    assert x.is_cuda, "tensors must be on CUDA"
+    shape, dev = x.shape, x.device
+    assert dev.type == "cuda", "tensors must be on CUDA"
     assert x.dtype in (torch.float16, torch.bfloat16), "fp16 (or bf16) only"
-    assert x.dim() == 4, "expected (batch, seqlen, heads, head_dim)"
-    assert x.shape[3] % 2 == 0 and rotary.dim <= x.shape[3], \
-        f"rotary dim {rotary.dim} does not fit head_dim {x.shape[3]}"
-    assert rotary.inv_freq.device == x.device, "inv_freq must be on the tensors' device"
+    assert len(shape) == 4, "expected (batch, seqlen, heads, head_dim)"
+    assert shape[3] % 2 == 0 and 2 * rotary.inv_freq.shape[0] <= shape[3], \
+        f"rotary dim {rotary.dim} does not fit head_dim {shape[3]}"
+    assert rotary.inv_freq.device == dev, "inv_freq must be on the tensors' device"
     if positions is not None:
-        assert positions.device == x.device, "positions must be on the tensors' device"
+        assert positions.device == dev, "positions must be on the tensors' device"
         assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
-        assert positions.shape == x.shape[:2] or positions.shape == x.shape[1:2], \
+        assert positions.shape in (shape[:2], shape[1:2]), \
             f"positions must be (seqlen,) or (batch, seqlen), got {tuple(positions.shape)}"
 
 
@@ -112,8 +113,9 @@ def rotary_embed_qk(q: torch.Tensor, k: torch.Tensor, rotary: Rotary,
     """rotary_embed of q (B, S, H, D) and k (B, S, H_kv, D) at the same
     positions, in one launch (and one for both gradients)."""
     _check(q, rotary, positions)
-    assert k.dim() == 4 and q.shape[:2] == k.shape[:2] and q.shape[3] == k.shape[3], \
-        f"qk shape mismatch {q.shape} {k.shape}"
+    qs, ks = q.shape, k.shape
+    assert len(ks) == 4 and qs[0] == ks[0] and qs[1] == ks[1] and qs[3] == ks[3], \
+        f"qk shape mismatch {qs} {ks}"
     assert k.dtype == q.dtype and k.device == q.device, "q and k must have one dtype and device"
     ops.load()
     return torch.ops.fav.rotary_qk(q, k, rotary.inv_freq, positions, first, rotary.interleaved,

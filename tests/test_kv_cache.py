@@ -178,15 +178,15 @@ def test_fake_shapes():
     ops.load()
     m = lambda *s, t=F16: torch.empty(s, dtype=t, device="meta")  # noqa: E731
     q, kp, table, n = m(2, 3, 4, 64), m(9, 2, 32, 64), m(2, 5, t=torch.int32), m(2, t=torch.int32)
-    out, lse = torch.ops.fav.decode(q, kp, kp, table, n, None, True, 0.1, True)
+    out, lse = torch.ops.fav.decode_lse(q, kp, kp, table, n, None, True, 0.1)
     assert out.shape == q.shape and lse.shape == (2, 4, 3)
     blocks = m(9, 2, 2, 20 * 64, t=torch.uint8)
     k, v = torch.ops.fav.kv_read(blocks, None, BF16, table, n, 77)
     assert k.shape == v.shape == (2, 77, 2, 64) and k.dtype == BF16
     new = m(2, 3, 2, 64)
     assert torch.ops.fav.kv_append(kp, kp, new, new, q, table, n, None, None, False, 1.0).shape == q.shape
-    for bad in (lambda: torch.ops.fav.decode(m(2, 3, 3, 64), kp, kp, table, n, None, True, 0.1, False),
-                lambda: torch.ops.fav.decode(q, m(9, 2, 32, 32), m(9, 2, 32, 32), table, n, None, True, 0.1, False),
+    for bad in (lambda: torch.ops.fav.decode(m(2, 3, 3, 64), kp, kp, table, n, None, True, 0.1),
+                lambda: torch.ops.fav.decode(q, m(9, 2, 32, 32), m(9, 2, 32, 32), table, n, None, True, 0.1),
                 lambda: torch.ops.fav.kv_append(kp, kp, m(2, 3, 1, 64), new, None, table, n, None, None, False, 1.0),
                 lambda: torch.ops.fav.kv_read(kp, m(9, 2, 16, 64), F16, table, n, 4)):
         with pytest.raises(RuntimeError):
@@ -630,8 +630,9 @@ def test_opcheck():
     q = torch.zeros((2, 1, 4, 64), dtype=F16, device=DEV)
     new = torch.zeros((2, 1, 2, 64), dtype=F16, device=DEV)
     tests = ("test_schema", "test_faketensor")
-    torch.library.opcheck(torch.ops.fav.decode, (q, c.k_pages, c.v_pages, pool.table_dev, pool.lengths,
-                                                 None, True, 0.1, True), test_utils=tests)
+    for op in (torch.ops.fav.decode, torch.ops.fav.decode_lse):
+        torch.library.opcheck(op, (q, c.k_pages, c.v_pages, pool.table_dev, pool.lengths, None, True,
+                                   0.1), test_utils=tests)
     torch.library.opcheck(torch.ops.fav.kv_read, (c.k_pages, c.v_pages, F16, pool.table_dev, pool.lengths,
                                                   20), test_utils=tests)
     torch.library.opcheck(torch.ops.fav.kv_append, (c.k_pages, c.v_pages, new, new, q, pool.table_dev,

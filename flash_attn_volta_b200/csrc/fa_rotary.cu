@@ -26,7 +26,14 @@ namespace {
 constexpr int kThreads = 256;
 // Vectors (half: pairs of vectors) in flight per thread: 64 bytes of loads.
 __host__ __device__ constexpr int items_of(bool interleaved) { return interleaved ? 4 : 2; }
+constexpr int kStreamRounds = 2;   // rounds of the plain kernel from which the streaming one takes over
 constexpr int kMaxAngles = 4096;   // cosines and sines of a CTA: 32 KB
+
+// The streaming kernel's ring: stages, and bytes of a CTA.
+__host__ __device__ constexpr int stages_of(bool interleaved) { return interleaved ? 6 : 4; }
+constexpr size_t ring_bytes(bool interleaved, int vec) {
+  return (size_t)stages_of(interleaved) * (interleaved ? 1 : 2) * kThreads * 2 * vec;
+}
 
 struct RotaryPart {
   const void* in;
@@ -128,6 +135,98 @@ __global__ void __launch_bounds__(kThreads, 4) fa_rotary_kernel(const RotaryPara
   }
 }
 
+// The same for many tokens: a CTA takes so many that the grid is one wave, and
+// each thread streams its vectors through a ring of its own in shared memory
+// (no other thread reads them, so the waits are the thread's own): the loads in
+// flight then need no registers and do not stop while a round is computed.  A
+// thread keeps its column (its dims of a head) and steps down the rows (heads of
+// tokens).
+template <typename T, int VEC, bool INTER>
+__global__ void __launch_bounds__(kThreads, 4) fa_rotary_stream_kernel(const RotaryParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  griddep_wait();
+  griddep_launch_dependents();
+  using V = Pack16<VEC>;
+  constexpr int PAIRS = INTER ? VEC / 2 : VEC, LOADS = INTER ? 1 : 2, NS = stages_of(INTER);
+  V* ring = reinterpret_cast<V*>(smem) + threadIdx.x;  // (stage, load) at * kThreads
+  float2* cs = reinterpret_cast<float2*>(smem + (size_t)NS * LOADS * kThreads * sizeof(V));
+  const int half = p.half, turning = half / PAIRS;
+  const int b = p.per_seq.div(blockIdx.x), s0 = (blockIdx.x - b * p.per_seq.d) * p.per_cta;
+  const int ntok = min(p.per_cta, p.S - s0), rows = ntok * (int)p.heads.d;
+  const T* in_q = static_cast<const T*>(p.q.in) + b * p.q.sb + s0 * p.q.ss;
+  const T* in_k = static_cast<const T*>(p.k.in) + b * p.k.sb + s0 * p.k.ss;
+  T* out_q = static_cast<T*>(p.q.out) + ((long long)b * p.S + s0) * p.q.heads * p.D;
+  T* out_k = static_cast<T*>(p.k.out) + ((long long)b * p.S + s0) * p.k.heads * p.D;
+  const int first = p.per_head.div(threadIdx.x), col = threadIdx.x - first * p.per_head.d;
+  const int step = kThreads / p.per_head.d;
+  const bool turns = col < turning;
+  const int e = turns ? col * VEC : 2 * half + (col - turning) * VEC;
+  const int start = first < step ? first : rows;  // threads without a whole row idle
+
+  auto load = [&](int row, int stage) {
+    if (row < rows) {
+      const int tok = p.heads.div(row), h = row - tok * p.heads.d;
+      const T* src = h < p.q.heads
+                         ? in_q + (tok * (int)p.q.ss + h * (int)p.q.sh + e)
+                         : in_k + (tok * (int)p.k.ss + (h - p.q.heads) * (int)p.k.sh + e);
+      const uint32_t dst = smem_u32(ring + stage * LOADS * kThreads);
+      cp_async<sizeof(V)>(dst, src);
+      if (!INTER && turns) cp_async<sizeof(V)>(dst + kThreads * sizeof(V), src + half);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) load(start + i * step, i);
+  for (int i = threadIdx.x; i < ntok * half; i += kThreads) {
+    const int at = i / half, f = i - at * half;
+    const long long s = s0 + at, where = b * p.pos_sb + s;
+    const long long pos = p.positions == nullptr ? p.first + s
+                          : p.pos64 ? static_cast<const long long*>(p.positions)[where]
+                                    : static_cast<const int*>(p.positions)[where];
+    float2 c = rotary_cos_sin((double)pos, p.inv_freq[f], p.magnitude);
+    c.y *= p.sign;
+    cs[at * half + f % PAIRS * turning + f / PAIRS] = c;
+  }
+  __syncthreads();
+  int stage = 0;
+  for (int row = start; row < rows; row += step) {
+    load(row + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
+    cp_async_wait<NS - 1>();
+    V a = ring[stage * LOADS * kThreads], o;
+    const int tok = p.heads.div(row), h = row - tok * p.heads.d;
+    T* dst = h < p.q.heads ? out_q + ((tok * p.q.heads + h) * p.D + e)
+                           : out_k + ((tok * p.k.heads + h - p.q.heads) * p.D + e);
+    if (turns) {
+      if (!INTER) o = ring[(stage * LOADS + 1) * kThreads];
+      const float2* w = cs + tok * half + col;
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) {
+        const float2 c = w[i * turning];
+        uint16_t& lo = INTER ? a.v[2 * i] : a.v[i];
+        uint16_t& hi = INTER ? a.v[2 * i + 1] : o.v[i];
+        const float x = Elem<T>::value(lo), y = Elem<T>::value(hi);
+        lo = Elem<T>::bits(x * c.x - y * c.y);
+        hi = Elem<T>::bits(y * c.x + x * c.y);
+      }
+      if (!INTER) *reinterpret_cast<V*>(dst + half) = o;
+    }
+    *reinterpret_cast<V*>(dst) = a;
+    if (++stage == NS) stage = 0;
+  }
+  cp_async_wait<0>();
+}
+
+template <typename T, int VEC>
+int launch_stream(const RotaryParams& p, bool interleaved, unsigned grid, size_t angles, cudaStream_t st) {
+  if constexpr (VEC > 1) {
+    auto kernel = interleaved ? fa_rotary_stream_kernel<T, VEC, true> : fa_rotary_stream_kernel<T, VEC, false>;
+    const size_t smem = ring_bytes(interleaved, VEC) + angles;  // below 48 KB
+    return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p) == cudaSuccess ? FA_OK
+                                                                                      : FA_ERR_LAUNCH;
+  }
+  return FA_ERR_ARG;
+}
+
 template <typename T, int VEC>
 int launch(const RotaryParams& p, bool interleaved, bool small, unsigned grid, size_t smem,
            cudaStream_t st) {
@@ -141,8 +240,15 @@ int launch(const RotaryParams& p, bool interleaved, bool small, unsigned grid, s
 }
 
 template <typename T>
-int launch_vec(const RotaryParams& p, int vec, bool interleaved, bool small, unsigned grid,
-               size_t smem, cudaStream_t st) {
+int launch_vec(const RotaryParams& p, int vec, bool interleaved, bool small, bool stream,
+               unsigned grid, size_t smem, cudaStream_t st) {
+  if (stream) {
+    switch (vec) {
+      case 8: return launch_stream<T, 8>(p, interleaved, grid, smem, st);
+      case 4: return launch_stream<T, 4>(p, interleaved, grid, smem, st);
+      default: return launch_stream<T, 2>(p, interleaved, grid, smem, st);
+    }
+  }
   switch (vec) {
     case 8: return launch<T, 8>(p, interleaved, small, grid, smem, st);
     case 4: return launch<T, 4>(p, interleaved, small, grid, smem, st);
@@ -215,7 +321,19 @@ extern "C" int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k,
   // whole tokens until the threads have their vectors: one round, so that CTAs
   // in different phases overlap (two rounds: 95 against 87 us at 40009 tokens of
   // 32 heads of 64)
-  long long per_cta = (long long)kThreads * items_of(interleaved != 0) / ((long long)heads * per_head);
+  const long long per_token = (long long)heads * per_head;
+  const long long per_round = (long long)kThreads * items_of(interleaved != 0);
+  long long per_cta = per_round / per_token;
+  // many tokens: one wave of four CTAs per SM that stream, where that gives each
+  // thread enough rounds
+  const long long slots = 4LL * sm_count() / batch, per_seq = slots < 1 ? 1 : slots;
+  const long long room = (long long)(48 * 1024 - ring_bytes(interleaved != 0, vec)) / (8LL * p.half);
+  long long many = (seqlen + per_seq - 1) / per_seq;
+  if (room >= 1 && many > room) many = (many + (many + room - 1) / room - 1) / ((many + room - 1) / room);
+  const bool fits = small_offsets(*q, many, head_dim) && (!k || small_offsets(*k, many, head_dim));
+  const bool stream_rounds =
+      vec > 1 && per_head <= kThreads && many <= room && fits && many * per_token >= kStreamRounds * per_round;
+  if (stream_rounds) per_cta = many;
   if (per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
   if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
@@ -229,6 +347,8 @@ extern "C" int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k,
   const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FA_DTYPE_BF16
-             ? launch_vec<__nv_bfloat16>(p, vec, interleaved != 0, small, (unsigned)grid, smem, st)
-             : launch_vec<__half>(p, vec, interleaved != 0, small, (unsigned)grid, smem, st);
+             ? launch_vec<__nv_bfloat16>(p, vec, interleaved != 0, small, stream_rounds, (unsigned)grid,
+                                         smem, st)
+             : launch_vec<__half>(p, vec, interleaved != 0, small, stream_rounds, (unsigned)grid,
+                                         smem, st);
 }

@@ -174,6 +174,48 @@ __device__ __forceinline__ void rotate_any(const uint16_t* row, int e, int half,
   }
 }
 
+// 8 dims (chunk c) of head h of K (part 1) or V (part 2) to the cache row
+// `place` (of head 0; -1: not stored).  4 bits: all lanes of the warp take part.
+template <typename T, int BITS>
+__device__ __forceinline__ void store_item(const AppendParams& p, int part, int c, int h, int place,
+                                           float (&x)[8]) {
+  const KvView& kv = p.kv;
+  const int to = place + (h << p.page_shift);  // row of the cache
+  if constexpr (BITS == 16) {
+    if (place >= 0)
+      *reinterpret_cast<uint4*>((part == 1 ? kv.k : kv.v) + ((long long)to * kv.D + c * 8) * 2) = pack8<T>(x);
+  } else {
+    uint32_t code[8];
+    const uint32_t sm = quantise(x, code);
+    if (place < 0) return;
+    const Kv4 lay(kv.D);
+    const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = to % kBlockTokens;
+    uint8_t* blk = kv.k + (long long)(to / kBlockTokens) * lay.bytes();
+    if (part == 1) {
+      const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 |
+                         code[3] << 20 | code[5] << 24 | code[7] << 28;
+      reinterpret_cast<uint32_t*>(blk)[(r * 4 + t4) * NG + grp] = w;
+      if (t4 == 0) reinterpret_cast<uint32_t*>(blk + lay.k_params())[r * NG + grp] = sm;
+    } else {
+      const int tp = r / 8, tt = r % 8 / 2, hi = r % 2;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int g = 2 * t4 + n;
+        const uint32_t w =
+            code[4 * n] | code[4 * n + 1] << 4 | code[4 * n + 2] << 8 | code[4 * n + 3] << 12;
+        reinterpret_cast<uint16_t*>(blk + lay.v_codes())[(((tp * 8 + g) * 4 + tt) * NG + grp) * 2 + hi] =
+            (uint16_t)w;
+      }
+      if (t4 == 0) {
+        uint16_t* vp = reinterpret_cast<uint16_t*>(blk + lay.v_params());
+        const int k = (grp * 4 + tt) * 4 + tp * 2 + hi;
+        vp[k] = (uint16_t)sm;
+        vp[k + 16 * NG] = (uint16_t)(sm >> 16);
+      }
+    }
+  }
+}
+
 // New tokens into the cache.  Bound by HBM for prompts (every input is read
 // once, every output written once) and by latency for single tokens: one
 // launch does the rotation of q and k, the page lookup and both writes.
@@ -273,43 +315,107 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
         if (part == 0) *reinterpret_cast<uint4*>(q_out + (long long)i * 8) = pack8<T>(x);
       }
       if (part == 0) continue;
-      const int place = there ? places[tok] : -1;
-      const int to = place + (h << p.page_shift);  // row of the cache
-      if (BITS == 16) {
-        if (place >= 0)
-          *reinterpret_cast<uint4*>((part == 1 ? kv.k : kv.v) + ((long long)to * kv.D + e) * 2) = pack8<T>(x);
-        continue;
-      }
-      uint32_t code[8];
-      const uint32_t sm = quantise(x, code);
-      if (place < 0) continue;
-      const Kv4 lay(kv.D);
-      const int NG = lay.groups(), grp = c / 4, t4 = c % 4, r = to % kBlockTokens;
-      uint8_t* blk = kv.k + (long long)(to / kBlockTokens) * lay.bytes();
-      if (part == 1) {
-        const uint32_t w = code[0] | code[2] << 4 | code[4] << 8 | code[6] << 12 | code[1] << 16 |
-                           code[3] << 20 | code[5] << 24 | code[7] << 28;
-        reinterpret_cast<uint32_t*>(blk)[(r * 4 + t4) * NG + grp] = w;
-        if (t4 == 0) reinterpret_cast<uint32_t*>(blk + lay.k_params())[r * NG + grp] = sm;
-      } else {
-        const int tp = r / 8, tt = r % 8 / 2, hi = r % 2;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int g = 2 * t4 + n;
-          const uint32_t w =
-              code[4 * n] | code[4 * n + 1] << 4 | code[4 * n + 2] << 8 | code[4 * n + 3] << 12;
-          reinterpret_cast<uint16_t*>(blk + lay.v_codes())[(((tp * 8 + g) * 4 + tt) * NG + grp) * 2 + hi] =
-              (uint16_t)w;
-        }
-        if (t4 == 0) {
-          uint16_t* vp = reinterpret_cast<uint16_t*>(blk + lay.v_params());
-          const int k = (grp * 4 + tt) * 4 + tp * 2 + hi;
-          vp[k] = (uint16_t)sm;
-          vp[k + 16 * NG] = (uint16_t)(sm >> 16);
-        }
-      }
+      store_item<T, BITS>(p, part, c, h, there ? places[tok] : -1, x);
     }
   }
+}
+
+// The same for prompts: a CTA takes so many tokens that the grid is one wave, and
+// each thread streams its vectors through a ring of its own in shared memory.
+// The rows are the heads of q, then of k, then of v of the CTA's tokens, each
+// filled up to whole warps; a thread keeps its dims of a row.
+constexpr int kStreamStages = 4;
+
+template <typename T, bool INTER, int BITS>
+__global__ void __launch_bounds__(kThreads, 4) fa_kv_append_stream_kernel(const AppendParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  griddep_wait();
+  griddep_launch_dependents();
+  constexpr int LOADS = INTER ? 1 : 2, NS = kStreamStages, N = INTER ? 4 : 8;
+  const KvView& kv = p.kv;
+  uint4* ring = reinterpret_cast<uint4*>(smem) + threadIdx.x;
+  float2* cs = reinterpret_cast<float2*>(smem + NS * LOADS * kThreads * 16);
+  int* places = reinterpret_cast<int*>(cs + p.per_cta * p.half);
+  const int b = p.per_seq.div(blockIdx.x), s0 = (blockIdx.x - b * p.per_seq.d) * p.per_cta;
+  const int ntok = min(p.per_cta, p.S - s0), hk = kv.heads;
+  const long long first = (long long)p.starts[b] + s0;
+  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, p.counts[b] - s0));
+  const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), e = c * 8;
+  const int step = kThreads >> p.chunk_shift, whole = (32 >> p.chunk_shift) - 1;  // rows of a warp - 1
+  const int nq = ntok * (int)p.q_heads.d, nk = fresh * hk;
+  const int k0 = (nq + whole) & ~whole, v0 = k0 + ((nk + whole) & ~whole), end = v0 + ((nk + whole) & ~whole);
+  const T* from_q = static_cast<const T*>(p.part[0].in) + b * p.part[0].sb + s0 * p.part[0].ss + e;
+  const T* from_k = static_cast<const T*>(p.part[1].in) + b * p.part[1].sb + s0 * p.part[1].ss + e;
+  const T* from_v = static_cast<const T*>(p.part[2].in) + b * p.part[2].sb + s0 * p.part[2].ss + e;
+  const bool turning = e < 2 * p.half, lower = e < p.half;
+  const int partner = lower ? p.half : -p.half;
+  T* q_out = static_cast<T*>(p.q_out) + ((((long long)b * p.S + s0) * p.q_heads.d) << (p.chunk_shift + 3)) + e;
+  const int start = threadIdx.x >> p.chunk_shift;
+
+  auto load = [&](int row, int stage) {
+    if (row < end) {
+      const int part = row < k0 ? 0 : row < v0 ? 1 : 2;
+      const int i = row - (part == 0 ? 0 : part == 1 ? k0 : v0);
+      if (i < (part == 0 ? nq : nk)) {
+        const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
+        const int tok = heads.div(i), h = i - tok * heads.d;
+        const T* at = (part == 0 ? from_q : part == 1 ? from_k : from_v) +
+                      (tok * (int)p.part[part].ss + h * (int)p.part[part].sh);
+        const uint32_t dst = smem_u32(ring + stage * LOADS * kThreads);
+        cp_async<16>(dst, at);
+        if (!INTER && turning && part < 2) cp_async<16>(dst + kThreads * 16, at + partner);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) load(start + i * step, i);
+  for (int i = threadIdx.x; i < fresh; i += kThreads) {
+    const long long pos = first + i;
+    const int id = kv.page_of(b, pos, p.page_shift);
+    if (id < 0) kv.report(kStatusPage);
+    places[i] = id < 0 ? -1 : ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
+  }
+  for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
+    const int tok = i / p.half, f = i - tok * p.half;
+    cs[tok * p.half + f % N * (p.half / N) + f / N] =
+        rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
+  }
+  __syncthreads();
+  const float2* angles = cs + (INTER || lower ? c : c - p.half / 8);
+  int stage = 0;
+  // the same number of rounds for all lanes of a warp: `end` is whole warps
+  for (int row = start; row < end; row += step) {
+    load(row + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
+    cp_async_wait<NS - 1>();
+    const int part = row < k0 ? 0 : row < v0 ? 1 : 2;
+    const int i = row - (part == 0 ? 0 : part == 1 ? k0 : v0);
+    const bool there = i < (part == 0 ? nq : nk);
+    const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
+    const int tok = there ? heads.div(i) : 0, h = i - tok * heads.d;
+    float x[8] = {};
+    if (there) {
+      unpack8<T>(ring[stage * LOADS * kThreads], x);
+      if (turning && part < 2) {
+        float y[8];
+        if (!INTER) unpack8<T>(ring[(stage * LOADS + 1) * kThreads], y);
+        rotate_wide<INTER>(angles + tok * p.half, p.half / N, lower ? -1.f : 1.f, x, y);
+      }
+      if (part == 0) *reinterpret_cast<uint4*>(q_out + ((long long)i << (p.chunk_shift + 3))) = pack8<T>(x);
+    }
+    if (part > 0) store_item<T, BITS>(p, part, c, h, there ? places[tok] : -1, x);
+    if (++stage == NS) stage = 0;
+  }
+  cp_async_wait<0>();
+}
+
+template <typename T, int BITS>
+int launch_append_stream(const AppendParams& p, bool interleaved, unsigned grid, size_t smem,
+                         cudaStream_t st) {
+  auto kernel = interleaved ? fa_kv_append_stream_kernel<T, true, BITS>
+                            : fa_kv_append_stream_kernel<T, false, BITS>;
+  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p) == cudaSuccess ? FA_OK
+                                                                                    : FA_ERR_LAUNCH;
 }
 
 template <typename T, int BITS, bool WIDE>
@@ -324,8 +430,11 @@ int launch_append(const AppendParams& p, bool interleaved, unsigned grid, size_t
 }
 
 template <typename T>
-int launch_append_t(const AppendParams& p, bool is_wide, bool interleaved, unsigned grid, size_t smem,
-                    cudaStream_t st) {
+int launch_append_t(const AppendParams& p, bool is_wide, bool stream, bool interleaved, unsigned grid,
+                    size_t smem, cudaStream_t st) {
+  if (stream)
+    return p.kv.bits == 16 ? launch_append_stream<T, 16>(p, interleaved, grid, smem, st)
+                           : launch_append_stream<T, 4>(p, interleaved, grid, smem, st);
   if (p.kv.bits == 16)
     return is_wide ? launch_append<T, 16, true>(p, interleaved, grid, smem, st)
                    : launch_append<T, 16, false>(p, interleaved, grid, smem, st);
@@ -567,22 +676,37 @@ extern "C" int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100
   // whole tokens until every thread has two items: one round
   const long long per_token = (long long)((q ? q->heads : 0) + 2 * k->heads) * (cache->head_dim / 8);
   long long per_cta = 2 * kThreads / per_token;
+  // prompts: one wave of four CTAs per SM that stream, where that gives each thread
+  // enough rounds
+  const size_t ring = (size_t)kStreamStages * (interleaved ? 1 : 2) * kThreads * 16;
+  const size_t each = p.half * sizeof(float2) + sizeof(int);  // of a token
+  const long long slots = 4LL * sm_count() / batch, per_seq = slots < 1 ? 1 : slots;
+  const long long room = (long long)((48 * 1024 - ring) / each);
+  long long many = (seqlen + per_seq - 1) / per_seq;
+  if (many > room) many = (many + (many + room - 1) / room - 1) / ((many + room - 1) / room);
+  const auto fits = [&](long long tokens) {
+    return wide(*k, tokens) && wide(*v, tokens) && (!q || wide(*q, tokens)) &&
+           (interleaved ? p.half % 4 : p.half % 8) == 0;
+  };
+  const bool streams = fits(many) && many * per_token >= 2 * 2 * kThreads;
+  if (streams) per_cta = many;
   if (p.half > 0 && per_cta > kMaxAngles / p.half) per_cta = kMaxAngles / p.half;
   if (per_cta > seqlen) per_cta = seqlen;
   if (per_cta < 1) per_cta = 1;
   p.per_cta = (int)per_cta;
-  const bool is_wide = wide(*k, per_cta) && wide(*v, per_cta) && (!q || wide(*q, per_cta)) &&
-                       (interleaved ? p.half % 4 : p.half % 8) == 0;
+  const bool is_wide = fits(per_cta);
   p.per_seq = FastDiv((unsigned)((seqlen + per_cta - 1) / per_cta));
   p.k_heads = FastDiv((unsigned)k->heads);
   if (q) p.q_heads = FastDiv((unsigned)q->heads);
   const long long grid = (long long)p.per_seq.d * batch;
   if (grid > 2147483647LL) return FA_ERR_ARG;
-  const size_t smem = (size_t)per_cta * (p.half * sizeof(float2) + sizeof(int));
+  const size_t smem = (streams ? ring : 0) + (size_t)per_cta * each;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return cache->dtype == FA_DTYPE_BF16
-             ? launch_append_t<__nv_bfloat16>(p, is_wide, interleaved != 0, (unsigned)grid, smem, st)
-             : launch_append_t<__half>(p, is_wide, interleaved != 0, (unsigned)grid, smem, st);
+             ? launch_append_t<__nv_bfloat16>(p, is_wide, streams, interleaved != 0, (unsigned)grid,
+                                              smem, st)
+             : launch_append_t<__half>(p, is_wide, streams, interleaved != 0, (unsigned)grid,
+                                              smem, st);
 }
 
 extern "C" int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_table,

@@ -299,6 +299,30 @@ def test_append_rotates_on_the_way(bits, R, inter):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits,B,S,H,Hkv,D,R,inter,dtype", [
+    (16, 1, 4001, 8, 2, 128, 128, False, BF16), (4, 1, 4001, 8, 2, 128, 128, False, BF16),
+    (16, 2, 3001, 12, 3, 64, 32, True, F16), (4, 2, 3001, 12, 3, 64, 32, True, F16),
+    (16, 3, 2003, 5, 5, 16, 16, False, F16), (4, 3, 2003, 5, 5, 32, 0, False, F16)])
+def test_long_prompts_match_short_calls(bits, B, S, H, Hkv, D, R, inter, dtype):
+    """Prompts long enough for each thread to stream several rounds: the cache and
+    q are bit for bit what appends of a few tokens leave, ragged counts."""
+    counts = [S, S - 700, 13][:B]
+    g = torch.Generator(device=DEV).manual_seed(S)
+    mk = lambda h: torch.randn((B, S, h, D), generator=g, device=DEV).to(dtype)  # noqa: E731
+    q, k, v = mk(H), mk(Hkv), mk(Hkv)
+    rot = Rotary.build(R, interleaved=inter, device=DEV) if R else None
+    long, short = (Pool([S + 9] * B, 32, Hkv, D, dtype, bits) for _ in range(2))
+    qo = kv_cache_append(long.cache, k, v, long.table_dev, _ints([9] * B), _ints(counts), q=q, rotary=rot)
+    qs = torch.cat([kv_cache_append(short.cache, k[:, a:a + 50], v[:, a:a + 50], short.table_dev,
+                                    _ints([9 + a] * B), _ints([max(0, min(50, n - a)) for n in counts]),
+                                    q=q[:, a:a + 50], rotary=rot) for a in range(0, S, 50)], 1)
+    check_status(DEV)
+    assert torch.equal(qo, qs)
+    for a, b in ((long.cache.k_pages, short.cache.k_pages), (long.cache.v_pages, short.cache.v_pages)):
+        assert a is None or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
 def test_append_strides_and_copy_of_q():
     """k, v and q as slices of one projection, at an odd offset too; without
     rotary q comes back as it is."""

@@ -134,6 +134,29 @@ def test_matches_oracle(B, S, H, D, R, inter, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B,S,H,Hkv,D,R,inter,dtype", [
+    (1, 9001, 24, 8, 64, 64, False, torch.float16), (2, 5003, 32, 1, 80, 40, True, torch.bfloat16),
+    (3, 3001, 20, 4, 128, 32, False, torch.bfloat16), (700, 21, 9, 3, 64, 64, True, torch.float16),
+    (1, 2500, 50, 7, 96, 12, True, torch.float16), (1, 4001, 33, 3, 40, 20, False, torch.float16)])
+def test_many_tokens(B, S, H, Hkv, D, R, inter, dtype):
+    """Enough tokens for each thread to stream several rounds; odd counts, and rows
+    that are no multiple of the threads."""
+    g = torch.Generator(device=DEV).manual_seed(S)
+    q = torch.randn((B, S, H, D), generator=g, device=DEV).to(dtype)
+    k = torch.randn((B, S, Hkv, D), generator=g, device=DEV).to(dtype)
+    pos = torch.randint(0, 30000, (B, 1), generator=g, device=DEV) + torch.arange(S, device=DEV)
+    qo, ko = rotary_embed_qk(q, k, Rotary(_freq(R).to(DEV), inter), pos)
+    part = slice(0, None, max(1, B // 3)), slice(0, None, 7)
+    _check(qo[part], q[part], pos[part].cpu(), _freq(R), inter)
+    _check(ko[part], k[part], pos[part].cpu(), _freq(R), inter)
+    # every other row is what a call with fewer tokens gives
+    for b in (0, B - 1):
+        at = slice(S // 2, S // 2 + 5)
+        few = rotary_embed_qk(q[b:b + 1, at], k[b:b + 1, at], Rotary(_freq(R).to(DEV), inter), pos[b:b + 1, at])
+        assert torch.equal(few[0], qo[b:b + 1, at]) and torch.equal(few[1], ko[b:b + 1, at])
+
+
+@pytest.mark.gpu
 def test_far_positions():
     """Angles of 10^6 and 2^40 rad: an fp32 product would be off by 0.1 rad and more."""
     x = torch.randn((1, 4, 2, 64), generator=torch.Generator().manual_seed(3)).half()

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "fa_kernels.h"
 #include "fa_kv_cache.cuh"
 #include "fa_rotary.cuh"
@@ -114,11 +116,11 @@ __device__ __forceinline__ uint32_t quantise(float (&x)[8], uint32_t (&code)[8])
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8], uint32_t signs = 0u) {
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = Elem<T>::unpack2(v[i]);
+    const float2 f = Elem<T>::unpack2(v[i] ^ signs);
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
   }
@@ -131,10 +133,10 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 
 // Rotates the 8 dims e.. of a row whose own values are x.  WIDE: the thread's
 // angles stand `stride` apart from `w` on (neighbouring lanes read neighbouring
-// words), the partner dims' values are y, and `sign` is -1 in the first halves.
+// words) and the partner dims' values are y, negated in the first halves.
 // Otherwise `w` holds the angles in order and partner dims are read from `row`.
 template <bool INTER>
-__device__ __forceinline__ void rotate_wide(const float2* w, int stride, float sign, float (&x)[8],
+__device__ __forceinline__ void rotate_wide(const float2* w, int stride, float (&x)[8],
                                             const float (&y)[8]) {
   if constexpr (INTER) {
 #pragma unroll
@@ -148,7 +150,7 @@ __device__ __forceinline__ void rotate_wide(const float2* w, int stride, float s
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 c = w[i * stride];
-      x[i] = x[i] * c.x + sign * y[i] * c.y;
+      x[i] = x[i] * c.x + y[i] * c.y;
     }
   }
 }
@@ -301,10 +303,9 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
           unpack8<T>(own[u], x);
           if (turns) {
             float y[8];
-            if (!INTER) unpack8<T>(other[u], y);
             const bool lower = e < p.half;
-            rotate_wide<INTER>(w + (INTER || lower ? c : c - p.half / 8), p.half / (INTER ? 4 : 8),
-                               lower ? -1.f : 1.f, x, y);
+            if (!INTER) unpack8<T>(other[u], y, lower ? 0x80008000u : 0u);
+            rotate_wide<INTER>(w + (INTER || lower ? c : c - p.half / 8), p.half / (INTER ? 4 : 8), x, y);
           }
         } else {
           const uint16_t* raw = reinterpret_cast<const uint16_t*>(at[u]);
@@ -320,10 +321,10 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
   }
 }
 
-// The same for prompts: a CTA takes so many tokens that the grid is one wave, and
+// The same for prompts: a CTA takes so many tokens that the grid is few waves, and
 // each thread streams its vectors through a ring of its own in shared memory.
-// The rows are the heads of q, then of k, then of v of the CTA's tokens, each
-// filled up to whole warps; a thread keeps its dims of a row.
+// The rows are the heads of q, then of k, then of v of the CTA's tokens; a thread
+// keeps its dims of a row.
 constexpr int kStreamStages = 4;
 
 template <typename T, bool INTER, int BITS>
@@ -343,70 +344,73 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_stream_kernel(const 
   const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), e = c * 8;
   const int step = kThreads >> p.chunk_shift, whole = (32 >> p.chunk_shift) - 1;  // rows of a warp - 1
   const int nq = ntok * (int)p.q_heads.d, nk = fresh * hk;
-  const int k0 = (nq + whole) & ~whole, v0 = k0 + ((nk + whole) & ~whole), end = v0 + ((nk + whole) & ~whole);
-  const T* from_q = static_cast<const T*>(p.part[0].in) + b * p.part[0].sb + s0 * p.part[0].ss + e;
-  const T* from_k = static_cast<const T*>(p.part[1].in) + b * p.part[1].sb + s0 * p.part[1].ss + e;
-  const T* from_v = static_cast<const T*>(p.part[2].in) + b * p.part[2].sb + s0 * p.part[2].ss + e;
   const bool turning = e < 2 * p.half, lower = e < p.half;
+  const uint32_t signs = lower ? 0x80008000u : 0u;
   const int partner = lower ? p.half : -p.half;
   T* q_out = static_cast<T*>(p.q_out) + ((((long long)b * p.S + s0) * p.q_heads.d) << (p.chunk_shift + 3)) + e;
   const int start = threadIdx.x >> p.chunk_shift;
+  const float2* angles = cs + (INTER || lower ? c : c - p.half / 8);
 
-  auto load = [&](int row, int stage) {
-    if (row < end) {
-      const int part = row < k0 ? 0 : row < v0 ? 1 : 2;
-      const int i = row - (part == 0 ? 0 : part == 1 ? k0 : v0);
-      if (i < (part == 0 ? nq : nk)) {
-        const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
-        const int tok = heads.div(i), h = i - tok * heads.d;
-        const T* at = (part == 0 ? from_q : part == 1 ? from_k : from_v) +
-                      (tok * (int)p.part[part].ss + h * (int)p.part[part].sh);
+  // The rows of one of q (0), k (1) and v (2); `ready` runs behind the first loads.
+  auto run = [&](auto part_tag, int rows, const FastDiv heads, auto&& ready) {
+    constexpr int PART = decltype(part_tag)::value;
+    const AppendPart& src = p.part[PART];
+    const T* from = static_cast<const T*>(src.in) + b * src.sb + s0 * src.ss + e;
+    const int ss = (int)src.ss, sh = (int)src.sh;
+    auto load = [&](int row, int stage) {
+      if (row < rows) {
+        const int tok = heads.div(row), h = row - tok * heads.d;
+        const T* at = from + (tok * ss + h * sh);
         const uint32_t dst = smem_u32(ring + stage * LOADS * kThreads);
         cp_async<16>(dst, at);
-        if (!INTER && turning && part < 2) cp_async<16>(dst + kThreads * 16, at + partner);
+        if (!INTER && PART < 2 && turning) cp_async<16>(dst + kThreads * 16, at + partner);
       }
-    }
-    cp_async_commit();
-  };
+      cp_async_commit();
+    };
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i) load(start + i * step, i);
-  for (int i = threadIdx.x; i < fresh; i += kThreads) {
-    const long long pos = first + i;
-    const int id = kv.page_of(b, pos, p.page_shift);
-    if (id < 0) kv.report(kStatusPage);
-    places[i] = id < 0 ? -1 : ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
-  }
-  for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
-    const int tok = i / p.half, f = i - tok * p.half;
-    cs[tok * p.half + f % N * (p.half / N) + f / N] =
-        rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
-  }
-  __syncthreads();
-  const float2* angles = cs + (INTER || lower ? c : c - p.half / 8);
-  int stage = 0;
-  // the same number of rounds for all lanes of a warp: `end` is whole warps
-  for (int row = start; row < end; row += step) {
-    load(row + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
-    cp_async_wait<NS - 1>();
-    const int part = row < k0 ? 0 : row < v0 ? 1 : 2;
-    const int i = row - (part == 0 ? 0 : part == 1 ? k0 : v0);
-    const bool there = i < (part == 0 ? nq : nk);
-    const FastDiv& heads = part == 0 ? p.q_heads : p.k_heads;
-    const int tok = there ? heads.div(i) : 0, h = i - tok * heads.d;
-    float x[8] = {};
-    if (there) {
-      unpack8<T>(ring[stage * LOADS * kThreads], x);
-      if (turning && part < 2) {
-        float y[8];
-        if (!INTER) unpack8<T>(ring[(stage * LOADS + 1) * kThreads], y);
-        rotate_wide<INTER>(angles + tok * p.half, p.half / N, lower ? -1.f : 1.f, x, y);
+    for (int i = 0; i < NS - 1; ++i) load(start + i * step, i);
+    ready();
+    int stage = 0;
+    // the same number of rounds for all lanes of a warp
+    const int end = PART == 0 ? rows : (rows + whole) & ~whole;
+    for (int row = start; row < end; row += step) {
+      load(row + (NS - 1) * step, stage == 0 ? NS - 1 : stage - 1);
+      cp_async_wait<NS - 1>();
+      const bool there = PART == 0 || row < rows;
+      const int tok = there ? heads.div(row) : 0, h = row - tok * heads.d;
+      float x[8] = {};
+      if (there) {
+        unpack8<T>(ring[stage * LOADS * kThreads], x);
+        if (PART < 2 && turning) {
+          float y[8];
+          if (!INTER) unpack8<T>(ring[(stage * LOADS + 1) * kThreads], y, signs);
+          rotate_wide<INTER>(angles + tok * p.half, p.half / N, x, y);
+        }
       }
-      if (part == 0) *reinterpret_cast<uint4*>(q_out + ((long long)i << (p.chunk_shift + 3))) = pack8<T>(x);
+      if (PART == 0)
+        *reinterpret_cast<uint4*>(q_out + ((long long)row << (p.chunk_shift + 3))) = pack8<T>(x);
+      else
+        store_item<T, BITS>(p, PART, c, h, there ? places[tok] : -1, x);
+      if (++stage == NS) stage = 0;
     }
-    if (part > 0) store_item<T, BITS>(p, part, c, h, there ? places[tok] : -1, x);
-    if (++stage == NS) stage = 0;
-  }
-  cp_async_wait<0>();
+    cp_async_wait<0>();
+  };
+  run(std::integral_constant<int, 0>{}, nq, p.q_heads, [&]() {
+    for (int i = threadIdx.x; i < fresh; i += kThreads) {
+      const long long pos = first + i;
+      const int id = kv.page_of(b, pos, p.page_shift);
+      if (id < 0) kv.report(kStatusPage);
+      places[i] = id < 0 ? -1 : ((id * hk) << p.page_shift) | ((int)pos & (kv.page - 1));
+    }
+    for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
+      const int tok = i / p.half, f = i - tok * p.half;
+      cs[tok * p.half + f % N * (p.half / N) + f / N] =
+          rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
+    }
+    __syncthreads();
+  });
+  run(std::integral_constant<int, 1>{}, nk, p.k_heads, [] {});
+  run(std::integral_constant<int, 2>{}, nk, p.k_heads, [] {});
 }
 
 template <typename T, int BITS>
@@ -676,11 +680,11 @@ extern "C" int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100
   // whole tokens until every thread has two items: one round
   const long long per_token = (long long)((q ? q->heads : 0) + 2 * k->heads) * (cache->head_dim / 8);
   long long per_cta = 2 * kThreads / per_token;
-  // prompts: one wave of four CTAs per SM that stream, where that gives each thread
-  // enough rounds
+  // prompts: CTAs that stream, two waves of four per SM (ragged counts leave some
+  // CTAs with less to do), where that gives each thread enough rounds
   const size_t ring = (size_t)kStreamStages * (interleaved ? 1 : 2) * kThreads * 16;
   const size_t each = p.half * sizeof(float2) + sizeof(int);  // of a token
-  const long long slots = 4LL * sm_count() / batch, per_seq = slots < 1 ? 1 : slots;
+  const long long slots = 8LL * sm_count() / batch, per_seq = slots < 1 ? 1 : slots;
   const long long room = (long long)((48 * 1024 - ring) / each);
   long long many = (seqlen + per_seq - 1) / per_seq;
   if (many > room) many = (many + (many + room - 1) / room - 1) / ((many + room - 1) / room);

@@ -38,6 +38,7 @@
 
 #include "fa_kernels.h"
 #include "fa_kv_cache.cuh"
+#include "fast_div.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fa_sm100 {
@@ -89,10 +90,13 @@ struct DecodeParams {
   float* lse;          // (B, H, Sq) or null
   const int* lengths;  // (B)
   const int* starts;   // (B) or null: length - Sq
+  FastDiv grid_div, group_div, rb_div, segs_div;
   float* part_o;       // (2 * grid, ROWS, D)
   float2* part_ml;     // (2 * grid, ROWS): maximum (log2 domain), sum
   int B, Sq, H, group, row_blocks, causal, page_shift, bf16;
-  int grid, negate, whole;  // whole: CTA i computes segment i
+  int negate;
+  int whole;   // a share is whole segments: those that begin in it
+  int direct;  // and CTA i's is segment i
   float scale_log2;  // |scale| log2 e, above 0; `negate`: the scale is negative (q's sign changes)
   unsigned long long timeout_ns;
 };
@@ -186,45 +190,71 @@ __device__ __forceinline__ int tiles_of(int len) {
   return n < 1 ? 1 : n;  // a sequence without tokens has one tile, which writes its zeros
 }
 
-// Sums the places of all sequences in the list (box[0]) and finds the sequence
-// that holds the first place of a share (box[1]) and the places before that
-// sequence (box[2]).  All threads of the CTA take part.
+// The list's places cut into shares: the first `more` hold each + 1, the others
+// `each`.
+struct Shares {
+  unsigned total, each, more;
+  __device__ __forceinline__ unsigned begin(unsigned c) const { return c * each + min(c, more); }
+  __device__ __forceinline__ unsigned of(unsigned place) const {
+    const unsigned cut = more * (each + 1);
+    return place < cut ? place / (each + 1) : more + (place - cut) / each;
+  }
+};
+
+// Where a share begins: the sequence that holds its first place, the places
+// before that sequence, its tiles and length.
+struct Spot {
+  unsigned before;
+  int b, len;
+};
+
+// Sums the places of all sequences and finds the first place of a share.  All
+// threads of the CTA take part; each looks at the sequences of its own.
 template <int TILE>
-__device__ __forceinline__ void locate(const DecodeParams& p, int segs, long long (&box)[3],
-                                       long long* warp_sum, int share) {
+__device__ __forceinline__ Shares locate(const DecodeParams& p, int segs, unsigned share, Spot& spot,
+                                         unsigned* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int chunk = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b)
-    mine += (long long)(tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) + kSegmentCost) * segs;
-  long long before = mine;  // inclusive scan
+  auto places = [&](int len) { return (unsigned)(tiles_of<TILE>(len) + kSegmentCost) * segs; };
+  unsigned mine = 0;
+  int len = 0;
+  for (int b = b0; b < b1; ++b) {
+    len = p.kv.clamp_length(p.lengths[b]);
+    mine += places(len);
+  }
+  unsigned before = mine;  // inclusive scan
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) {
-    const long long o = __shfl_up_sync(0xffffffffu, before, d);
+    const unsigned o = __shfl_up_sync(0xffffffffu, before, d);
     if (lane >= d) before += o;
   }
   if (lane == 31) warp_sum[w] = before;
+  if (tid == 0) spot = {0, 0, 0};  // a share behind the list's end has no first place
   __syncthreads();
-  long long total = 0;
+  Shares sh = {};
 #pragma unroll
   for (int i = 0; i < kWarps; ++i) {
     if (i < w) before += warp_sum[i];
-    total += warp_sum[i];
+    sh.total += warp_sum[i];
   }
-  before -= mine;
-  const long long want = total * share / p.grid;
-  if (tid == 0) box[0] = total;
-  long long at = before;
-  for (int b = b0; b < b1; ++b) {
-    const long long n = (long long)(tiles_of<TILE>(p.kv.clamp_length(p.lengths[b])) + kSegmentCost) * segs;
-    if (want >= at && want < at + n) {
-      box[1] = b;
-      box[2] = at;
+  sh.each = p.grid_div.div(sh.total);
+  sh.more = sh.total - sh.each * p.grid_div.d;
+  const unsigned want = sh.begin(share);
+  unsigned at = before - mine;
+  if (want >= at && want < before) {
+    for (int b = b0; b < b1; ++b) {
+      if (chunk > 1) len = p.kv.clamp_length(p.lengths[b]);
+      const unsigned n = places(len);
+      if (want < at + n) {
+        spot = {at, b, len};
+        break;
+      }
+      at += n;
     }
-    at += n;
   }
   __syncthreads();
+  return sh;
 }
 
 // 8 dims of a finished row: out = x / sum, and the row's log-sum-exp.
@@ -259,7 +289,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   struct Misc {
     uint64_t bars[kWarps * NS];
-    long long box[3], warp_sum[kWarps];
+    Spot spot;
+    unsigned warp_sum[kWarps];
     float2 join_ml[kWarps][8];
     int abort_flag;
   };
@@ -274,38 +305,13 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   if (tid == 0) sh.abort_flag = 0;
   if (lane < NS) mbar_init(my_bars + lane * 8, U);
   fence_barrier_init();
+  __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
 
   const int segs = p.kv.heads * p.row_blocks;  // segments of a sequence
   const WaitCtx wait{&sh.abort_flag, p.kv.status, p.timeout_ns};
-  Cursor cur;
-  long long left;
-  if (p.whole) {
-    cur.b = blockIdx.x / segs;
-    const int hr = blockIdx.x - cur.b * segs;
-    cur.len = p.kv.clamp_length(p.lengths[cur.b]);
-    cur.nt = tiles_of<C::kTile>(cur.len);
-    cur.tt = 0;
-    cur.h = hr / p.row_blocks;
-    cur.rb = hr - cur.h * p.row_blocks;
-    left = cur.nt;
-    __syncthreads();
-  } else {
-    locate<C::kTile>(p, segs, sh.box, sh.warp_sum, blockIdx.x);  // ends with __syncthreads
-    const long long total = sh.box[0];
-    const long long begin = total * blockIdx.x / p.grid, end = total * (blockIdx.x + 1) / p.grid;
-    if (begin >= end) return;
-    cur.b = (int)sh.box[1];
-    cur.len = p.kv.clamp_length(p.lengths[cur.b]);
-    cur.nt = tiles_of<C::kTile>(cur.len);
-    const long long in = begin - sh.box[2];
-    const int places = cur.nt + kSegmentCost, hr = (int)(in / places);
-    cur.tt = (int)(in % places);
-    cur.h = hr / p.row_blocks;
-    cur.rb = hr % p.row_blocks;
-    left = end - begin;
-  }
+  int left;  // places of the share
   // To the next tile; returns the places of the list that this takes.
   auto advance = [&](Cursor& c) {
     if (++c.tt < c.nt) return 1;
@@ -320,30 +326,55 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     c.nt = tiles_of<C::kTile>(c.len);
     return places;
   };
-  if (cur.tt >= cur.nt) {  // the share begins behind a segment's tiles
-    const int over = cur.tt - cur.nt;
-    cur.tt = cur.nt - 1;
-    left -= advance(cur) - 1 - over;
+  Cursor cur;
+  if (p.direct) {
+    cur.b = (int)p.segs_div.div(blockIdx.x);
+    const unsigned hr = blockIdx.x - cur.b * p.segs_div.d;
+    cur.len = p.kv.clamp_length(p.lengths[cur.b]);
+    cur.nt = tiles_of<C::kTile>(cur.len);
+    cur.h = (int)p.rb_div.div(hr);
+    cur.rb = (int)hr - cur.h * p.row_blocks;
+    cur.tt = 0;
+    left = cur.nt;
+    __syncthreads();
+  } else {
+    const Shares shares = locate<C::kTile>(p, segs, blockIdx.x, sh.spot, sh.warp_sum);  // synchronises
+    left = (int)(shares.begin(blockIdx.x + 1) - shares.begin(blockIdx.x));
+    if (left == 0) return;
+    cur.b = sh.spot.b;
+    cur.len = sh.spot.len;
+    cur.nt = tiles_of<C::kTile>(cur.len);
+    const unsigned in = shares.begin(blockIdx.x) - sh.spot.before, places = cur.nt + kSegmentCost;
+    const unsigned hr = in / places;
+    cur.tt = (int)(in - hr * places);
+    cur.h = (int)p.rb_div.div(hr);
+    cur.rb = (int)hr - cur.h * p.row_blocks;
+    if (cur.tt >= cur.nt || (p.whole && cur.tt > 0)) {  // on to the next segment
+      const int over = (int)places - cur.tt;
+      cur.tt = cur.nt - 1;
+      advance(cur);
+      left -= over;
+      if (left <= 0) return;
+    }
   }
 
   // ---- producer: lane u < U brings block u of the warp's share of a tile
+  // (a whole segment that begins in the share is brought to its end)
   Cursor pc = cur;
-  long long to_issue = left;
-  int next_id = -1;
+  int to_issue = left;
+  auto more_to_issue = [&]() { return to_issue > 0 || (p.whole && pc.tt > 0); };
   uint32_t ok_bits = 0;  // this lane's block of each stage holds tokens
   uint32_t in_flight = 0;  // stages whose copies have not been waited for
   auto block_token = [&](const Cursor& c, int u) {
     return c.tt * C::kTile + (warp * U + u) * kBlockTokens;
   };
-  auto look_up = [&]() {  // page of the next block to issue: read ahead of its use
-    next_id = -2;
-    if (lane < U && to_issue > 0) {
-      const int tok = block_token(pc, lane);
-      if (tok < pc.len) next_id = p.kv.table[(long long)pc.b * p.kv.table_width + (tok >> p.page_shift)];
-    }
+  auto look_up = [&](const Cursor& c, bool wanted) {  // page of the lane's block; -2: none
+    const int tok = block_token(c, lane);
+    return wanted && lane < U && tok < c.len
+               ? p.kv.table[(long long)c.b * p.kv.table_width + (tok >> p.page_shift)]
+               : -2;
   };
-  auto issue = [&](int stage) {
-    if (to_issue <= 0) return;
+  auto issue = [&](int stage, int next_id) {
     if (lane < U) {
       const uint32_t bar = my_bars + stage * 8;
       const bool ok = next_id != -2 && !p.kv.bad_page(next_id);
@@ -370,13 +401,10 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     }
     in_flight |= 1u << stage;
     to_issue -= advance(pc);
-    look_up();
   };
-  look_up();
-#pragma unroll 1
-  for (int s = 0; s < NS; ++s) issue(s);
 
   // ---- consumer state
+  uint32_t raw[NT][KSTEPS][2];  // q as it is loaded
   uint32_t qf[NT][KSTEPS][2];   // q as the second operand of S^T
   uint32_t qsum[NT][2];         // 4-bit: (0, head), (0, tail) of group t's sum
   float f[NT][2];               // factor of a score to the log2 domain, per column (above 0)
@@ -392,12 +420,40 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     return n < 0 ? 0 : n < cur.len ? (int)n : cur.len;
   };
 
-  auto begin_segment = [&]() {
-    const int h = cur.h, rb = cur.rb;
+  auto load_q = [&](const Cursor& c) {
     const int rows = p.Sq * p.group;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int rr = c.rb * ROWS + n * 8 + g;
+      const bool there = rr < rows;
+      const int qpos = there ? (int)p.group_div.div(rr) : 0, hq = c.h * p.group + (there ? rr - qpos * p.group : 0);
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (((long long)c.b * p.Sq + qpos) * p.H + hq) * D;
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int k = 0; k < KSTEPS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            raw[n][k][i] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 * i + 2 * t) : 0u;
+      } else {
+#pragma unroll
+        for (int grp = 0; grp < NG; ++grp) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (there) w = *reinterpret_cast<const uint4*>(src + 32 * grp + 8 * t);
+          raw[n][2 * grp][0] = w.x;
+          raw[n][2 * grp][1] = w.y;
+          raw[n][2 * grp + 1][0] = w.z;
+          raw[n][2 * grp + 1][1] = w.w;
+        }
+      }
+    }
+  };
+
+  // Limits, sums and q of the segment at `cur`, whose q load_q has read.
+  auto begin_segment = [&]() {
+    const int rb = cur.rb, rows = p.Sq * p.group;
     start = p.starts ? p.starts[cur.b] : cur.len - p.Sq;
-    qp_first = rb * ROWS / p.group;
-    qp_last = (min(rows, (rb + 1) * ROWS) - 1) / p.group;
+    qp_first = (int)p.group_div.div(rb * ROWS);
+    qp_last = (int)p.group_div.div(min(rows, (rb + 1) * ROWS) - 1);
     min_lim = limit_of(qp_first);
     max_lim = limit_of(qp_last);
 #pragma unroll
@@ -405,8 +461,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int rr = rb * ROWS + n * 8 + 2 * t + i;
-        lim[n][i] = rr < rows ? limit_of(rr / p.group) : 0;
-        col_q[n][i] = rr < rows ? rr / p.group : -1;
+        col_q[n][i] = rr < rows ? (int)p.group_div.div(rr) : -1;
+        lim[n][i] = rr < rows ? limit_of(col_q[n][i]) : 0;
         mf[n][i] = -INFINITY;
         l[n][i] = 0.f;
       }
@@ -417,40 +473,29 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
 
-      const int rr = rb * ROWS + n * 8 + g;
-      const bool there = rr < rows;
-      const int qpos = there ? rr / p.group : 0, hq = h * p.group + (there ? rr % p.group : 0);
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + (((long long)cur.b * p.Sq + qpos) * p.H + hq) * D;
       if constexpr (BITS == 16) {
+        const uint32_t signs = p.negate ? 0x80008000u : 0u;
 #pragma unroll
         for (int k = 0; k < KSTEPS; ++k) {
-          qf[n][k][0] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 2 * t) : 0u;
-          qf[n][k][1] = there ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8 + 2 * t) : 0u;
-        }
-        if (p.negate) {
-#pragma unroll
-          for (int k = 0; k < KSTEPS; ++k) {
-            qf[n][k][0] ^= 0x80008000u;
-            qf[n][k][1] ^= 0x80008000u;
-          }
+          qf[n][k][0] = raw[n][k][0] ^ signs;
+          qf[n][k][1] = raw[n][k][1] ^ signs;
         }
         f[n][0] = f[n][1] = p.scale_log2;
       } else {
         // q scaled by a power of two, largest element in [2^10, 2^11), as fp16;
         // its elements are exact down to 2^-24 of the largest
-        uint4 raw[NG];
+        auto pair = [&](int grp, int i) {
+          const uint32_t w = raw[n][2 * grp + i / 2][i % 2];
+          return p.bf16 ? Elem<__nv_bfloat16>::unpack2(w) : Elem<__half>::unpack2(w);
+        };
         float top = 0.f;
 #pragma unroll
-        for (int grp = 0; grp < NG; ++grp) {
-          raw[grp] = there ? *reinterpret_cast<const uint4*>(src + 32 * grp + 8 * t)
-                           : make_uint4(0, 0, 0, 0);
-          const uint32_t ws[4] = {raw[grp].x, raw[grp].y, raw[grp].z, raw[grp].w};
+        for (int grp = 0; grp < NG; ++grp)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = p.bf16 ? Elem<__nv_bfloat16>::unpack2(ws[i]) : Elem<__half>::unpack2(ws[i]);
+            const float2 v = pair(grp, i);
             top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
           }
-        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
@@ -461,11 +506,10 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         float mine = 0.f;  // sum of group t
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
-          const uint32_t ws[4] = {raw[grp].x, raw[grp].y, raw[grp].z, raw[grp].w};
           float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = p.bf16 ? Elem<__nv_bfloat16>::unpack2(ws[i]) : Elem<__half>::unpack2(ws[i]);
+            const float2 v = pair(grp, i);
             const uint32_t h2 = Elem<__half>::pack2(v.x * turn, v.y * turn);
             const float2 r = Elem<__half>::unpack2(h2);
             sum += r.x + r.y;
@@ -502,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (skipped(u)) continue;
-      const uint32_t blk = base + u * C::kBlockBytes;
+      [[maybe_unused]] const uint32_t blk = base + u * C::kBlockBytes;
       if constexpr (BITS == 16) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -609,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (skipped(u)) continue;
-      const uint32_t blk = base + u * C::kBlockBytes;
+      [[maybe_unused]] const uint32_t blk = base + u * C::kBlockBytes;
       uint32_t pf[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -788,16 +832,40 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   };
 
   // ---- the share, tile by tile
+  // The first pages, q and copies are asked for before anything waits.
+  constexpr bool AHEAD = NT == 1;  // q is read ahead where there are registers for it
+  if (AHEAD) load_q(cur);
+  {
+    int ids[NS];
+    Cursor c = pc;
+    int rest = to_issue;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const bool wanted = rest > 0 || (p.whole && c.tt > 0);
+      ids[s] = look_up(c, wanted);
+      if (wanted) rest -= advance(c);
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      if (more_to_issue()) issue(s, ids[s]);
+  }
+  int next_id = look_up(pc, more_to_issue());  // read ahead of its use
   int stage = 0;
   uint32_t phase = 0;
-  bool fresh = true, first = false;
+  bool fresh = true, first = false, stopped = false;
 #pragma unroll 1
-  while (left > 0) {
+  while (left > 0 || (p.whole && !fresh)) {
     if (fresh) {
       first = cur.tt == 0;
+      if (!AHEAD) load_q(cur);
       begin_segment();
       if (first && tid == 0 && cur.h == 0 && cur.rb == 0 && p.kv.bad_length(p.lengths[cur.b])) p.kv.report(kStatusPage);
     }
+    const bool last = cur.tt + 1 == cur.nt;
+    Cursor next = cur;
+    const int places = advance(next);
+    const bool goes_on = left > places || (p.whole && !last);
+    if (AHEAD && last && goes_on) load_q(next);
     const bool here = mbar_wait(my_bars + stage * 8, phase, wait);
     if (here) {
       in_flight &= ~(1u << stage);
@@ -808,15 +876,15 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         step(stage, ok, std::true_type{});
     }
     __syncwarp();
-    if (here) {
-      issue(stage);
-    } else {
-      to_issue = 0;  // a copy did not arrive: bring no more
+    stopped |= !here;  // a copy did not arrive: bring no more
+    if (!stopped && more_to_issue()) {
+      issue(stage, next_id);
+      next_id = look_up(pc, more_to_issue());
     }
-    const bool last = cur.tt + 1 == cur.nt;
-    if (last || left == 1) end_segment(first, last);
+    if (last || !goes_on) end_segment(first, last);
     fresh = last;
-    left -= advance(cur);
+    left -= places;
+    cur = next;
     if (++stage == NS) {
       stage = 0;
       phase ^= 1;
@@ -836,20 +904,23 @@ template <int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeParams p) {
   using C = Cfg<D, BITS, NT>;
   constexpr int ROWS = 8 * NT, PER_ROW = D / 8, P = kThreads / 2 / PER_ROW;
-  __shared__ long long box[3], warp_sum[kWarps];
+  __shared__ Spot spot;
+  __shared__ unsigned warp_sum[kWarps];
   __shared__ float4 part_x[2][P][D / 4];
   __shared__ float2 part_ml[2][P];
-  const int segs = p.kv.heads * p.row_blocks, border = blockIdx.x + 1;
-  locate<C::kTile>(p, segs, box, warp_sum, border);
-  const long long total = box[0], at = total * border / p.grid, in = at - box[2];
-  const int b = (int)box[1], nt = tiles_of<C::kTile>(p.kv.clamp_length(p.lengths[b]));
-  const int places = nt + kSegmentCost, hr = (int)(in / places);
-  const long long t0 = box[2] + (long long)hr * places, t1 = t0 + nt - 1;
-  griddep_wait();
+  const int segs = p.kv.heads * p.row_blocks;
+  const unsigned border = blockIdx.x + 1;
+  const Shares shares = locate<C::kTile>(p, segs, border, spot, warp_sum);
+  const unsigned at = shares.begin(border);
+  const int b = spot.b, nt = tiles_of<C::kTile>(spot.len);
+  const unsigned places = nt + kSegmentCost, hr = (at - spot.before) / places;
+  const unsigned t0 = spot.before + hr * places, t1 = t0 + nt - 1;
+  const bool crossed = at < shares.total && at > t0 && at <= t1 && shares.begin(border - 1) <= t0;
+  const int c0 = (int)border - 1, c1 = crossed ? (int)shares.of(t1) : 0;
+  griddep_wait();  // also where nothing is to do: the grid after this one may rely on it
   griddep_launch_dependents();
-  if (at == t0 || at > t1 || total * (border - 1) / p.grid > t0) return;
-  const int c0 = border - 1, c1 = (int)(((t1 + 1) * p.grid - 1) / total);
-  const int h = hr / p.row_blocks, rb = hr % p.row_blocks, rows = p.Sq * p.group;
+  if (!crossed) return;
+  const int h = (int)p.rb_div.div(hr), rb = (int)hr - h * p.row_blocks, rows = p.Sq * p.group;
   const int half = threadIdx.x / (kThreads / 2), i = threadIdx.x % (kThreads / 2);
   const int pg = i / PER_ROW, d = i % PER_ROW * 8;
   for (int pair = blockIdx.y; pair < ROWS / 2; pair += gridDim.y) {
@@ -866,7 +937,6 @@ __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeP
     };
 #pragma unroll 4
     for (int c = c0 + pg; c <= c1; c += P) {
-      if (total * (c + 1) / p.grid == total * c / p.grid) continue;  // an empty share
       const long long slot = (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r;
       const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
       const float4 u = src[0], v = src[1];
@@ -896,13 +966,13 @@ int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
   constexpr int kTag = 1000 + ((sizeof(T) == 2 && Elem<T>::kIdescAB == 0) ? 0 : 1) + 2 * NT +
                        8 * (BITS == 4) + 16 * D;
   if (!smem_attr_set<kTag>(reinterpret_cast<const void*>(kernel), C::kSmem)) return FA_ERR_LAUNCH;
-  if (launch_pdl(kernel, dim3(p.grid), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
+  if (launch_pdl(kernel, dim3(p.grid_div.d), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
     return FA_ERR_LAUNCH;
   if (!split) return FA_OK;
   // Many shares to a segment (few segments): its rows are spread over CTAs, too.
   const long long segs = (long long)p.B * p.kv.heads * p.row_blocks;
-  const unsigned y = p.grid > 8 * segs ? 4 * NT : NT;
-  return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid - 1, y), dim3(kThreads), 0, st,
+  const unsigned y = p.grid_div.d > 8 * segs ? 4 * NT : NT;
+  return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid_div.d - 1, y), dim3(kThreads), 0, st,
                     p) == cudaSuccess
              ? FA_OK
              : FA_ERR_LAUNCH;
@@ -945,9 +1015,12 @@ int launch_decode_any(DecodeParams& p, int nt, const CUtensorMap& tk, const CUte
 
 // Tokens up to which a segment is not split.
 constexpr int kWholeTokens = 1024;
+// Places are counted in 31 bits.
+constexpr long long kMaxPlaces = 1LL << 31;
 
 struct Plan {
   int nt, row_blocks, grid;
+  long long places;  // of the list, at most
   bool split;  // segments may cross shares: a second launch joins them
 };
 
@@ -961,12 +1034,12 @@ Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen,
   pl.nt = (int)((rows + 8LL * pl.row_blocks - 1) / (8LL * pl.row_blocks));
   const int tile = kWarps * kBlockTokens * blocks_of(c->head_dim, c->bits, pl.nt);
   const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
-  const long long tiles = (long long)batch * c->nheads_kv * pl.row_blocks * per_seg;
+  const long long segs = (long long)batch * c->nheads_kv * pl.row_blocks, tiles = segs * per_seg;
   const long long most = (long long)sm_count() * kCtas;
-  // Short tables: a CTA per segment, no join.
-  const long long segs = tiles / per_seg;
-  pl.split = (long long)table_width * c->page_size > kWholeTokens || segs > (1LL << 30);
-  pl.grid = (int)(!pl.split ? segs : tiles < most ? tiles : most);
+  pl.places = segs * (per_seg + kSegmentCost);
+  pl.split = (long long)table_width * c->page_size > kWholeTokens;
+  const long long grid = pl.split ? tiles : segs;
+  pl.grid = (int)(grid < most ? grid : most);
   if (pl.grid == 1) pl.split = false;
   return pl;
 }
@@ -989,7 +1062,8 @@ extern "C" size_t fa_sm100_decode_workspace_bytes(const fa_sm100_kv_cache* cache
                                                   int batch, int seqlen, int nheads) {
   using namespace fa_sm100;
   if (!decode_shape_ok(cache, table_width, batch, seqlen, nheads)) return 0;
-  return partial_bytes(plan_of(cache, table_width, batch, seqlen, nheads), cache->head_dim) + 256;
+  const Plan pl = plan_of(cache, table_width, batch, seqlen, nheads);
+  return pl.places < kMaxPlaces ? partial_bytes(pl, cache->head_dim) + 256 : 0;
 }
 
 extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, void* out, float* lse,
@@ -1007,6 +1081,7 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   int rc = bind_device();
   if (rc != FA_OK) return rc;
   const Plan pl = plan_of(cache, table_width, batch, seqlen, nheads);
+  if (pl.places >= kMaxPlaces) return FA_ERR_ARG;
   const size_t need = partial_bytes(pl, cache->head_dim);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return FA_ERR_WORKSPACE;
@@ -1036,8 +1111,12 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   p.row_blocks = pl.row_blocks;
   p.causal = causal ? 1 : 0;
   while ((1 << p.page_shift) < cache->page_size) ++p.page_shift;
-  p.grid = pl.grid;
-  p.whole = !pl.split && pl.grid > 1;
+  p.grid_div = FastDiv(pl.grid);
+  p.group_div = FastDiv(p.group);
+  p.rb_div = FastDiv(pl.row_blocks);
+  p.segs_div = FastDiv(cache->nheads_kv * pl.row_blocks);
+  p.whole = !pl.split;
+  p.direct = p.whole && pl.grid == (long long)batch * cache->nheads_kv * pl.row_blocks;
   p.negate = sm_scale < 0.f;
   p.bf16 = cache->dtype == FA_DTYPE_BF16;
   p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);

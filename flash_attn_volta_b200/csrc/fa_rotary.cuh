@@ -4,6 +4,8 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include "fast_div.cuh"
+
 namespace fa_sm100 {
 
 // (M cos a, M sin a) of a = pos * inv_freq.  The angle of a far position is
@@ -22,18 +24,6 @@ __device__ __forceinline__ float2 rotary_cos_sin(double pos, double inv_freq, fl
   sincospif(head, &s, &c);
   return make_float2(magnitude * fmaf(-d, s, c), magnitude * fmaf(d, c, s));
 }
-
-// Division of n < 2^31 by a number fixed at launch as one high product, an
-// addition and a shift (Granlund and Montgomery).
-struct FastDiv {
-  unsigned d, mul, shift;
-  FastDiv() = default;
-  explicit FastDiv(unsigned divisor) : d(divisor), shift(0) {
-    while ((1ull << shift) < d) ++shift;
-    mul = (unsigned)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
-  }
-  __device__ __forceinline__ unsigned div(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
-};
 
 // N consecutive 16-bit elements as one load or store.
 template <int N>

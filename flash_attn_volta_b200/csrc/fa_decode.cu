@@ -63,6 +63,15 @@ constexpr int stages_of(int D, int bits, int nt) {
   return bits == 16 ? 3 : D == 128 ? (nt == 1 ? 2 : 4) : 4;
 }
 constexpr int kCtas = 2;
+// The start and end of a segment (its q, the join of the warps) take a CTA about
+// as long as so many tiles, so the list has that many empty places behind each
+// segment's tiles and shares with many short segments hold fewer tiles.  96
+// sequences of 5 to 8192 tokens at 4 bits (tiles of 256): 134, 114, 105, 108 us
+// with 0, 1, 2, 4 places; 24 sequences of 5 query tokens (tiles of 128): 45, 41,
+// 37, 36 us; 64 sequences at 16 bits (tiles of 64): 180, 177, 175, 179 us.
+constexpr int cost_of(int D, int bits, int nt) {
+  return bits == 4 ? 512 / (kWarps * blocks_of(D, bits, nt) * 16) : 2;
+}
 
 template <int D, int BITS, int NT>
 struct Cfg {
@@ -71,6 +80,7 @@ struct Cfg {
   static constexpr int kStageBytes = kU * kBlockBytes;
   static constexpr int kStages = stages_of(D, BITS, NT);
   static constexpr int kTile = kWarps * kU * kBlockTokens;  // tokens
+  static constexpr int kCost = cost_of(D, BITS, NT);
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
   static constexpr int kJoinStride = D + 4;  // floats of a row in the join buffer
   // The warps join all 8 rows of a column block at once, or 4 where there is no room.
@@ -179,11 +189,6 @@ struct Cursor {
   int b, h, rb, tt, nt, len;  // sequence, K/V head, row block, tile of nt (nt: behind them), length
 };
 
-// The start and end of a segment (its q, the join of the warps) take a CTA about
-// as long as kSegmentCost tiles, so the list has that many empty places behind
-// each segment's tiles and shares with many short segments hold fewer tiles.
-constexpr int kSegmentCost = 4;
-
 template <int TILE>
 __device__ __forceinline__ int tiles_of(int len) {
   const int n = (len + TILE - 1) / TILE;
@@ -210,13 +215,13 @@ struct Spot {
 
 // Sums the places of all sequences and finds the first place of a share.  All
 // threads of the CTA take part; each looks at the sequences of its own.
-template <int TILE>
+template <int TILE, int COST>
 __device__ __forceinline__ Shares locate(const DecodeParams& p, int segs, unsigned share, Spot& spot,
                                          unsigned* warp_sum) {
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int chunk = (p.B + kThreads - 1) / kThreads;
   const int b0 = min(tid * chunk, p.B), b1 = min(b0 + chunk, p.B);
-  auto places = [&](int len) { return (unsigned)(tiles_of<TILE>(len) + kSegmentCost) * segs; };
+  auto places = [&](int len) { return (unsigned)(tiles_of<TILE>(len) + COST) * segs; };
   unsigned mine = 0;
   int len = 0;
   for (int b = b0; b < b1; ++b) {
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   // To the next tile; returns the places of the list that this takes.
   auto advance = [&](Cursor& c) {
     if (++c.tt < c.nt) return 1;
-    const int places = 1 + kSegmentCost + c.nt - c.tt;
+    const int places = 1 + C::kCost + c.nt - c.tt;
     c.tt = 0;
     if (++c.rb < p.row_blocks) return places;
     c.rb = 0;
@@ -338,13 +343,13 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     left = cur.nt;
     __syncthreads();
   } else {
-    const Shares shares = locate<C::kTile>(p, segs, blockIdx.x, sh.spot, sh.warp_sum);  // synchronises
+    const Shares shares = locate<C::kTile, C::kCost>(p, segs, blockIdx.x, sh.spot, sh.warp_sum);  // synchronises
     left = (int)(shares.begin(blockIdx.x + 1) - shares.begin(blockIdx.x));
     if (left == 0) return;
     cur.b = sh.spot.b;
     cur.len = sh.spot.len;
     cur.nt = tiles_of<C::kTile>(cur.len);
-    const unsigned in = shares.begin(blockIdx.x) - sh.spot.before, places = cur.nt + kSegmentCost;
+    const unsigned in = shares.begin(blockIdx.x) - sh.spot.before, places = cur.nt + C::kCost;
     const unsigned hr = in / places;
     cur.tt = (int)(in - hr * places);
     cur.h = (int)p.rb_div.div(hr);
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   uint32_t ok_bits = 0;  // this lane's block of each stage holds tokens
   uint32_t in_flight = 0;  // stages whose copies have not been waited for
   auto block_token = [&](const Cursor& c, int u) {
-    return c.tt * C::kTile + (warp * U + u) * kBlockTokens;
+    return c.tt * C::kTile + (u * kWarps + warp) * kBlockTokens;  // a short tile's blocks go to all warps
   };
   auto look_up = [&](const Cursor& c, bool wanted) {  // page of the lane's block; -2: none
     const int tok = block_token(c, lane);
@@ -870,7 +875,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     if (here) {
       in_flight &= ~(1u << stage);
       const uint32_t ok = __ballot_sync(0xffffffffu, ok_bits >> stage & 1u) & ((1u << U) - 1u);
-      if (ok == (1u << U) - 1u && block_token(cur, U) <= min_lim)
+      if (ok == (1u << U) - 1u && block_token(cur, U - 1) + kBlockTokens <= min_lim)
         step(stage, ok, std::false_type{});
       else if (ok != 0)
         step(stage, ok, std::true_type{});
@@ -910,10 +915,10 @@ __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeP
   __shared__ float2 part_ml[2][P];
   const int segs = p.kv.heads * p.row_blocks;
   const unsigned border = blockIdx.x + 1;
-  const Shares shares = locate<C::kTile>(p, segs, border, spot, warp_sum);
+  const Shares shares = locate<C::kTile, C::kCost>(p, segs, border, spot, warp_sum);
   const unsigned at = shares.begin(border);
   const int b = spot.b, nt = tiles_of<C::kTile>(spot.len);
-  const unsigned places = nt + kSegmentCost, hr = (at - spot.before) / places;
+  const unsigned places = nt + C::kCost, hr = (at - spot.before) / places;
   const unsigned t0 = spot.before + hr * places, t1 = t0 + nt - 1;
   const bool crossed = at < shares.total && at > t0 && at <= t1 && shares.begin(border - 1) <= t0;
   const int c0 = (int)border - 1, c1 = crossed ? (int)shares.of(t1) : 0;
@@ -1036,7 +1041,7 @@ Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen,
   const long long per_seg = ((long long)table_width * c->page_size + tile - 1) / tile;
   const long long segs = (long long)batch * c->nheads_kv * pl.row_blocks, tiles = segs * per_seg;
   const long long most = (long long)sm_count() * kCtas;
-  pl.places = segs * (per_seg + kSegmentCost);
+  pl.places = segs * (per_seg + cost_of(c->head_dim, c->bits, pl.nt));
   pl.split = (long long)table_width * c->page_size > kWholeTokens;
   const long long grid = pl.split ? tiles : segs;
   pl.grid = (int)(grid < most ? grid : most);

@@ -23,10 +23,12 @@
 // errors of the C ABI raise RuntimeError with the library's message.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <atomic>
 #include <mutex>
 #include <tuple>
 
@@ -181,6 +183,25 @@ void merge_cuda(at::Tensor& acc_o, at::Tensor& acc_lse, const at::Tensor& o_in,
   check_rc(rc, "fa_sm100_merge");
 }
 
+// The serving operators run on a few tokens at a time, where the host's steps
+// are what counts: outputs are allocated without a dispatch, and the status
+// word's address is kept.
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, at::Device device) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, device, std::nullopt));
+}
+
+int* status_ptr(at::Device device) {
+  static std::atomic<int*> kept[kMaxDev];
+  const int i = device.index();
+  if (i < 0 || i >= kMaxDev) return status_word(i).data_ptr<int>();  // refuses the index
+  int* ptr = kept[i].load(std::memory_order_acquire);
+  if (!ptr) {
+    ptr = status_word(i).data_ptr<int>();
+    kept[i].store(ptr, std::memory_order_release);
+  }
+  return ptr;
+}
+
 // ------------------------------------------------------------ rotary positions
 using OptTensor = std::optional<at::Tensor>;
 
@@ -265,7 +286,8 @@ void rotary_launch(const at::Tensor& q_in, const at::Tensor* k_in, at::Tensor& q
 at::Tensor rotary_cuda(const at::Tensor& x, const at::Tensor& inv_freq, const OptTensor& positions,
                        int64_t first, bool interleaved, double magnitude, bool inverse) {
   c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor out = at::empty(x.sizes(), x.options());
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  at::Tensor out = new_tensor(x.sizes(), x.scalar_type(), x.device());
   rotary_launch(x, nullptr, out, nullptr, inv_freq, positions, first, interleaved, magnitude, inverse);
   return out;
 }
@@ -275,8 +297,9 @@ std::tuple<at::Tensor, at::Tensor> rotary_qk_cuda(const at::Tensor& q, const at:
                                                   const OptTensor& positions, int64_t first,
                                                   bool interleaved, double magnitude, bool inverse) {
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor qo = at::empty(q.sizes(), q.options());
-  at::Tensor ko = at::empty(k.sizes(), k.options());
+  TORCH_CHECK(q.is_cuda() && k.device() == q.device(), "q and k must be on one CUDA device");
+  at::Tensor qo = new_tensor(q.sizes(), q.scalar_type(), q.device());
+  at::Tensor ko = new_tensor(k.sizes(), k.scalar_type(), k.device());
   rotary_launch(q, &k, qo, &ko, inv_freq, positions, first, interleaved, magnitude, inverse);
   return {qo, ko};
 }
@@ -445,9 +468,9 @@ at::Tensor kv_append_cuda(const at::Tensor& k_pages, const OptTensor& v_pages, c
     q = heads_input(*q_in, "q", false);
     check_like(q, {B, S, q.size(2), D}, k, "q");
     TORCH_CHECK(q.scalar_type() == k.scalar_type(), "q must have k's dtype");
-    q_out = at::empty(q.sizes(), q.options());
+    q_out = new_tensor(q.sizes(), q.scalar_type(), q.device());
   } else {
-    q_out = at::empty({0}, k.options());
+    q_out = new_tensor({0}, k.scalar_type(), k.device());
   }
   const at::Tensor table = int_input(table_in, 2, B, k_pages, "page_table");
   const at::Tensor starts = int_input(starts_in, 1, B, k_pages, "starts");
@@ -462,13 +485,12 @@ at::Tensor kv_append_cuda(const at::Tensor& k_pages, const OptTensor& v_pages, c
   fa_sm100_heads hq;
   const bool with_q = q.defined() && q.size(2) > 0;
   if (with_q) hq = heads_of(q, &q_out);
-  at::Tensor st = status_word(k_pages.get_device());
   const int rc = fa_sm100_kv_append(
       &cache, &hk, &hv, with_q ? &hq : nullptr, table.data_ptr<int>(), (int)table.size(1),
       starts.data_ptr<int>(), counts.defined() ? counts.data_ptr<int>() : nullptr,
       freq.defined() ? freq.data_ptr<double>() : nullptr,
       freq.defined() ? 2 * (int)freq.size(0) : 0, interleaved, (float)magnitude, (int)B, (int)S,
-      st.data_ptr<int>(), at::cuda::getCurrentCUDAStream().stream());
+      status_ptr(k_pages.device()), at::cuda::getCurrentCUDAStream().stream());
   check_rc(rc, "fa_sm100_kv_append");
   return q_out;
 }
@@ -484,14 +506,12 @@ std::tuple<at::Tensor, at::Tensor> kv_read_cuda(const at::Tensor& k_pages, const
   const at::Tensor lengths = int_input(lengths_in, 1, B, k_pages, "lengths");
   TORCH_CHECK(max_len >= 0 && max_len <= 2147483647, "max_len out of range");
   c10::cuda::CUDAGuard guard(k_pages.device());
-  const auto opts = k_pages.options().dtype(dtype);
-  at::Tensor k = at::empty({B, max_len, cache.nheads_kv, cache.head_dim}, opts);
-  at::Tensor v = at::empty({B, max_len, cache.nheads_kv, cache.head_dim}, opts);
+  at::Tensor k = new_tensor({B, max_len, cache.nheads_kv, cache.head_dim}, dtype, k_pages.device());
+  at::Tensor v = new_tensor({B, max_len, cache.nheads_kv, cache.head_dim}, dtype, k_pages.device());
   if (B == 0 || max_len == 0) return {k, v};
-  at::Tensor st = status_word(k_pages.get_device());
   const int rc = fa_sm100_kv_read(&cache, table.data_ptr<int>(), (int)table.size(1),
                                   lengths.data_ptr<int>(), k.data_ptr(), v.data_ptr(), (int)B,
-                                  (int)max_len, st.data_ptr<int>(),
+                                  (int)max_len, status_ptr(k_pages.device()),
                                   at::cuda::getCurrentCUDAStream().stream());
   check_rc(rc, "fa_sm100_kv_read");
   return {k, v};
@@ -513,21 +533,20 @@ at::Tensor decode_launch(const at::Tensor& q_in, const at::Tensor& k_pages,
   at::Tensor starts;
   if (starts_in) starts = int_input(*starts_in, 1, B, k_pages, "starts");
   c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
-  if (lse) *lse = at::empty({B, H, S}, q.options().dtype(at::kFloat));
+  at::Tensor out = new_tensor(q.sizes(), q.scalar_type(), q.device());
+  if (lse) *lse = new_tensor({B, H, S}, at::kFloat, q.device());
   if (B * S == 0) return out;
   const size_t nbytes = fa_sm100_decode_workspace_bytes(&cache, (int)table.size(1), (int)B, (int)S, (int)H);
   TORCH_CHECK(nbytes > 0, "fa_sm100_decode: unsupported shape");
   // 256 bytes mean that the shape needs none
   at::Tensor ws;
-  if (nbytes > 256) ws = at::empty({(int64_t)nbytes}, q.options().dtype(at::kByte));
-  at::Tensor st = status_word(q.get_device());
+  if (nbytes > 256) ws = new_tensor({(int64_t)nbytes}, at::kByte, q.device());
   const int rc = fa_sm100_decode(
       &cache, q.data_ptr(), out.data_ptr(), lse ? lse->data_ptr<float>() : nullptr,
       table.data_ptr<int>(), (int)table.size(1), lengths.data_ptr<int>(),
       starts.defined() ? starts.data_ptr<int>() : nullptr,
       ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? nbytes : 0, (int)B, (int)S,
-      (int)H, (float)sm_scale, causal ? 1 : 0, st.data_ptr<int>(),
+      (int)H, (float)sm_scale, causal ? 1 : 0, status_ptr(q.device()),
       at::cuda::getCurrentCUDAStream().stream());
   check_rc(rc, "fa_sm100_decode");
   return out;

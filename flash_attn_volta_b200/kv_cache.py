@@ -94,19 +94,47 @@ class PagedKVCache:
                    torch.empty(shape, dtype=dtype, device=device))
 
 
-def _check_table(page_table, batch, dev):
+_INFERENCE = "the cache operators are for inference: call them under torch.no_grad()"
+
+
+# The operators check their arguments themselves; the assertions, which say what
+# is wrong in this module's terms, run when one refuses (they cost as much host
+# time as a small call's launch).
+def _check_ints(cache, batch, page_table, **vectors):
+    dev = cache.device
+    assert dev.type == "cuda", "the cache must be on CUDA"
     shape = page_table.shape
     assert len(shape) == 2 and shape[0] == batch and shape[1] > 0 \
         and page_table.dtype == torch.int32 and page_table.device == dev, \
         "page_table must be (batch, pages) int32 on the cache's device"
+    for name, t in vectors.items():
+        assert t is None or (t.shape == (batch,) and t.dtype == torch.int32 and t.device == dev), \
+            f"{name} must be (batch,) int32 on the cache's device"
 
 
-def _check_vector(t, batch, dev, name):
-    assert t.shape == (batch,) and t.dtype == torch.int32 and t.device == dev, \
-        f"{name} must be (batch,) int32 on the cache's device"
+def _check_append(cache, k, v, page_table, starts, counts, q, rotary):
+    shape = k.shape
+    assert len(shape) == 4 and v.shape == shape, f"kv shape mismatch {shape} {v.shape}"
+    B, S, Hkv, D = shape
+    assert Hkv == cache.n_heads and D == cache.head_dim, \
+        f"k {tuple(shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
+    assert v.dtype == cache.dtype, f"k and v must have the cache's dtype {cache.dtype}"
+    assert k.device == v.device == cache.device, "k and v must be on the cache's device"
+    _check_ints(cache, B, page_table, starts=starts, counts=counts)
+    if q is not None:
+        assert q.dim() == 4 and q.shape[:2] == (B, S) and q.shape[3] == D and q.dtype == k.dtype \
+            and q.device == cache.device, f"q {tuple(q.shape)} does not fit k {tuple(shape)}"
+    if rotary is not None:
+        assert rotary.dim <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
+        assert rotary.inv_freq.device == cache.device, "inv_freq must be on the cache's device"
 
 
-_INFERENCE = "the cache operators are for inference: call them under torch.no_grad()"
+def _check_decode(q, cache, page_table, lengths, starts):
+    shape, H = q.shape, cache.n_heads
+    assert len(shape) == 4 and shape[3] == cache.head_dim and shape[2] > 0 and shape[2] % H == 0, \
+        f"q {tuple(shape)} does not fit a cache of {H} heads of {cache.head_dim}"
+    assert q.device == cache.device, "q must be on the cache's device"
+    _check_ints(cache, shape[0], page_table, lengths=lengths, starts=starts)
 
 
 def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
@@ -124,36 +152,22 @@ def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
             without ``rotary``), contiguous, padding rows included.
     No two tokens of one call may go to the same place of the cache.
     """
-    shape = k.shape
-    assert len(shape) == 4 and v.shape == shape, f"kv shape mismatch {shape} {v.shape}"
-    B, S, Hkv, D = shape
-    assert Hkv == cache.n_heads and D == cache.head_dim, \
-        f"k {tuple(shape)} does not fit a cache of {cache.n_heads} heads of {cache.head_dim}"
-    dev, dtype = cache.device, cache.dtype
-    assert dev.type == "cuda", "the cache must be on CUDA"
-    assert k.dtype == dtype and v.dtype == dtype, f"k and v must have the cache's dtype {dtype}"
-    assert k.device == dev and v.device == dev, "k and v must be on the cache's device"
-    _check_table(page_table, B, dev)
-    _check_vector(starts, B, dev, "starts")
-    if counts is not None:
-        _check_vector(counts, B, dev, "counts")
-    grad = k.requires_grad or v.requires_grad
-    if q is not None:
-        qs = q.shape
-        assert len(qs) == 4 and qs[0] == B and qs[1] == S and qs[3] == D and q.dtype == dtype \
-            and q.device == dev, f"q {tuple(qs)} does not fit k {tuple(shape)}"
-        grad = grad or q.requires_grad
-    assert not (grad and torch.is_grad_enabled()), _INFERENCE
+    dtype, dev = cache.dtype, cache.device
+    assert k.dtype == dtype, f"k and v must have the cache's dtype {dtype}"
+    assert not ((k.requires_grad or v.requires_grad or (q is not None and q.requires_grad))
+                and torch.is_grad_enabled()), _INFERENCE
     if rotary is None:
         freq, interleaved, magnitude = None, False, 1.0
     else:
         freq, interleaved, magnitude = rotary.inv_freq, rotary.interleaved, rotary.magnitude
-        assert 2 * freq.shape[0] <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
-        assert freq.device == dev, "inv_freq must be on the cache's device"
     ops.load()
+    try:
+        out = torch.ops.fav.kv_append(cache.k_pages, cache.v_pages, k, v, q, page_table, starts,
+                                      counts, freq, interleaved, magnitude)
+    except RuntimeError:
+        _check_append(cache, k, v, page_table, starts, counts, q, rotary)
+        raise
     ops.note_device(dev.index)
-    out = torch.ops.fav.kv_append(cache.k_pages, cache.v_pages, k, v, q, page_table, starts, counts,
-                                  freq, interleaved, magnitude)
     if _lib.debug_sync():
         _lib.check_status(dev)
     return out if q is not None else None
@@ -167,10 +181,8 @@ def kv_cache_read(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.
     if max_len is None:
         max_len = page_table.shape[-1] * cache.page_size
     assert max_len >= 0, "max_len must not be negative"
-    dev, B = cache.device, lengths.shape[0]
-    assert dev.type == "cuda", "the cache must be on CUDA"
-    _check_table(page_table, B, dev)
-    _check_vector(lengths, B, dev, "lengths")
+    dev = cache.device
+    _check_ints(cache, lengths.shape[0], page_table, lengths=lengths)
     ops.load()
     ops.note_device(dev.index)
     k, v = torch.ops.fav.kv_read(cache.k_pages, cache.v_pages, cache.dtype, page_table, lengths,
@@ -200,23 +212,19 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
         out (B, S, H, D), with return_softmax_lse also lse (B, H, S) fp32.  A row
         that sees no token gets out 0 and lse +inf.
     """
-    shape, H = q.shape, cache.n_heads
-    assert len(shape) == 4 and shape[3] == cache.head_dim and shape[2] > 0 and shape[2] % H == 0, \
-        f"q {tuple(shape)} does not fit a cache of {H} heads of {cache.head_dim}"
-    dev, B = cache.device, shape[0]
-    assert dev.type == "cuda", "the cache must be on CUDA"
-    assert q.dtype == cache.dtype and q.device == dev, "q must have the cache's dtype and device"
-    _check_table(page_table, B, dev)
-    _check_vector(lengths, B, dev, "lengths")
-    if starts is not None:
-        _check_vector(starts, B, dev, "starts")
+    assert q.dtype == cache.dtype, f"q must have the cache's dtype {cache.dtype}"
     assert not (q.requires_grad and torch.is_grad_enabled()), _INFERENCE
     if sm_scale is None:
-        sm_scale = 1.0 / math.sqrt(shape[3])
+        sm_scale = 1.0 / math.sqrt(cache.head_dim)
     ops.load()
-    ops.note_device(dev.index)
     fn = torch.ops.fav.decode_lse if return_softmax_lse else torch.ops.fav.decode
-    out = fn(q, cache.k_pages, cache.v_pages, page_table, lengths, starts, causal, sm_scale)
+    try:
+        out = fn(q, cache.k_pages, cache.v_pages, page_table, lengths, starts, causal, sm_scale)
+    except RuntimeError:
+        _check_decode(q, cache, page_table, lengths, starts)
+        raise
+    dev = cache.device
+    ops.note_device(dev.index)
     if _lib.debug_sync():
         _lib.check_status(dev)
     return out

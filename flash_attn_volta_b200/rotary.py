@@ -79,12 +79,13 @@ class Rotary:
         return cls(inv.to(device), interleaved, magnitude)
 
 
-def _check(x: torch.Tensor, rotary: Rotary, positions) -> None:
+def _check(x: torch.Tensor, rotary: Rotary, positions, k=None) -> None:
+    """Raise AssertionError for a call the operators refuse."""
     shape, dev = x.shape, x.device
     assert dev.type == "cuda", "tensors must be on CUDA"
     assert x.dtype in (torch.float16, torch.bfloat16), "fp16 (or bf16) only"
     assert len(shape) == 4, "expected (batch, seqlen, heads, head_dim)"
-    assert shape[3] % 2 == 0 and 2 * rotary.inv_freq.shape[0] <= shape[3], \
+    assert shape[3] % 2 == 0 and rotary.dim <= shape[3], \
         f"rotary dim {rotary.dim} does not fit head_dim {shape[3]}"
     assert rotary.inv_freq.device == dev, "inv_freq must be on the tensors' device"
     if positions is not None:
@@ -92,8 +93,16 @@ def _check(x: torch.Tensor, rotary: Rotary, positions) -> None:
         assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
         assert positions.shape in (shape[:2], shape[1:2]), \
             f"positions must be (seqlen,) or (batch, seqlen), got {tuple(positions.shape)}"
+    if k is not None:
+        ks = k.shape
+        assert len(ks) == 4 and shape[:2] == ks[:2] and shape[3] == ks[3], \
+            f"qk shape mismatch {shape} {ks}"
+        assert k.dtype == x.dtype and k.device == dev, "q and k must have one dtype and device"
 
 
+# The operators check their arguments themselves; the assertions, which say what
+# is wrong in this module's terms, run when one refuses (they cost as much host
+# time as a small call's launch).
 def rotary_embed(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor | None = None,
                  first: int = 0) -> torch.Tensor:
     """x (B, S, H, D), fp16 or bf16, any strides, rotated; autograd-aware.
@@ -101,10 +110,13 @@ def rotary_embed(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor | None
     positions: (S,) or (B, S) int32 / int64; None: first, first + 1, ...
     The result is contiguous, in x's dtype; sums are in fp32, rounded once.
     """
-    _check(x, rotary, positions)
     ops.load()
-    return torch.ops.fav.rotary(x, rotary.inv_freq, positions, first, rotary.interleaved,
-                                rotary.magnitude, False)
+    try:
+        return torch.ops.fav.rotary(x, rotary.inv_freq, positions, first, rotary.interleaved,
+                                    rotary.magnitude, False)
+    except RuntimeError:
+        _check(x, rotary, positions)
+        raise
 
 
 def rotary_embed_qk(q: torch.Tensor, k: torch.Tensor, rotary: Rotary,
@@ -112,14 +124,13 @@ def rotary_embed_qk(q: torch.Tensor, k: torch.Tensor, rotary: Rotary,
                     first: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
     """rotary_embed of q (B, S, H, D) and k (B, S, H_kv, D) at the same
     positions, in one launch (and one for both gradients)."""
-    _check(q, rotary, positions)
-    qs, ks = q.shape, k.shape
-    assert len(ks) == 4 and qs[0] == ks[0] and qs[1] == ks[1] and qs[3] == ks[3], \
-        f"qk shape mismatch {qs} {ks}"
-    assert k.dtype == q.dtype and k.device == q.device, "q and k must have one dtype and device"
     ops.load()
-    return torch.ops.fav.rotary_qk(q, k, rotary.inv_freq, positions, first, rotary.interleaved,
-                                   rotary.magnitude, False)
+    try:
+        return torch.ops.fav.rotary_qk(q, k, rotary.inv_freq, positions, first,
+                                       rotary.interleaved, rotary.magnitude, False)
+    except RuntimeError:
+        _check(q, rotary, positions, k)
+        raise
 
 
 def rotate_for_attention(q, k, rotary: Rotary, positions=None):

@@ -508,6 +508,39 @@ def test_empty_calls():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_refusals_on_the_gpu(bits):
+    """Arguments that do not fit are refused before a launch; the cache stays."""
+    pool, *_ = _filled([20, 5], 16, 2, 64, F16, bits)
+    c, table, n = pool.cache, pool.table_dev, pool.lengths
+    q, k = torch.zeros((2, 3, 4, 64), dtype=F16, device=DEV), torch.zeros((2, 3, 2, 64), dtype=F16, device=DEV)
+    rot, cpu = Rotary.build(64, device=DEV), torch.zeros(2, dtype=torch.int32)
+    before = c.k_pages.clone()
+    for bad in (lambda: flash_attn_decode(q[:, :, :3], c, table, n), lambda: flash_attn_decode(q[0], c, table, n),
+                lambda: flash_attn_decode(q[..., :32], c, table, n), lambda: flash_attn_decode(q.cpu(), c, table, n),
+                lambda: flash_attn_decode(q.bfloat16(), c, table, n), lambda: flash_attn_decode(q[:1], c, table, n),
+                lambda: flash_attn_decode(q, c, table.long(), n), lambda: flash_attn_decode(q, c, table[0], n),
+                lambda: flash_attn_decode(q, c, table[:, :0], n), lambda: flash_attn_decode(q, c, table, n.long()),
+                lambda: flash_attn_decode(q, c, table, cpu), lambda: flash_attn_decode(q, c, table, n, starts=n[:1]),
+                lambda: kv_cache_append(c, k[:, :, :1], k[:, :, :1], table, n),
+                lambda: kv_cache_append(c, k, k[:, :2], table, n), lambda: kv_cache_append(c, k, k.float(), table, n),
+                lambda: kv_cache_append(c, k.bfloat16(), k.bfloat16(), table, n),
+                lambda: kv_cache_append(c, k, k, table, n, n[:1]), lambda: kv_cache_append(c, k, k, table[:1], n),
+                lambda: kv_cache_append(c, k, k, table, n, q=q[:, :2]), lambda: kv_cache_append(c, k, k.cpu(), table, n),
+                lambda: kv_cache_append(c, k, k, table, n, rotary=Rotary.build(66, device=DEV)),
+                lambda: kv_cache_append(c, k, k, table, n, rotary=Rotary.build(64, device="cpu")),
+                lambda: kv_cache_read(c, table, n.long()), lambda: kv_cache_read(c, table[:1], n),
+                lambda: kv_cache_read(c, table, cpu)):
+        with pytest.raises(AssertionError):
+            bad()
+    torch.cuda.synchronize(DEV)
+    check_status(DEV)
+    assert torch.equal(c.k_pages.view(torch.uint8), before.view(torch.uint8))
+    assert flash_attn_decode(q, c, table, n).shape == q.shape  # and the right call works
+    assert kv_cache_append(c, k, k, table, _ints([0, 0]), q=q, rotary=rot).shape == q.shape
+
+
+@pytest.mark.gpu
 def test_gradients_are_refused():
     pool, *_ = _filled([5], 16, 2, 64, F16, 16)
     q = torch.zeros((1, 1, 2, 64), dtype=F16, device=DEV, requires_grad=True)

@@ -194,6 +194,21 @@ def test_strides(how, inter):
 
 
 @pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    x, f = torch.zeros((2, 3, 4, 64), dtype=torch.float16, device=DEV), _freq(64).to(DEV)
+    r, pos = Rotary(f), torch.zeros((2, 3), dtype=torch.int32, device=DEV)
+    for bad in (lambda: rotary_embed(x.float(), r), lambda: rotary_embed(x[0], r),
+                lambda: rotary_embed(x[..., :32], r), lambda: rotary_embed(x[..., :63], r),
+                lambda: rotary_embed(x, Rotary(f.cpu())), lambda: rotary_embed(x.cpu(), r),
+                lambda: rotary_embed(x, r, pos.float()), lambda: rotary_embed(x, r, pos[:, :2]),
+                lambda: rotary_embed(x, r, pos.cpu()), lambda: rotary_embed_qk(x, x[:, :2], r),
+                lambda: rotary_embed_qk(x, x.bfloat16(), r), lambda: rotary_embed_qk(x, x.cpu(), r)):
+        with pytest.raises(AssertionError):
+            bad()
+    torch.cuda.synchronize(DEV)
+
+
+@pytest.mark.gpu
 def test_empty():
     rot = Rotary(_freq(64).to(DEV))
     for shape in ((0, 3, 2, 64), (2, 0, 2, 64), (2, 3, 0, 64)):

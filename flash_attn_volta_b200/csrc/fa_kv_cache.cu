@@ -131,11 +131,23 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                     Elem<T>::pack2(x[4], x[5]), Elem<T>::pack2(x[6], x[7]));
 }
 
+// a c - b s and a c + b s of one rotated dim.  For 4 bits each product and the
+// sum are rounded to fp32 apart, as the formula reads, so that the value that
+// is rounded to a code does not depend on what is fused.
+template <int BITS>
+__device__ __forceinline__ float turn(float a, float c, float b, float s) {
+  return BITS == 4 ? __fadd_rn(__fmul_rn(a, c), __fmul_rn(b, s)) : a * c + b * s;
+}
+template <int BITS>
+__device__ __forceinline__ float2 angle(double pos, double inv_freq, float magnitude) {
+  return BITS == 4 ? rotary_cos_sin_exact(pos, inv_freq, magnitude) : rotary_cos_sin(pos, inv_freq, magnitude);
+}
+
 // Rotates the 8 dims e.. of a row whose own values are x.  WIDE: the thread's
 // angles stand `stride` apart from `w` on (neighbouring lanes read neighbouring
 // words) and the partner dims' values are y, negated in the first halves.
 // Otherwise `w` holds the angles in order and partner dims are read from `row`.
-template <bool INTER>
+template <bool INTER, int BITS>
 __device__ __forceinline__ void rotate_wide(const float2* w, int stride, float (&x)[8],
                                             const float (&y)[8]) {
   if constexpr (INTER) {
@@ -143,18 +155,18 @@ __device__ __forceinline__ void rotate_wide(const float2* w, int stride, float (
     for (int i = 0; i < 8; i += 2) {
       const float2 c = w[i / 2 * stride];
       const float a = x[i], b = x[i + 1];
-      x[i] = a * c.x - b * c.y;
-      x[i + 1] = b * c.x + a * c.y;
+      x[i] = turn<BITS>(a, c.x, -b, c.y);
+      x[i + 1] = turn<BITS>(b, c.x, a, c.y);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 c = w[i * stride];
-      x[i] = x[i] * c.x + y[i] * c.y;
+      x[i] = turn<BITS>(x[i], c.x, y[i], c.y);
     }
   }
 }
-template <typename T, bool INTER>
+template <typename T, bool INTER, int BITS>
 __device__ __forceinline__ void rotate_any(const uint16_t* row, int e, int half, const float2* w,
                                            float (&x)[8]) {
 #pragma unroll
@@ -165,13 +177,13 @@ __device__ __forceinline__ void rotate_any(const uint16_t* row, int e, int half,
       if (i % 2) continue;
       const float2 c = w[d / 2];
       const float a = x[i], b = x[i + 1];
-      x[i] = a * c.x - b * c.y;
-      x[i + 1] = b * c.x + a * c.y;
+      x[i] = turn<BITS>(a, c.x, -b, c.y);
+      x[i + 1] = turn<BITS>(b, c.x, a, c.y);
     } else {
       const bool first = d < half;
       const float2 c = w[first ? d : d - half];
       const float y = Elem<T>::value(row[first ? d + half : d - half]);
-      x[i] = x[i] * c.x + (first ? -y : y) * c.y;
+      x[i] = turn<BITS>(x[i], c.x, first ? -y : y, c.y);
     }
   }
 }
@@ -281,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
       for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
         const int tok = i / p.half, f = i - tok * p.half;
         cs[tok * p.half + (WIDE ? f % N * (p.half / N) + f / N : f)] =
-            rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
+            angle<BITS>((double)(first + tok), p.inv_freq[f], p.magnitude);
       }
       __syncthreads();
     }
@@ -305,13 +317,13 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
             float y[8];
             const bool lower = e < p.half;
             if (!INTER) unpack8<T>(other[u], y, lower ? 0x80008000u : 0u);
-            rotate_wide<INTER>(w + (INTER || lower ? c : c - p.half / 8), p.half / (INTER ? 4 : 8), x, y);
+            rotate_wide<INTER, BITS>(w + (INTER || lower ? c : c - p.half / 8), p.half / (INTER ? 4 : 8), x, y);
           }
         } else {
           const uint16_t* raw = reinterpret_cast<const uint16_t*>(at[u]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) x[k] = Elem<T>::value(raw[e + k]);
-          if (turns) rotate_any<T, INTER>(raw, e, p.half, w, x);
+          if (turns) rotate_any<T, INTER, BITS>(raw, e, p.half, w, x);
         }
         if (part == 0) *reinterpret_cast<uint4*>(q_out + (long long)i * 8) = pack8<T>(x);
       }
@@ -384,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_stream_kernel(const 
         if (PART < 2 && turning) {
           float y[8];
           if (!INTER) unpack8<T>(ring[(stage * LOADS + 1) * kThreads], y, signs);
-          rotate_wide<INTER>(angles + tok * p.half, p.half / N, x, y);
+          rotate_wide<INTER, BITS>(angles + tok * p.half, p.half / N, x, y);
         }
       }
       if (PART == 0)
@@ -405,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_stream_kernel(const 
     for (int i = threadIdx.x; i < ntok * p.half; i += kThreads) {
       const int tok = i / p.half, f = i - tok * p.half;
       cs[tok * p.half + f % N * (p.half / N) + f / N] =
-          rotary_cos_sin((double)(first + tok), p.inv_freq[f], p.magnitude);
+          angle<BITS>((double)(first + tok), p.inv_freq[f], p.magnitude);
     }
     __syncthreads();
   });

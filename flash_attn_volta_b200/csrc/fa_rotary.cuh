@@ -25,6 +25,17 @@ __device__ __forceinline__ float2 rotary_cos_sin(double pos, double inv_freq, fl
   return make_float2(magnitude * fmaf(-d, s, c), magnitude * fmaf(d, c, s));
 }
 
+// The same with the sine and cosine in 64 bits, each rounded to fp32 once: for
+// keys that are then rounded to 4 bits, where the last bit of a value next to the
+// border of two codes decides between values a whole step apart (28.1 against
+// 27.4 us for 4 x 1024 tokens of 32 + 2 x 8 heads of 128).
+__device__ __forceinline__ float2 rotary_cos_sin_exact(double pos, double inv_freq, float magnitude) {
+  const double t = pos * inv_freq * 0.15915494309189533577;  // 1 / (2 pi)
+  double s, c;
+  sincospi(2.0 * (t - rint(t)), &s, &c);
+  return make_float2(magnitude * (float)c, magnitude * (float)s);
+}
+
 // N consecutive 16-bit elements as one load or store.
 template <int N>
 struct alignas(2 * N) Pack16 {

@@ -266,7 +266,7 @@ __device__ __forceinline__ Shares locate(const DecodeParams& p, int segs, unsign
 template <int D>
 __device__ __forceinline__ void write_row(const DecodeParams& p, int b, int h, int rr, int d,
                                           float top, float sum, const float (&x)[8]) {
-  const int qpos = rr / p.group, hq = h * p.group + (rr - qpos * p.group);
+  const int qpos = (int)p.group_div.div(rr), hq = h * p.group + (rr - qpos * p.group);
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
   uint32_t w[4];
 #pragma unroll
@@ -493,16 +493,15 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           const uint32_t w = raw[n][2 * grp + i / 2][i % 2];
           return p.bf16 ? Elem<__nv_bfloat16>::unpack2(w) : Elem<__half>::unpack2(w);
         };
-        float top = 0.f;
+        uint32_t most = 0;  // largest magnitudes of the even and odd dims, as 16-bit patterns
 #pragma unroll
-        for (int grp = 0; grp < NG; ++grp)
+        for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = pair(grp, i);
-            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          for (int i = 0; i < 2; ++i) most = __vmaxu2(most, raw[n][k][i] & 0x7FFF7FFFu);
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const uint32_t one = max(most & 0xFFFFu, most >> 16);
+        const float top = p.bf16 ? Elem<__nv_bfloat16>::value((uint16_t)one) : Elem<__half>::value((uint16_t)one);
         int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
         e = max(-90, min(e, 110));
         const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
@@ -515,11 +514,11 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = pair(grp, i);
-            const uint32_t h2 = Elem<__half>::pack2(v.x * turn, v.y * turn);
-            const float2 r = Elem<__half>::unpack2(h2);
-            sum += r.x + r.y;
+            const float x = v.x * turn, y = v.y * turn;
+            sum += x + y;
             // codes of the first two dims of four stand 4 bits lower: their q is 2^4 larger
-            qf[n][2 * grp + i / 2][i % 2] = i % 2 ? h2 : Elem<__half>::pack2(r.x * 16.f, r.y * 16.f);
+            const uint32_t h2 = Elem<__half>::pack2(x, y);
+            qf[n][2 * grp + i / 2][i % 2] = i % 2 ? h2 : hmul2(h2, 0x4C004C00u);  // x 16
           }
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -756,14 +755,15 @@ __global__ void __launch_bounds__(kThreads, kCtas)
               sc[0] &= keep0;
               sc[1] &= keep1;
             }
-            const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
+            // rows e0 and e2 take the whole byte (16 c1 + c0), rows e1 and e3 its upper
+            // nibble; their difference is taken once, at the segment's end
+            const uint32_t y0 = w0[grp] & 0x00FF00FFu, y1 = w1[grp] & 0x00FF00FFu;
+            const uint32_t x0 = __byte_perm(w0[grp], 0, 0x4341), x1 = __byte_perm(w1[grp], 0, 0x4341);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t b0 = hmul2(pf[n][0], sc[0]), b1 = hmul2(pf[n][1], sc[1]);
-              add(o[2 * grp][n], n, w0[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
-                  w1[grp] & 0x000F000Fu, w1[grp] & 0x00F000F0u, b0, b1);
-              add(o[2 * grp + 1][n], n, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
-                  x1 & 0x00F000F0u, b0, b1);
+              add(o[2 * grp][n], n, y0, w0[grp] & 0x00F000F0u, y1, w1[grp] & 0x00F000F0u, b0, b1);
+              add(o[2 * grp + 1][n], n, x0, x0 & 0x00F000F0u, x1, x1 & 0x00F000F0u, b0, b1);
             }
           }
         }
@@ -796,8 +796,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           for (int grp = 0; grp < NG; ++grp) {
             const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t);
             *reinterpret_cast<float4*>(dst + 32 * grp + 4 * g) =
-                make_float4(fmaf(o[2 * grp][n][i], 0x1p24f, mm), fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
-                            fmaf(o[2 * grp + 1][n][i], 0x1p24f, mm),
+                make_float4(fmaf(o[2 * grp][n][i] - o[2 * grp][n][i + 2], 0x1p24f, mm),
+                            fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
+                            fmaf(o[2 * grp + 1][n][i] - o[2 * grp + 1][n][i + 2], 0x1p24f, mm),
                             fmaf(o[2 * grp + 1][n][i + 2], 0x1p20f, mm));
           }
         }
@@ -900,11 +901,30 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, s >= stage ? phase : phase ^ 1u, p.timeout_ns);
 }
 
+// Running join of partial results: 8 dims of a row.
+struct RowSum {
+  float top = -INFINITY, sum = 0.f, x[8] = {};
+  __device__ __forceinline__ void add(float2 ml, float4 u, float4 v) {
+    const float now = fmaxf(top, ml.x);
+    const float safe = now == -INFINITY ? 0.f : now;
+    const float old = ex2(top - safe), e = ex2(ml.x - safe);
+    const float y[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    top = now;
+    sum = fmaf(e, ml.y, sum * old);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = fmaf(e, y[j], x[j] * old);
+  }
+  __device__ __forceinline__ void take(const DecodeParams& p, long long slot, int D, int d) {
+    const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
+    add(p.part_ml[slot], src[0], src[1]);
+  }
+};
+
 // Joins the partial results of the segments that cross shares, in the order of
 // the shares.  blockIdx.x is a border between two shares; the border that a
-// segment crosses first does its work, two rows to a CTA (blockIdx.y).  A thread
-// holds 8 dims of a row and takes every P-th share, all loads independent;
-// blockIdx.y takes every gridDim.y-th pair of rows.
+// segment crosses first does its work.  With many shares to a segment a CTA takes
+// two rows (blockIdx.y) and a thread, which holds 8 dims, every P-th share, so
+// that all loads are in flight at once.
 template <int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeParams p) {
   using C = Cfg<D, BITS, NT>;
@@ -926,41 +946,32 @@ __global__ void __launch_bounds__(kThreads) fa_decode_merge_kernel(const DecodeP
   griddep_launch_dependents();
   if (!crossed) return;
   const int h = (int)p.rb_div.div(hr), rb = (int)hr - h * p.row_blocks, rows = p.Sq * p.group;
+  if (gridDim.y == 1) {
+    // few shares to a segment: a thread takes all of them for its 8 dims
+    for (int i = threadIdx.x; i < min(rows - rb * ROWS, ROWS) * PER_ROW; i += kThreads) {
+      const int r = i / PER_ROW, d = i % PER_ROW * 8;
+      RowSum sum;
+#pragma unroll 4
+      for (int c = c0; c <= c1; ++c)
+        sum.take(p, (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r, D, d);
+      write_row<D>(p, b, h, rb * ROWS + r, d, sum.top, sum.sum, sum.x);
+    }
+    return;
+  }
   const int half = threadIdx.x / (kThreads / 2), i = threadIdx.x % (kThreads / 2);
   const int pg = i / PER_ROW, d = i % PER_ROW * 8;
-  for (int pair = blockIdx.y; pair < ROWS / 2; pair += gridDim.y) {
-    const int r = pair * 2 + half, rr = rb * ROWS + r;
-    float top = -INFINITY, sum = 0.f, x[8] = {};
-    auto take = [&](float2 ml, const float (&v)[8]) {
-      const float now = fmaxf(top, ml.x);
-      const float safe = now == -INFINITY ? 0.f : now;
-      const float old = ex2(top - safe), e = ex2(ml.x - safe);
-      top = now;
-      sum = fmaf(e, ml.y, sum * old);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = fmaf(e, v[j], x[j] * old);
-    };
+  const int r = blockIdx.y * 2 + half, rr = rb * ROWS + r;
+  RowSum sum;
 #pragma unroll 4
-    for (int c = c0 + pg; c <= c1; c += P) {
-      const long long slot = (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r;
-      const float4* src = reinterpret_cast<const float4*>(p.part_o + slot * D + d);
-      const float4 u = src[0], v = src[1];
-      take(p.part_ml[slot], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
-    }
-    part_x[half][pg][d / 4] = make_float4(x[0], x[1], x[2], x[3]);
-    part_x[half][pg][d / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
-    if (d == 0) part_ml[half][pg] = make_float2(top, sum);
-    __syncthreads();
-    if (pg == 0 && rr < rows) {
+  for (int c = c0 + pg; c <= c1; c += P) sum.take(p, (2LL * c + (c == c0 ? 1 : 0)) * ROWS + r, D, d);
+  part_x[half][pg][d / 4] = make_float4(sum.x[0], sum.x[1], sum.x[2], sum.x[3]);
+  part_x[half][pg][d / 4 + 1] = make_float4(sum.x[4], sum.x[5], sum.x[6], sum.x[7]);
+  if (d == 0) part_ml[half][pg] = make_float2(sum.top, sum.sum);
+  __syncthreads();
+  if (pg != 0 || rr >= rows) return;
 #pragma unroll
-      for (int k = 1; k < P; ++k) {
-        const float4 u = part_x[half][k][d / 4], v = part_x[half][k][d / 4 + 1];
-        take(part_ml[half][k], {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w});
-      }
-      write_row<D>(p, b, h, rr, d, top, sum, x);
-    }
-    __syncthreads();
-  }
+  for (int k = 1; k < P; ++k) sum.add(part_ml[half][k], part_x[half][k][d / 4], part_x[half][k][d / 4 + 1]);
+  write_row<D>(p, b, h, rr, d, sum.top, sum.sum, sum.x);
 }
 
 template <typename T, int D, int BITS, int NT>
@@ -974,9 +985,10 @@ int launch_decode(DecodeParams& p, const CUtensorMap& tk, const CUtensorMap& tv,
   if (launch_pdl(kernel, dim3(p.grid_div.d), dim3(kThreads), C::kSmem, st, p, tk, tv) != cudaSuccess)
     return FA_ERR_LAUNCH;
   if (!split) return FA_OK;
-  // Many shares to a segment (few segments): its rows are spread over CTAs, too.
+  // Many shares to a segment (few segments): its rows are spread over CTAs, too
+  // (with two or three shares that takes 3.5 us of dependent steps, this way 1.5).
   const long long segs = (long long)p.B * p.kv.heads * p.row_blocks;
-  const unsigned y = p.grid_div.d > 8 * segs ? 4 * NT : NT;
+  const unsigned y = p.grid_div.d > 4 * segs ? 4 * NT : 1;
   return launch_pdl(fa_decode_merge_kernel<D, BITS, NT>, dim3(p.grid_div.d - 1, y), dim3(kThreads), 0, st,
                     p) == cudaSuccess
              ? FA_OK

@@ -1030,8 +1030,12 @@ int launch_decode_any(DecodeParams& p, int nt, const CUtensorMap& tk, const CUte
   }
 }
 
-// Tokens up to which a segment is not split.
-constexpr int kWholeTokens = 1024;
+// Tiles (of the table's room) up to which segments are not split, so that no second
+// launch joins them.  Replayed, whole against split, us: 16-bit, 16 heads of 64,
+// 300 tokens (3 tiles) 5.6 / 7.0, 777 (7) 9.1 / 7.2, where the second launch costs
+// the host 2.5 us more, 2000 (16) 16.5 / 8.0; 4-bit, 8 heads of 128, 1000 tokens (4)
+// 11.1 / 11.3, of 16 sequences 11.9 / 14.8, 2000 (8) 16.4 / 11.5.
+constexpr int whole_tiles(int bits) { return bits == 4 ? 4 : 7; }
 // Places are counted in 31 bits.
 constexpr long long kMaxPlaces = 1LL << 31;
 
@@ -1054,7 +1058,7 @@ Plan plan_of(const fa_sm100_kv_cache* c, int table_width, int batch, int seqlen,
   const long long segs = (long long)batch * c->nheads_kv * pl.row_blocks, tiles = segs * per_seg;
   const long long most = (long long)sm_count() * kCtas;
   pl.places = segs * (per_seg + cost_of(c->head_dim, c->bits, pl.nt));
-  pl.split = (long long)table_width * c->page_size > kWholeTokens;
+  pl.split = per_seg > whole_tiles(c->bits);
   const long long grid = pl.split ? tiles : segs;
   pl.grid = (int)(grid < most ? grid : most);
   if (pl.grid == 1) pl.split = false;

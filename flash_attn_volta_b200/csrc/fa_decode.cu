@@ -24,11 +24,27 @@
 //   operand by one 8x8 transpose (movmatrix) each.
 // * 4-bit codes are used as they are: a nibble masked out of its word is the
 //   fp16 subnormal c 2^-24 (bits 0..3) or c 2^-20 (bits 4..7), exact in the
-//   matrix instruction, so 8 codes cost one shift and four ANDs.  The power of
-//   two goes into q (K) or the final factor (V).  Scales and minima enter
+//   matrix instruction, so 8 codes cost one shift and four ANDs (the integer pipe
+//   is the busiest: 44 % at 2 x 131072 tokens).  The power of two goes into q (K) or
+//   the final factor (V).  Summing V's even dims as whole bytes 16 c1 + c0 and parting
+//   them at the end saves an AND in five and 5 % of the time, but the matrix
+//   instruction's sums are truncated, and 16 c1 is 17 times the sum that is wanted:
+//   the error against 64 bits grew from 2.1e-4 to 2.6e-4 there.  Scales and minima enter
 //   outside: S = sum_g s_g (c_g . q_g) + m_g sum(q_g), with the second sum as
 //   one more matrix instruction on the parameter words themselves (q's group
 //   sums as an fp16 head and tail), and O = sum_t (p_t s_t) c_t + p_t m_t.
+//
+// Rounded to fewer than 32 bits: p to the operand type (fp16 at 4 bits, where it is
+// then multiplied by its token's scale in fp16), q to fp16 at 4 bits after a
+// power of two per row (exact but for elements below 2^-24 of the largest).
+//
+// Measured on one B200 (replayed): 64 sequences of 5 to 8192 tokens, 32 / 8 heads of
+// 128, 16-bit 172 us (6.2 TB/s of the cache), 96 such at 4 bits 98 us (5.2 TB/s); two
+// of 100003 and 131072 tokens at 4 bits 57 us, of which 46 stream at 6.4 TB/s and 11
+// are fixed: lengths, pages and the first copy follow one another (5 us), and the
+// last tile, the join of the warps and the second launch (6 us).  One CTA holds 4
+// warps, two an SM: 12 or 16 warps an SM with 2 blocks a tile were slower (69 and 76
+// against 64 us for the two long ones), as a tile's fixed steps then count twice.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -755,15 +771,14 @@ __global__ void __launch_bounds__(kThreads, kCtas)
               sc[0] &= keep0;
               sc[1] &= keep1;
             }
-            // rows e0 and e2 take the whole byte (16 c1 + c0), rows e1 and e3 its upper
-            // nibble; their difference is taken once, at the segment's end
-            const uint32_t y0 = w0[grp] & 0x00FF00FFu, y1 = w1[grp] & 0x00FF00FFu;
-            const uint32_t x0 = __byte_perm(w0[grp], 0, 0x4341), x1 = __byte_perm(w1[grp], 0, 0x4341);
+            const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint32_t b0 = hmul2(pf[n][0], sc[0]), b1 = hmul2(pf[n][1], sc[1]);
-              add(o[2 * grp][n], n, y0, w0[grp] & 0x00F000F0u, y1, w1[grp] & 0x00F000F0u, b0, b1);
-              add(o[2 * grp + 1][n], n, x0, x0 & 0x00F000F0u, x1, x1 & 0x00F000F0u, b0, b1);
+              add(o[2 * grp][n], n, w0[grp] & 0x000F000Fu, w0[grp] & 0x00F000F0u,
+                  w1[grp] & 0x000F000Fu, w1[grp] & 0x00F000F0u, b0, b1);
+              add(o[2 * grp + 1][n], n, x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu,
+                  x1 & 0x00F000F0u, b0, b1);
             }
           }
         }
@@ -796,9 +811,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           for (int grp = 0; grp < NG; ++grp) {
             const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t);
             *reinterpret_cast<float4*>(dst + 32 * grp + 4 * g) =
-                make_float4(fmaf(o[2 * grp][n][i] - o[2 * grp][n][i + 2], 0x1p24f, mm),
-                            fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
-                            fmaf(o[2 * grp + 1][n][i] - o[2 * grp + 1][n][i + 2], 0x1p24f, mm),
+                make_float4(fmaf(o[2 * grp][n][i], 0x1p24f, mm), fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
+                            fmaf(o[2 * grp + 1][n][i], 0x1p24f, mm),
                             fmaf(o[2 * grp + 1][n][i + 2], 0x1p20f, mm));
           }
         }
@@ -898,7 +912,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   }
   // After a wait that ran out, copies may still be under way into this CTA's memory.
   for (int s = 0; s < NS; ++s)
-    if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, s >= stage ? phase : phase ^ 1u, p.timeout_ns);
+    if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, s >= stage ? phase : phase ^ 1u, max(p.timeout_ns, 1000000000ull));
 }
 
 // Running join of partial results: 8 dims of a row.

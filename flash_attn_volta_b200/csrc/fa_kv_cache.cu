@@ -240,7 +240,8 @@ __device__ __forceinline__ void store_item(const AppendParams& p, int part, int 
 // 32, so a warp works on one of them, and the 4 lanes that hold a group of 32
 // dims reduce its minimum and maximum by shuffles.
 // WIDE: 16-byte loads at 32-bit offsets, and rotated dims that end at an item's
-// border.
+// border.  One token of each of 64 sequences takes the host longer (7 us) than
+// the device.
 template <typename T, bool INTER, int BITS, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendParams p) {
   extern __shared__ float2 cs[];
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
   int* places = reinterpret_cast<int*>(cs + p.per_cta * p.half);  // row of head 0, or -1
   const int hk = kv.heads;
   const long long first = (long long)p.starts[b] + s0;
-  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, p.counts[b] - s0));  // tokens to store
+  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, max(p.counts[b], 0) - s0));  // tokens to store
   const int nq = (ntok * (int)p.q_heads.d) << p.chunk_shift, nk = (fresh * hk) << p.chunk_shift;
   const int k0 = (nq + 31) & ~31, v0 = k0 + ((nk + 31) & ~31), end = v0 + ((nk + 31) & ~31);
   for (int i = threadIdx.x; i < fresh; i += kThreads) {
@@ -336,7 +337,11 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_kernel(const AppendP
 // The same for prompts: a CTA takes so many tokens that the grid is few waves, and
 // each thread streams its vectors through a ring of its own in shared memory.
 // The rows are the heads of q, then of k, then of v of the CTA's tokens; a thread
-// keeps its dims of a row.
+// keeps its dims of a row.  Measured on one B200: 6 prompts of up to 4096 tokens, 3 x 16
+// heads of 64, fp16 44 us, against 89 with the kernel above (its issue slots were 78 %
+// busy with each token's set-up) and 35 that its reads and writes (q of the padding
+// rows among them) take at the copy rate; 4 x 1024 tokens of 32 + 2 x 8 heads of 128 into
+// 4 bits 28 us, issue-bound (rounding to codes).
 constexpr int kStreamStages = 4;
 
 template <typename T, bool INTER, int BITS>
@@ -352,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 4) fa_kv_append_stream_kernel(const 
   const int b = p.per_seq.div(blockIdx.x), s0 = (blockIdx.x - b * p.per_seq.d) * p.per_cta;
   const int ntok = min(p.per_cta, p.S - s0), hk = kv.heads;
   const long long first = (long long)p.starts[b] + s0;
-  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, p.counts[b] - s0));
+  const int fresh = p.counts == nullptr ? ntok : max(0, min(ntok, max(p.counts[b], 0) - s0));
   const int c = threadIdx.x & ((1 << p.chunk_shift) - 1), e = c * 8;
   const int step = kThreads >> p.chunk_shift, whole = (32 >> p.chunk_shift) - 1;  // rows of a warp - 1
   const int nq = ntok * (int)p.q_heads.d, nk = fresh * hk;
@@ -496,7 +501,8 @@ __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N])
 // once.  4-bit: lane (g, t) = (lane / 4, lane % 4) reads the words that it
 // would read in the attention kernel, each once: 8 dims of each group of tokens
 // g and g + 8 (K), 4 dims of each group of tokens 2 t, 2 t + 1 and the two 8
-// further (V); a store instruction writes whole 32-byte sectors.
+// further (V); a store instruction writes whole 32-byte sectors.  Measured on one
+// B200: 12 sequences of 33 to 6001 tokens, 8 heads of 64, 4-bit 27 us (6.3 TB/s).
 template <typename T, int D, int BITS>
 __global__ void __launch_bounds__(kThreads) fa_kv_read_kernel(const ReadParams p) {
   griddep_wait();
@@ -675,6 +681,7 @@ extern "C" int fa_sm100_kv_append(const fa_sm100_kv_cache* cache, const fa_sm100
                          reinterpret_cast<uintptr_t>(counts);
   if ((ints & 3u) || (reinterpret_cast<uintptr_t>(inv_freq) & 7u)) return FA_ERR_ARG;
   if (inv_freq && (rotary_dim < 2 || rotary_dim % 2 || rotary_dim > cache->head_dim)) return FA_ERR_ARG;
+  if ((rc = bind_device()) != FA_OK) return rc;
   AppendParams p = {};
   p.kv = kv_view(cache, page_table, table_width, status);
   if (q) p.part[0] = {q->in, q->stride_batch, q->stride_seq, q->stride_head, q->heads};
@@ -738,6 +745,7 @@ extern "C" int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
     return FA_ERR_ARG;
   if ((long long)cache->nheads_kv * cache->head_dim > (1 << 20)) return FA_ERR_ARG;
+  if ((rc = bind_device()) != FA_OK) return rc;
   ReadParams p;
   p.kv = kv_view(cache, page_table, table_width, status);
   p.lengths = lengths;

@@ -39,12 +39,13 @@
 // power of two per row (exact but for elements below 2^-24 of the largest).
 //
 // Measured on one B200 (replayed): 64 sequences of 5 to 8192 tokens, 32 / 8 heads of
-// 128, 16-bit 172 us (6.2 TB/s of the cache), 96 such at 4 bits 98 us (5.2 TB/s); two
-// of 100003 and 131072 tokens at 4 bits 57 us, of which 46 stream at 6.4 TB/s and 11
-// are fixed: lengths, pages and the first copy follow one another (5 us), and the
-// last tile, the join of the warps and the second launch (6 us).  One CTA holds 4
-// warps, two an SM: 12 or 16 warps an SM with 2 blocks a tile were slower (69 and 76
-// against 64 us for the two long ones), as a tile's fixed steps then count twice.
+// 128, 16-bit 172 to 177 us (6.1 TB/s of the cache), 96 such at 4 bits 103 us
+// (4.9 TB/s); two of 100003 and 131072 tokens at 4 bits 60 us, of which 49 stream at
+// 6 TB/s and 11 are fixed: lengths, pages and the first copy follow one another
+// (5 us), and the last tile, the join of the warps and the second launch (6 us).
+// A CTA holds 4 warps, an SM two CTAs: 12 or 16 warps an SM with 2 blocks a tile were
+// slower (69 and 76 against 64 us for the two long ones), as a tile's fixed steps
+// then count twice.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -85,7 +85,7 @@ def block_bytes(kc, km, ks, vc, vm, vs):
 def decode(q, k, v, sizes, limits, scale):
     """q (R, D) query rows, k, v (n, D) and |v|'s bound `sizes` (n, D) in float64;
     row r sees keys j < limits[r].  Returns out (R, D), lse (R,), and per row
-    sum_j p_j sizes_j (R, D) and max_j scale sum_d |q_d k_jd|."""
+    sum_j p_j sizes_j (R, D) and max_j |scale| sum_d |q_d k_jd|."""
     R, D = q.shape
     out, lse = torch.zeros(R, D, dtype=torch.float64), torch.full((R,), math.inf, dtype=torch.float64)
     mass, reach = torch.zeros(R, D, dtype=torch.float64), torch.zeros(R, dtype=torch.float64)
@@ -97,5 +97,5 @@ def decode(q, k, v, sizes, limits, scale):
         lse[r] = torch.logsumexp(sc, 0)
         p = torch.softmax(sc, 0)
         out[r], mass[r] = p @ v[:n], p @ sizes[:n]
-        reach[r] = ((k[:n].abs() @ q[r].abs()) * scale).max()
+        reach[r] = ((k[:n].abs() @ q[r].abs()) * abs(scale)).max()
     return out, lse, mass, reach

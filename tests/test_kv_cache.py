@@ -671,6 +671,51 @@ def test_shared_pages():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits,pages", [(16, 40000), (4, 60000)])
+def test_offsets_beyond_32_bits(bits, pages):
+    """Pages at the end of a cache whose byte offsets (and elements) pass 2^32."""
+    cache = PagedKVCache.allocate(pages, 64, 8, 128, BF16, bits, DEV)
+    assert cache.k_pages.numel() * cache.k_pages.element_size() > 2 ** 32
+    k, v = _kv(1, 100, 8, 128, BF16, 3)
+    table = _ints([[pages - 1, pages - 2]])
+    kv_cache_append(cache, k.to(DEV), v.to(DEV), table, _ints([0]))
+    ko, vo = kv_cache_read(cache, table, _ints([100]), 100)
+    q = torch.randn((1, 1, 16, 128), generator=torch.Generator().manual_seed(8)).bfloat16()
+    out = flash_attn_decode(q.to(DEV), cache, table, _ints([100]))
+    check_status(DEV)
+    if bits == 16:
+        assert torch.equal(ko.cpu(), k) and torch.equal(vo.cpu(), v)
+        _check_decode(q, out, None, k.double(), v.double(), v.double().abs(), [100], None, True, 16)
+    else:
+        kc, km, ks = so.four_bit(k)
+        vc, vm, vs = so.four_bit(v)
+        _check_decode(q, out, None, so.values(kc, km, ks), so.values(vc, vm, vs),
+                      so.values(vc, vm.abs(), vs), [100], None, True, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits,S,H,Hkv,D", [(4, 1, 64, 1, 128), (16, 1, 64, 1, 64), (4, 1, 71, 1, 64),
+                                            (16, 150, 4, 4, 32), (4, 40, 6, 3, 128)])
+def test_many_query_rows(bits, S, H, Hkv, D):
+    """More rows than one pass holds: row blocks, the last one short."""
+    lengths = [200, 170]
+    pool, k, v, size = _filled(lengths, 64, Hkv, D, F16, bits, seed=5)
+    q = torch.randn((2, S, H, D), generator=torch.Generator().manual_seed(8)).half()
+    out, lse = flash_attn_decode(q.to(DEV), pool.cache, pool.table_dev, pool.lengths,
+                                 return_softmax_lse=True)
+    _check_decode(q, out, lse, k, v, size, lengths, None, True, bits)
+
+
+@pytest.mark.gpu
+def test_strided_queries_and_negative_scale():
+    pool, k, v, size = _filled([90], 16, 2, 64, BF16, 4, seed=5)
+    wide = torch.randn((1, 2, 12, 64), generator=torch.Generator().manual_seed(8)).bfloat16()
+    for scale in (-0.2, 0.0):
+        out = flash_attn_decode(wide.to(DEV)[:, :, 1:9], pool.cache, pool.table_dev, pool.lengths, sm_scale=scale)
+        _check_decode(wide[:, :, 1:9], out, None, k, v, size, [90], None, True, 4, scale)
+
+
+@pytest.mark.gpu
 def test_many_sequences():
     """More sequences than threads of a CTA (each CTA sums the lengths itself)."""
     lengths = [(37 * i) % 50 for i in range(301)]

@@ -157,6 +157,21 @@ def test_many_tokens(B, S, H, Hkv, D, R, inter, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("inter", [False, True])
+def test_more_than_2_31_elements(inter):
+    S = 540_000  # x 32 heads of 128: 2.2e9 elements
+    x = torch.zeros((1, S, 32, 128), dtype=torch.bfloat16, device=DEV)
+    at = [0, 1, 262_143, 262_144, 524_287, 524_288, S - 1]
+    x[:, at] = torch.randn((1, len(at), 32, 128), generator=torch.Generator().manual_seed(1)).bfloat16().to(DEV)
+    y = rotary_embed(x, Rotary(_freq(128).to(DEV), inter))
+    _check(y[:, at], x[:, at], torch.tensor(at), _freq(128), inter)
+    # the same rows, every other head of a tensor whose strides pass 31 bits within a call
+    z = rotary_embed(x.transpose(0, 1)[at, :, ::2].transpose(0, 1), Rotary(_freq(128).to(DEV), inter),
+                     torch.tensor(at, device=DEV))
+    assert torch.equal(z, y[:, at][:, :, ::2])
+
+
+@pytest.mark.gpu
 def test_far_positions():
     """Angles of 10^6 and 2^40 rad: an fp32 product would be off by 0.1 rad and more."""
     x = torch.randn((1, 4, 2, 64), generator=torch.Generator().manual_seed(3)).half()

@@ -133,6 +133,8 @@ int bind_device() { return check_device(); }
 
 unsigned long long wait_timeout_ns() { return g_timeout_ns.load(); }
 
+int debug_flags() { return g_debug_flags.load(); }
+
 int make_rows_map(CUtensorMap* m, const void* ptr, long long rows, int D, int box_rows, int dtype) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return FA_ERR_DEVICE;

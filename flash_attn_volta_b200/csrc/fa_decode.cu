@@ -124,6 +124,7 @@ struct DecodeParams {
   int negate;
   int whole;   // a share is whole segments: those that begin in it
   int direct;  // and CTA i's is segment i
+  int skip_copy;  // test hook: the first CTA's first block is not brought
   float scale_log2;  // |scale| log2 e, above 0; `negate`: the scale is negative (q's sign changes)
   unsigned long long timeout_ns;
 };
@@ -385,8 +386,10 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   Cursor pc = cur;
   int to_issue = left;
   auto more_to_issue = [&]() { return to_issue > 0 || (p.whole && pc.tt > 0); };
-  uint32_t ok_bits = 0;  // this lane's block of each stage holds tokens
+  constexpr uint32_t ALL = (1u << U) - 1u;
+  uint32_t ok_bits = 0;    // U bits for each stage: blocks that hold tokens
   uint32_t in_flight = 0;  // stages whose copies have not been waited for
+  uint32_t odd = ~0u;      // stages whose last copies complete an odd phase
   auto block_token = [&](const Cursor& c, int u) {
     return c.tt * C::kTile + (u * kWarps + warp) * kBlockTokens;  // a short tile's blocks go to all warps
   };
@@ -397,18 +400,19 @@ __global__ void __launch_bounds__(kThreads, kCtas)
                : -2;
   };
   auto issue = [&](int stage, int next_id) {
+    const bool ok = next_id != -2 && !p.kv.bad_page(next_id);
     if (lane < U) {
       const uint32_t bar = my_bars + stage * 8;
-      const bool ok = next_id != -2 && !p.kv.bad_page(next_id);
       if (next_id != -2 && !ok) p.kv.report(kStatusPage);
-      ok_bits = ok ? ok_bits | (1u << stage) : ok_bits & ~(1u << stage);
       if (ok) {
         // block (16-bit: row) of the cache, below 2^31
         const int at = (((next_id * p.kv.heads + pc.h) << p.page_shift) |
                         (block_token(pc, lane) & (p.kv.page - 1)));
         const uint32_t dst = my_ring + stage * C::kStageBytes + lane * C::kBlockBytes;
         mbar_arrive_expect_tx(bar, C::kBlockBytes);
-        if constexpr (BITS == 4) {
+        if (p.skip_copy && blockIdx.x == 0 && tid == 0 && to_issue == left) {
+          // the barrier waits for bytes that do not come
+        } else if constexpr (BITS == 4) {
           bulk_load(dst, p.kv.k + (long long)(at / kBlockTokens) * C::kBlockBytes, C::kBlockBytes, bar);
         } else {
 #pragma unroll
@@ -421,7 +425,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         mbar_arrive(bar);
       }
     }
+    ok_bits = (ok_bits & ~(ALL << stage * U)) | (__ballot_sync(0xffffffffu, ok) & ALL) << stage * U;
     in_flight |= 1u << stage;
+    odd ^= 1u << stage;
     to_issue -= advance(pc);
   };
 
@@ -887,11 +893,12 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     const int places = advance(next);
     const bool goes_on = left > places || (p.whole && !last);
     if (AHEAD && last && goes_on) load_q(next);
-    const bool here = mbar_wait(my_bars + stage * 8, phase, wait);
+    // a wait may run out for some lanes and end for others: the warp goes one way
+    const bool here = __all_sync(0xffffffffu, mbar_wait(my_bars + stage * 8, phase, wait));
     if (here) {
       in_flight &= ~(1u << stage);
-      const uint32_t ok = __ballot_sync(0xffffffffu, ok_bits >> stage & 1u) & ((1u << U) - 1u);
-      if (ok == (1u << U) - 1u && block_token(cur, U - 1) + kBlockTokens <= min_lim)
+      const uint32_t ok = ok_bits >> stage * U & ALL;
+      if (ok == ALL && block_token(cur, U - 1) + kBlockTokens <= min_lim)
         step(stage, ok, std::false_type{});
       else if (ok != 0)
         step(stage, ok, std::true_type{});
@@ -913,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   }
   // After a wait that ran out, copies may still be under way into this CTA's memory.
   for (int s = 0; s < NS; ++s)
-    if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, s >= stage ? phase : phase ^ 1u, max(p.timeout_ns, 1000000000ull));
+    if (in_flight >> s & 1u) mbar_wait_drain(my_bars + s * 8, odd >> s & 1u, max(p.timeout_ns, 1000000000ull));
 }
 
 // Running join of partial results: 8 dims of a row.
@@ -1156,6 +1163,7 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   p.negate = sm_scale < 0.f;
   p.bf16 = cache->dtype == FA_DTYPE_BF16;
   p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);
+  p.skip_copy = debug_flags() & 2;
   p.timeout_ns = wait_timeout_ns();
   return launch_decode_any(p, pl.nt, tk, tv, pl.split, static_cast<cudaStream_t>(stream));
 }

@@ -163,6 +163,8 @@ int bwd_q_rows(int D);
 int bind_device();
 // Limit of the on-device waits (fa_sm100_set_wait_timeout_ns).
 unsigned long long wait_timeout_ns();
+// Test hooks (fa_sm100_set_debug_flags).
+int debug_flags();
 // Tensor map over `rows` contiguous rows of D 16-bit elements, box_rows rows
 // and min(D, 64) elements to a box, swizzled by the box's row width.
 int make_rows_map(CUtensorMap* m, const void* ptr, long long rows, int D, int box_rows, int dtype);

@@ -674,8 +674,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)  // no token seen yet: every probability is 0
-        from[n][i] = EDGE && mf[n][i] == -INFINITY ? 0.f : mf[n][i];
+      for (int i = 0; i < 2; ++i)  // no score above -inf yet: every probability is 0
+        from[n][i] = fmaxf(mf[n][i], -3.4e38f);
     // ---- P^T, O^T += V^T P^T
 #pragma unroll
     for (int u = 0; u < U; ++u) {

@@ -66,6 +66,10 @@ constexpr int kThreads = kWarps * 32;
 // A maximum is left as it is while no score is more than 2^kSlack above it (the
 // probabilities then reach 4, and times a scale of at most 8734 stay in fp16).
 constexpr float kSlack = 2.f;
+// Probabilities are taken times 2^kLift where they become 16-bit fp16 operands: they
+// reach 2^14 and are normal numbers down to 2^-26 of the largest (unlifted, 2^-14: of
+// 70000 tokens 18 below one in score a fifth of their part of the output was lost).
+constexpr float kLift = 12.f;
 constexpr float kLn2 = 0.69314718055994531f;
 
 // Per-instantiation constants.
@@ -309,6 +313,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   using M = T;  // operand type
   constexpr int U = C::kU, NS = C::kStages, ROWS = 8 * NT, NG = BITS == 4 ? C::kGroups : 1;
   constexpr int KSTEPS = D / 16;
+  constexpr float LIFT = BITS == 16 && Elem<M>::kIdescAB == 0 ? kLift : 0.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   struct Misc {
     uint64_t bars[kWarps * NS];
@@ -439,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   int lim[NT][2];               // tokens that a column's query row sees
   int col_q[NT][2];             // query token of a column's row; -1: none
   float o[KSTEPS][NT][4], om[NT][4], l[NT][2];
-  float mf[NT][2];              // running maximum in the log2 domain
+  float mf[NT][2];              // running maximum in the log2 domain, less LIFT
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
 
   auto limit_of = [&](int qpos) {
@@ -648,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + kSlack;
+      for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + (LIFT + kSlack);
     if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -657,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
           for (int d = 4; d < 32; d *= 2)
             top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], d));
-          const float now = fmaxf(mf[n][i], top[n][i] * f[n][i]);
+          const float now = fmaxf(mf[n][i], top[n][i] * f[n][i] - LIFT);
           const float keep = now == -INFINITY ? 1.f : ex2(mf[n][i] - now);
           mf[n][i] = now;
           l[n][i] *= keep;

@@ -6,8 +6,9 @@ import pytest
 import torch
 
 from flash_attn_volta_b200 import _lib, check_status
-from flash_attn_volta_b200.kv_cache import flash_attn_decode
-from tests.test_kv_cache import BF16, DEV, F16, _check_decode, _filled
+from flash_attn_volta_b200.kv_cache import flash_attn_decode, kv_cache_append
+from oracle import serving_oracle as so
+from tests.test_kv_cache import BF16, DEV, F16, Pool, _check_decode, _filled, _ints
 
 
 # ---------------------------------------------------------------- GPU: waits
@@ -61,3 +62,59 @@ def test_scores_of_minus_infinity_weigh_nothing(n, D, dtype):
     _check_decode(q[:1], out[:1], lse[:1], k[:1, seen], v[:1, seen], size[:1, seen], [int(seen.sum())], None,
                   True, 16)
     assert not out[1].any() and bool((lse[1] == math.inf).all())
+
+
+# ---------------------------------------------------------------- GPU: weights far below the largest
+def _far(n, D, gap, bits, low, high, seed, order="even"):
+    """One sequence of n tokens, one head: the scores of tokens 0, 16, 32 and 48 (each warp has one)
+    are `gap` above the others' mean, which spread by about 1; values from `low` to `high`, those
+    four tokens' all `low`.  `order`: 'even', or values that grow or shrink 1000-fold along the
+    context."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn((1, 1, 1, D), generator=g).half()
+    k = torch.randn((1, n, 1, D), generator=g)
+    k[0, :64:16, 0] = q[0, 0, 0].float() * (gap * math.sqrt(D) / float(q.double().square().sum()))
+    v = low + (high - low) * torch.rand((1, n, 1, D), generator=g)
+    v[0, :64:16] = low
+    if order != "even":
+        size = torch.logspace(-3, 0, n) if order == "growing" else torch.logspace(0, -3, n)
+        v[0] = v[0] * size[:, None, None]
+        v[0, :64:16] = low
+    k, v = k.half(), v.half()
+    pool = Pool([n], 64, 1, D, F16, bits)
+    kv_cache_append(pool.cache, k.to(DEV), v.to(DEV), pool.table_dev, _ints([0]))
+    if bits == 16:
+        return pool, q, k.double(), v.double(), v.double().abs()
+    kc, km, ks = so.four_bit(k)
+    vc, vm, vs = so.four_bit(v)
+    return pool, q, so.values(kc, km, ks), so.values(vc, vm, vs), so.values(vc, vm.abs(), vs)
+
+
+def _check_far(pool, q, k, v, size, bits):
+    """As many sequences of the same pages as CTAs run at once, so that each is one CTA's work.
+    Held to relative errors alone.  A probability p, relative to a running maximum that is at
+    most 2 (in log2) too low, is brought to 2^12 p and rounded to fp16: half a step of 2^-11, or
+    2^-25 where it is subnormal, 2^-37 of p.  At 4 bits its product with the token's scale, taken
+    relative to the power of two below the largest scale s, is rounded once more in the same way.
+    With n tokens and a sum of at least 1 the subnormal part is below 3 n 2^-37 of the largest
+    value (15 s, or |v|).  The rest as in the other tests of the attention."""
+    n, D = k.shape[1], q.shape[3]
+    B = 2 * torch.cuda.get_device_properties(DEV).multi_processor_count
+    out, lse = flash_attn_decode(q.to(DEV).expand(B, -1, -1, -1), pool.cache, pool.table_dev.expand(B, -1),
+                                 pool.lengths.expand(B), return_softmax_lse=True)
+    check_status(DEV)
+    ref, rl, mass, reach = so.decode(q[0, :, 0].double(), k[0, :, 0], v[0, :, 0], size[0, :, 0], [n], 1 / math.sqrt(D))
+    e = (D + 8) * 2.0 ** -22 * reach[:, None]
+    tol = 2.0 ** -11 * ref.abs() + ((1 if bits == 16 else 2) * 2.0 ** -11 + 2.0 ** -20 + 2 * e) * mass
+    tol = tol + 3 * n * 2.0 ** -37 * size.max() + 2.0 ** -25  # (the output's own subnormals)
+    off = (out[:, 0, 0].cpu().double() - ref).abs()
+    assert bool((off <= tol).all()), (float((off / tol).max()), float((off[0].norm() / ref.norm())))
+    assert bool(((lse[:, 0, 0].cpu().double() - rl).abs() <= 2.0 ** -20 * (1 + rl.abs()) + e[:, 0]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,gap", [(64, 0.0), (9000, 12.0), (70000, 12.0), (70000, 18.0)])
+@pytest.mark.parametrize("high", [1.0, 1000.0])
+def test_many_small_weights_16_bit(n, gap, high):
+    """One token far above the others, whose many small probabilities hold the output."""
+    _check_far(*_far(n, 64, gap, 16, 0.0, high, 5), 16)

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   using M = T;  // operand type
   constexpr int U = C::kU, NS = C::kStages, ROWS = 8 * NT, NG = BITS == 4 ? C::kGroups : 1;
   constexpr int KSTEPS = D / 16;
-  constexpr float LIFT = BITS == 16 && Elem<M>::kIdescAB == 0 ? kLift : 0.f;
+  constexpr float LIFT = Elem<M>::kIdescAB == 0 ? kLift : 0.f;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   struct Misc {
     uint64_t bars[kWarps * NS];
@@ -444,6 +444,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   int lim[NT][2];               // tokens that a column's query row sees
   int col_q[NT][2];             // query token of a column's row; -1: none
   float o[KSTEPS][NT][4], om[NT][4], l[NT][2];
+  // 4-bit: exponent field of the largest scale of V so far; scales enter the products
+  // times 2^(15 - se), below 2
+  uint32_t se = 0;
   float mf[NT][2];              // running maximum in the log2 domain, less LIFT
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
 
@@ -489,6 +492,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     qp_last = (int)p.group_div.div(min(rows, (rb + 1) * ROWS) - 1);
     min_lim = limit_of(qp_first);
     max_lim = limit_of(qp_last);
+    se = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -648,13 +652,47 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         top[n][1] = fmaxf(top[n][1], fmaxf(s[u][n][1], s[u][n][3]));
       }
     }
-    // ---- running maximum; O and the sum follow it
+    // ---- running maximum and largest scale; O and the sum follow them
     bool above = false;
+    // The lane's two scales of block u (tokens that no row sees: 0).
+    auto scales = [&](int u) {
+      uint32_t w[1] = {0};
+      if (lane < 8 * NG) {
+        load_words<1>(bytes + u * C::kBlockBytes + Kv4(D).v_params() + lane * 4, w);
+        if constexpr (EDGE) {
+          const int to = max_lim - block_token(cur, u), tok = (lane >> 1 & 3) * 2 + (lane & 1) * 8;
+          w[0] &= (tok < to ? 0xFFFFu : 0u) | (tok + 1 < to ? 0xFFFF0000u : 0u);
+        }
+      }
+      return w[0];
+    };
+    if constexpr (BITS == 4) {
+      uint32_t most = (se << 10 | 0x3FFu) * 0x10001u;  // the largest scales that `se` is right for
+      const uint32_t had = most;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (!skipped(u)) most = __vmaxu2(most, scales(u));
+      above = most != had;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + (LIFT + kSlack);
     if (__any_sync(0xffffffffu, above)) {
+      float shrink = 1.f;  // of O's codes
+      if constexpr (BITS == 4) {
+        uint32_t now = se;
+#pragma unroll 1
+        for (int u = 0; u < U; ++u) {
+          if (skipped(u)) continue;
+          const uint32_t w = scales(u), a = w >> 10 & 31u, b = w >> 26 & 31u;
+          if (a < 31u) now = max(now, a);  // a group with a NaN has none
+          if (b < 31u) now = max(now, b);
+        }
+        now = __reduce_max_sync(0xffffffffu, now);
+        shrink = __uint_as_float((127u + se - now) << 23);
+        se = now;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -670,8 +708,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           om[n][i + 2] *= keep;
 #pragma unroll
           for (int k = 0; k < KSTEPS; ++k) {
-            o[k][n][i] *= keep;
-            o[k][n][i + 2] *= keep;
+            o[k][n][i] *= keep * shrink;
+            o[k][n][i + 2] *= keep * shrink;
           }
         }
     }
@@ -681,6 +719,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
       for (int i = 0; i < 2; ++i)  // no score above -inf yet: every probability is 0
         from[n][i] = fmaxf(mf[n][i], -3.4e38f);
+    // 2^(15 - se), twice
+    const uint32_t unit = (se < 30 ? (30u - se) << 10 : 0x200u) * 0x10001u;
     // ---- P^T, O^T += V^T P^T
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -783,6 +823,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
               sc[0] &= keep0;
               sc[1] &= keep1;
             }
+            sc[0] = hmul2(sc[0], unit);
+            sc[1] = hmul2(sc[1], unit);
             const uint32_t x0 = w0[grp] >> 8, x1 = w1[grp] >> 8;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -822,10 +864,11 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
           for (int grp = 0; grp < NG; ++grp) {
             const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t);
+            // 2^24 2^(se - 15) and 2^20 2^(se - 15): the codes' and the scales' powers of two
+            const float x24 = __uint_as_float((136u + se) << 23), x20 = __uint_as_float((132u + se) << 23);
             *reinterpret_cast<float4*>(dst + 32 * grp + 4 * g) =
-                make_float4(fmaf(o[2 * grp][n][i], 0x1p24f, mm), fmaf(o[2 * grp][n][i + 2], 0x1p20f, mm),
-                            fmaf(o[2 * grp + 1][n][i], 0x1p24f, mm),
-                            fmaf(o[2 * grp + 1][n][i + 2], 0x1p20f, mm));
+                make_float4(fmaf(o[2 * grp][n][i], x24, mm), fmaf(o[2 * grp][n][i + 2], x20, mm),
+                            fmaf(o[2 * grp + 1][n][i], x24, mm), fmaf(o[2 * grp + 1][n][i + 2], x20, mm));
           }
         }
         if (EACH == 2 && i == 0) continue;

@@ -118,3 +118,35 @@ def _check_far(pool, q, k, v, size, bits):
 def test_many_small_weights_16_bit(n, gap, high):
     """One token far above the others, whose many small probabilities hold the output."""
     _check_far(*_far(n, 64, gap, 16, 0.0, high, 5), 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["even", "growing", "shrinking"])
+@pytest.mark.parametrize("n,gap", [(64, 0.0), (9000, 12.0), (70000, 12.0), (70000, 18.0)])
+@pytest.mark.parametrize("D,high", [(64, 1.0), (128, 0.003), (32, 3e-4), (64, 6e4)])
+def test_many_small_weights_4_bit(D, high, n, gap, order):
+    """The same over 4-bit values from 3e-4 to 6e4, whose scales meet those weights."""
+    _check_far(*_far(n, D, gap, 4, 0.0, high, 5, order), 4)
+
+
+@pytest.mark.gpu
+def test_scales_that_are_not_seen_or_not_numbers():
+    """Tokens behind the length with the largest scales, and a group of NaN before small values:
+    the other groups of the row are what they are without them."""
+    n, D = 300, 64
+    pool, q, k, v, size = _far(n, D, 6.0, 4, 0.0, 0.003, 9)
+    B = 3
+    call = lambda m: flash_attn_decode(q.to(DEV).expand(B, -1, -1, -1), pool.cache, pool.table_dev.expand(B, -1),  # noqa: E731
+                                       _ints([m] * B))
+    want = call(250)
+    big = torch.zeros((1, 50, 1, D), dtype=F16, device=DEV)
+    big[..., ::2] = 6e4
+    kv_cache_append(pool.cache, big, big, pool.table_dev, _ints([250]))
+    assert torch.equal(call(250), want)
+    bad = v[:, :1].half().to(DEV)
+    bad[..., 3] = math.nan
+    kv_cache_append(pool.cache, k[:, :1].half().to(DEV), bad, pool.table_dev, _ints([0]))
+    kv_cache_append(pool.cache, k[:, :1].half().to(DEV), torch.where(bad.isnan(), 0.0, bad), pool.table_dev, _ints([1]))
+    out = call(250)
+    check_status(DEV)
+    assert bool(out[..., :32].isnan().all()) and bool(out[..., 32:].isfinite().all())

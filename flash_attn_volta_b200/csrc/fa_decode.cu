@@ -398,17 +398,17 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   auto block_token = [&](const Cursor& c, int u) {
     return c.tt * C::kTile + (u * kWarps + warp) * kBlockTokens;  // a short tile's blocks go to all warps
   };
-  auto look_up = [&](const Cursor& c, bool wanted) {  // page of the lane's block; -2: none
+  auto look_up = [&](const Cursor& c, bool wanted) {  // page of the lane's block, if it has one
     const int tok = block_token(c, lane);
     return wanted && lane < U && tok < c.len
                ? p.kv.table[(long long)c.b * p.kv.table_width + (tok >> p.page_shift)]
-               : -2;
+               : 0;
   };
   auto issue = [&](int stage, int next_id) {
-    const bool ok = next_id != -2 && !p.kv.bad_page(next_id);
+    const bool tokens = lane < U && block_token(pc, lane) < pc.len, ok = tokens && !p.kv.bad_page(next_id);
     if (lane < U) {
       const uint32_t bar = my_bars + stage * 8;
-      if (next_id != -2 && !ok) p.kv.report(kStatusPage);
+      if (tokens && !ok) p.kv.report(kStatusPage);
       if (ok) {
         // block (16-bit: row) of the cache, below 2^31
         const int at = (((next_id * p.kv.heads + pc.h) << p.page_shift) |

@@ -150,3 +150,24 @@ def test_scales_that_are_not_seen_or_not_numbers():
     out = call(250)
     check_status(DEV)
     assert bool(out[..., :32].isnan().all()) and bool(out[..., 32:].isfinite().all())
+
+
+# ---------------------------------------------------------------- GPU: page ids
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("wrong", [-2, -3])
+def test_every_bad_page_id_is_reported(bits, wrong):
+    """(-2 was the kernel's own mark of 'no block here'.)"""
+    pool, k, v, size = _filled([40, 40], 16, 1, 64, F16, bits, seed=6)
+    q = torch.randn((2, 1, 2, 64), generator=torch.Generator().manual_seed(8)).half()
+    table = pool.table.clone()
+    table[1, 1] = wrong
+    check_status(DEV)
+    out = flash_attn_decode(q.to(DEV), pool.cache, table.to(DEV), pool.lengths)
+    with pytest.raises(RuntimeError, match="status 4"):
+        check_status(DEV)
+    keep = torch.cat([torch.arange(16), torch.arange(32, 40)])
+    ks, vs, ss = (t.clone() for t in (k, v, size))
+    for t, src in ((ks, k), (vs, v), (ss, size)):
+        t[1, :24] = src[1, keep]
+    _check_decode(q, out, None, ks, vs, ss, [40, 24], [39, 39], True, bits)

@@ -292,9 +292,11 @@ __device__ __forceinline__ void write_row(const DecodeParams& p, int b, int h, i
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : NAN;
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 4; ++j) {
     w[j] = p.bf16 ? Elem<__nv_bfloat16>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv)
                   : Elem<__half>::pack2(x[2 * j] * inv, x[2 * j + 1] * inv);
+    if (p.kv.bits == 4 && !p.bf16) w[j] = most_half2(w[j]);
+  }
   *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) +
                             (((long long)b * p.Sq + qpos) * p.H + hq) * D + d) =
       make_uint4(w[0], w[1], w[2], w[3]);

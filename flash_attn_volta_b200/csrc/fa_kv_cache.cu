@@ -84,7 +84,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // Rounds the 32 values of a group, 8 in each of 4 neighbouring lanes, to codes.
 // Returns (s, m); a group with a NaN reads back as NaN, infinities as the
-// largest fp16.  The quotient (x - m) / s is the correctly rounded one
+// largest fp16 (its rounding to codes apart).  The quotient (x - m) / s is the correctly rounded one
 // (Markstein: with r = 1/s rounded, q = d r, then q + r (d - q s) in fused
 // steps), so a code is the definition's also where it is half a step; adding
 // 1.5 2^23 rounds it to a whole number, ties to even, in the sum's low bits.
@@ -478,6 +478,12 @@ struct ReadParams {
 __device__ __forceinline__ float2 pair_of(uint32_t masked) {
   return __half22float2(*reinterpret_cast<const __half2*>(&masked));
 }
+// Two values of the cache in the result's type.
+template <typename T>
+__device__ __forceinline__ uint32_t read2(float a, float b) {
+  const uint32_t w = Elem<T>::pack2(a, b);
+  return std::is_same<T, __half>::value ? most_half2(w) : w;
+}
 template <int N>
 __device__ __forceinline__ void load_words(const uint32_t* at, uint32_t (&w)[N]) {
   if constexpr (N == 4) {
@@ -597,7 +603,8 @@ __global__ void __launch_bounds__(kThreads) fa_kv_read_kernel(const ReadParams p
             x[2 * i] = fmaf(i % 2 ? s20 : s24, c.x, sm.y);
             x[2 * i + 1] = fmaf(i % 2 ? s20 : s24, c.y, sm.y);
           }
-          k_out[r * pitch + grp * 4 + t] = pack8<T>(x);
+          k_out[r * pitch + grp * 4 + t] =
+              make_uint4(read2<T>(x[0], x[1]), read2<T>(x[2], x[3]), read2<T>(x[4], x[5]), read2<T>(x[6], x[7]));
         }
       }
       const int r0 = n * 8 + 2 * t;
@@ -616,9 +623,9 @@ __global__ void __launch_bounds__(kThreads) fa_kv_read_kernel(const ReadParams p
             y[i] = fmaf(s.y * (i % 2 ? 0x1p20f : 0x1p24f), c[i].y, m.y);
           }
           uint2* to = reinterpret_cast<uint2*>(v_out + r0 * pitch) + grp * 8 + g;
-          to[0] = make_uint2(Elem<T>::pack2(x[0], x[1]), Elem<T>::pack2(x[2], x[3]));
+          to[0] = make_uint2(read2<T>(x[0], x[1]), read2<T>(x[2], x[3]));
           if (r0 + 1 < copied)
-            to[2 * pitch] = make_uint2(Elem<T>::pack2(y[0], y[1]), Elem<T>::pack2(y[2], y[3]));
+            to[2 * pitch] = make_uint2(read2<T>(y[0], y[1]), read2<T>(y[2], y[3]));
         }
       }
     }

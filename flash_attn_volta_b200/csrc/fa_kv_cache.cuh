@@ -4,7 +4,8 @@
 // A group is 32 consecutive dims of one token: minimum m (fp16, rounded down),
 // scale s (fp16, (max - m) / 15 rounded up), codes c = rint((x - m) / s) in
 // 0..15, value m + s c.  Rounding m down and s up keeps every value inside
-// [m, m + 15 s], so no code is clipped.  A block is, in this order,
+// [m, m + 15 s], so no code is clipped; m + 15 s may reach 65536, which fp16
+// results hold to 65504 (most_half2).  A block is, in this order,
 //   K codes   one word of 8 codes per (token, t, group); it holds dims
 //             32 group + 8 t + 0..7, codes of even dims in the low half
 //             (dims 0, 2, 4, 6 from bit 0 up), of odd dims in the high half
@@ -35,6 +36,12 @@ struct Kv4 {  // offsets of a block's parts in bytes; D is 32, 64 or 128
   __host__ __device__ constexpr int v_params() const { return 18 * D; }
   __host__ __device__ constexpr int bytes() const { return 20 * D; }
 };
+
+// Two fp16 values, at most 65504 each; NaN stays.
+__device__ __forceinline__ uint32_t most_half2(uint32_t w) {
+  const __half2 r = __hmin2_nan(*reinterpret_cast<const __half2*>(&w), __half2half2(__ushort_as_half(0x7BFF)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
 struct KvView {  // a cache as the kernels take it
   uint8_t* k;    // 16-bit: keys (pages, heads, page, D); 4-bit: blocks

@@ -200,7 +200,8 @@ int fa_sm100_rotary(const fa_sm100_heads* q, const fa_sm100_heads* k, const doub
  *   32 dims of a token: m = the smallest value rounded down to fp16, s = (largest
  *   - m) / 15 rounded up to fp16, code = round((x - m) / s), value m + s * code.
  *   (The order of the codes in a block: csrc/fa_kv_cache.cuh.)  Values beyond
- *   +-65504 are clamped; a group that holds a NaN reads back as NaN.
+ *   +-65504 are clamped; a group that holds a NaN reads back as NaN.  As s is rounded
+ *   up, m + 15 s may reach 65536: fp16 results are held to 65504.
  * All bases 16-byte aligned; num_pages * nheads_kv * page_size <= 2^31 - 1. */
 typedef struct fa_sm100_kv_cache {
   void* k_pages;

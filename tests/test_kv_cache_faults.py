@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from flash_attn_volta_b200 import _lib, check_status
-from flash_attn_volta_b200.kv_cache import flash_attn_decode, kv_cache_append
+from flash_attn_volta_b200.kv_cache import flash_attn_decode, kv_cache_append, kv_cache_read
 from oracle import serving_oracle as so
 from tests.test_kv_cache import BF16, DEV, F16, Pool, _check_decode, _filled, _ints
 
@@ -171,3 +171,30 @@ def test_every_bad_page_id_is_reported(bits, wrong):
     for t, src in ((ks, k), (vs, v), (ss, size)):
         t[1, :24] = src[1, keep]
     _check_decode(q, out, None, ks, vs, ss, [40, 24], [39, 39], True, bits)
+
+
+# ---------------------------------------------------------------- GPU: the largest 4-bit values
+@pytest.mark.gpu
+@pytest.mark.parametrize("top", [65504.0, 65472.0, math.inf])
+@pytest.mark.parametrize("bottom", [0.0, -65504.0, 60000.0, -math.inf])
+def test_the_largest_values_stay_finite_in_fp16(top, bottom):
+    """The scale is rounded up, so minimum + 15 scale passes 65504 (0 + 15 x 4368, -65504 + 15 x
+    8736): what is read back, and the attention's output, is 65504 at most, not infinite."""
+    x = torch.linspace(0.0, 1.0, 64).half().view(1, 1, 1, 64).repeat(1, 2, 1, 1)
+    x[..., 7], x[..., 9] = top, bottom
+    x[0, 1, 0, 40] = math.nan
+    pool = Pool([2], 16, 1, 64, F16, 4)
+    kv_cache_append(pool.cache, torch.zeros_like(x).to(DEV), x.to(DEV), pool.table_dev, _ints([0]))
+    _, got = kv_cache_read(pool.cache, pool.table_dev, pool.lengths, 2)
+    q = torch.ones((1, 1, 1, 64), dtype=F16, device=DEV)
+    out = flash_attn_decode(q, pool.cache, pool.table_dev, _ints([1]))
+    check_status(DEV)
+    want = x[0, 0, 0].double().clamp(-65504, 65504)
+    step = (want[:32].max() - want[:32].min()) / 15
+    for t in (got[0, 0, 0], out[0, 0, 0]):
+        t = t.cpu().double()
+        assert bool(t.isfinite().all())
+        # half a step, the step's own rounding up (2^-10), 15 times, and the result's rounding
+        assert bool(((t[:32] - want[:32]).abs() <= step * (0.5 + 16 * 2.0 ** -10) + 2.0 ** -11 * 65504).all())
+        assert t[7] == 65504 or top < 65504
+    assert bool(got[0, 1, 0, 32:].isnan().all()) and bool(got[0, 1, 0, :32].isfinite().all())

@@ -51,6 +51,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cfloat>
+#include <cmath>
 #include <type_traits>
 
 #include "fa_kernels.h"
@@ -1166,7 +1168,7 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
                                void* stream) {
   using namespace fa_sm100;
   if (!cache || !decode_shape_ok(cache, table_width, batch, seqlen, nheads)) return FA_ERR_ARG;
-  if (!q || !out || !page_table || !lengths) return FA_ERR_ARG;
+  if (!q || !out || !page_table || !lengths || !std::isfinite(sm_scale)) return FA_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) return FA_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(page_table) |
        reinterpret_cast<uintptr_t>(lengths) | reinterpret_cast<uintptr_t>(starts)) & 3u)

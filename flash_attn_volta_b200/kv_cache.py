@@ -129,7 +129,8 @@ def _check_append(cache, k, v, page_table, starts, counts, q, rotary):
         assert rotary.inv_freq.device == cache.device, "inv_freq must be on the cache's device"
 
 
-def _check_decode(q, cache, page_table, lengths, starts):
+def _check_decode(q, cache, page_table, lengths, starts, sm_scale):
+    assert math.isfinite(sm_scale), f"sm_scale {sm_scale} is not finite"
     shape, H = q.shape, cache.n_heads
     assert len(shape) == 4 and shape[3] == cache.head_dim and shape[2] > 0 and shape[2] % H == 0, \
         f"q {tuple(shape)} does not fit a cache of {H} heads of {cache.head_dim}"
@@ -221,7 +222,7 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
     try:
         out = fn(q, cache.k_pages, cache.v_pages, page_table, lengths, starts, causal, sm_scale)
     except RuntimeError:
-        _check_decode(q, cache, page_table, lengths, starts)
+        _check_decode(q, cache, page_table, lengths, starts, sm_scale)
         raise
     dev = cache.device
     ops.note_device(dev.index)

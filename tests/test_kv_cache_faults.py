@@ -198,3 +198,22 @@ def test_the_largest_values_stay_finite_in_fp16(top, bottom):
         assert bool(((t[:32] - want[:32]).abs() <= step * (0.5 + 16 * 2.0 ** -10) + 2.0 ** -11 * 65504).all())
         assert t[7] == 65504 or top < 65504
     assert bool(got[0, 1, 0, 32:].isnan().all()) and bool(got[0, 1, 0, :32].isfinite().all())
+
+
+# ---------------------------------------------------------------- scales and sizes of q
+@pytest.mark.gpu
+def test_scales_that_are_not_finite_are_refused():
+    pool, *_ = _filled([5], 16, 1, 64, F16, 16)
+    q = torch.zeros((1, 1, 2, 64), dtype=F16, device=DEV)
+    for scale in (math.nan, math.inf, -math.inf):
+        with pytest.raises(AssertionError, match="finite"):
+            flash_attn_decode(q, pool.cache, pool.table_dev, pool.lengths, sm_scale=scale)
+
+
+def test_c_abi_refuses_scales_that_are_not_finite():
+    import ctypes
+    lib = _lib.load()
+    c = ctypes.byref(_lib.KvCache(4096, 4096, 2, 64, 2, 64, 0, 16))
+    for scale in (math.nan, math.inf, -math.inf):
+        assert lib.fa_sm100_decode(c, 256, 256, None, 256, 1, 256, None, 256, 0, 1, 1, 4, scale, 1, None,
+                                   None) == _lib.FA_ERR_ARG

@@ -539,10 +539,11 @@ __global__ void __launch_bounds__(kThreads, kCtas)
         const uint32_t one = max(most & 0xFFFFu, most >> 16);
         const float top = p.bf16 ? Elem<__nv_bfloat16>::value((uint16_t)one) : Elem<__half>::value((uint16_t)one);
         int e = (int)(__float_as_uint(top) >> 23) - 127;  // 2^e <= top < 2^(e + 1)
-        e = max(-90, min(e, 110));
+        e = max(-116, min(e, 127));
         const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
         const float turn = p.negate ? -up : up;
-        const float down = __uint_as_float((uint32_t)(127 + 10 + e) << 23) * p.scale_log2;  // 2^20 / up
+        float down = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2 * 1024.f;  // 2^20 / up
+        down = fmaxf(fminf(down, FLT_MAX), FLT_MIN);  // finite, and above 0
         float mine = 0.f;  // sum of group t
 #pragma unroll
         for (int grp = 0; grp < NG; ++grp) {
@@ -1214,7 +1215,7 @@ extern "C" int fa_sm100_decode(const fa_sm100_kv_cache* cache, const void* q, vo
   p.direct = p.whole && pl.grid == (long long)batch * cache->nheads_kv * pl.row_blocks;
   p.negate = sm_scale < 0.f;
   p.bf16 = cache->dtype == FA_DTYPE_BF16;
-  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, 1e-30f);
+  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.44269504088896341f, FLT_MIN);
   p.skip_copy = debug_flags() & 2;
   p.timeout_ns = wait_timeout_ns();
   return launch_decode_any(p, pl.nt, tk, tv, pl.split, static_cast<cudaStream_t>(stream));

@@ -217,3 +217,18 @@ def test_c_abi_refuses_scales_that_are_not_finite():
     for scale in (math.nan, math.inf, -math.inf):
         assert lib.fa_sm100_decode(c, 256, 256, None, 256, 1, 256, None, 256, 0, 1, 1, 4, scale, 1, None,
                                    None) == _lib.FA_ERR_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("power", [-100, 60, 100, 112, 116, 122])
+def test_large_queries_and_small_scales(bits, power):
+    """q times 2^power with sm_scale times 2^-power is the same attention, bit for bit: bf16 q may be
+    as large as 2^127, and a scale as small as 2^-125."""
+    pool, k, v, size = _filled([300, 77], 32, 1, 64, BF16, bits, seed=15)
+    q = torch.randn((2, 3, 4, 64), generator=torch.Generator().manual_seed(8)).bfloat16().to(DEV)
+    call = lambda x, scale: flash_attn_decode(x, pool.cache, pool.table_dev, pool.lengths, sm_scale=scale,  # noqa: E731
+                                              return_softmax_lse=True)
+    want = call(q, 0.125)
+    out = call(q * 2.0 ** power, 0.125 * 2.0 ** -power)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])

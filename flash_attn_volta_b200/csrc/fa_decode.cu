@@ -72,6 +72,12 @@ constexpr float kSlack = 2.f;
 // reach 2^14 and are normal numbers down to 2^-26 of the largest (unlifted, 2^-14: of
 // 70000 tokens 18 below one in score a fifth of their part of the output was lost).
 constexpr float kLift = 12.f;
+// From 2^kFar on (in log2) a maximum is off the fused product that it was rounded from by
+// half or more, and the probabilities would leave fp16: the row's scores are then divided
+// by the power of two that brings the maximum below 2^kFar.  (Gaps shrink with them, those
+// below 20 2^-23 of the maximum to where they count: less than the sums of products are
+// off, (D + 8) 2^-22.)
+constexpr int kFar = 24;
 constexpr float kLn2 = 0.69314718055994531f;
 
 // Per-instantiation constants.
@@ -105,12 +111,12 @@ struct Cfg {
   static constexpr int kTile = kWarps * kU * kBlockTokens;  // tokens
   static constexpr int kCost = cost_of(D, BITS, NT);
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kMiscBytes = NT <= 2 ? 512 : 640;  // barriers and small shared variables
   static constexpr int kJoinStride = D + 4;  // floats of a row in the join buffer
   // The warps join all 8 rows of a column block at once, or 4 where there is no room.
   static constexpr int kJoinRows =
-      kCtas * (kRingBytes + kWarps * 8 * kJoinStride * 4 + 512 + 1024) <= 228 * 1024 ? 8 : 4;
+      kCtas * (kRingBytes + kWarps * 8 * kJoinStride * 4 + kMiscBytes + 1024) <= 228 * 1024 ? 8 : 4;
   static constexpr int kJoinBytes = kWarps * kJoinRows * kJoinStride * 4;
-  static constexpr int kMiscBytes = 512;         // barriers and small shared variables
   static constexpr int kSmem = kRingBytes + kJoinBytes + kMiscBytes;
   static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
   static constexpr int kGroups = D / 32;
@@ -324,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     Spot spot;
     unsigned warp_sum[kWarps];
     float2 join_ml[kWarps][8];
+    uint8_t cut[kWarps][ROWS];  // powers of two that the rows' scores were divided by
     int abort_flag;
   };
   static_assert(sizeof(Misc) <= C::kMiscBytes, "small shared variables");
@@ -451,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   // 4-bit: exponent field of the largest scale of V so far; scales enter the products
   // times 2^(15 - se), below 2
   uint32_t se = 0;
-  float mf[NT][2];              // running maximum in the log2 domain, less LIFT
+  float mf[NT][2];              // running maximum in the log2 domain
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
 
   auto limit_of = [&](int qpos) {
@@ -497,6 +504,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     min_lim = limit_of(qp_first);
     max_lim = limit_of(qp_last);
     se = 0;
+    if (lane < ROWS) sh.cut[warp][lane] = 0;
+    __syncwarp();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -682,8 +691,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + (LIFT + kSlack);
+      for (int i = 0; i < 2; ++i) above |= top[n][i] * f[n][i] > mf[n][i] + kSlack;
     if (__any_sync(0xffffffffu, above)) {
+      bool far = false;
       float shrink = 1.f;  // of O's codes
       if constexpr (BITS == 4) {
         uint32_t now = se;
@@ -705,7 +715,8 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
           for (int d = 4; d < 32; d *= 2)
             top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], d));
-          const float now = fmaxf(mf[n][i], top[n][i] * f[n][i] - LIFT);
+          const float now = fmaxf(mf[n][i], top[n][i] * f[n][i]);
+          far |= fabsf(now) >= 0x1p24f && fabsf(now) < INFINITY;
           const float keep = now == -INFINITY ? 1.f : ex2(mf[n][i] - now);
           mf[n][i] = now;
           l[n][i] *= keep;
@@ -717,13 +728,28 @@ __global__ void __launch_bounds__(kThreads, kCtas)
             o[k][n][i + 2] *= keep * shrink;
           }
         }
+      static_assert(kFar == 24, "the bound above");
+      if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int by = (int)(__float_as_uint(mf[n][i]) >> 23 & 255u) - 127 - (kFar - 1);
+            if (by > 0 && by <= 128 - kFar) {  // (not an infinity)
+              const float less = __uint_as_float((uint32_t)(127 - by) << 23);
+              f[n][i] *= less;
+              mf[n][i] *= less;
+              if (g == 0) sh.cut[warp][n * 8 + 2 * t + i] += by;
+            }
+          }
+      }
     }
     float from[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i)  // no score above -inf yet: every probability is 0
-        from[n][i] = fmaxf(mf[n][i], -3.4e38f);
+        from[n][i] = fmaxf(mf[n][i], -3.4e38f) - LIFT;
     // 2^(15 - se), twice
     const uint32_t unit = (se < 30 ? (30u - se) << 10 : 0x200u) * 0x10001u;
     // ---- P^T, O^T += V^T P^T
@@ -857,20 +883,25 @@ __global__ void __launch_bounds__(kThreads, kCtas)
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], d);
         const int place = t * EACH + (EACH == 2 ? i : 0);
-        if (g == 0) sh.join_ml[warp][place] = make_float2(mf[n][i], l[n][i]);
+        constexpr float DOWN = LIFT > 0.f ? 0x1p-12f : 1.f;
+        static_assert(kLift == 12.f, "2^-kLift");
+        if (g == 0) {
+          const uint32_t cut = sh.cut[warp][n * 8 + 2 * t + i];
+          sh.join_ml[warp][place] = make_float2(mf[n][i] * __uint_as_float((127u + cut) << 23), l[n][i] * DOWN);
+        }
         float* dst = join + (warp * JR + place) * C::kJoinStride;
         if constexpr (BITS == 16) {
 #pragma unroll
           for (int k = 0; k < KSTEPS; ++k) {
-            dst[16 * k + g] = o[k][n][i];
-            dst[16 * k + 8 + g] = o[k][n][i + 2];
+            dst[16 * k + g] = o[k][n][i] * DOWN;
+            dst[16 * k + 8 + g] = o[k][n][i + 2] * DOWN;
           }
         } else {
 #pragma unroll
           for (int grp = 0; grp < NG; ++grp) {
-            const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t);
-            // 2^24 2^(se - 15) and 2^20 2^(se - 15): the codes' and the scales' powers of two
-            const float x24 = __uint_as_float((136u + se) << 23), x20 = __uint_as_float((132u + se) << 23);
+            const float mm = __shfl_sync(0xffffffffu, om[n][i], grp * 4 + t) * DOWN;
+            // 2^24 and 2^20 (codes), 2^(se - 15) (scales), 2^-kLift
+            const float x24 = __uint_as_float((124u + se) << 23), x20 = __uint_as_float((120u + se) << 23);
             *reinterpret_cast<float4*>(dst + 32 * grp + 4 * g) =
                 make_float4(fmaf(o[2 * grp][n][i], x24, mm), fmaf(o[2 * grp][n][i + 2], x20, mm),
                             fmaf(o[2 * grp + 1][n][i], x24, mm), fmaf(o[2 * grp + 1][n][i + 2], x20, mm));

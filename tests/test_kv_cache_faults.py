@@ -232,3 +232,25 @@ def test_large_queries_and_small_scales(bits, power):
     want = call(q, 0.125)
     out = call(q * 2.0 ** power, 0.125 * 2.0 ** -power)
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("power", [16, 22, 24, 27, 31, 40, 80, 118])
+@pytest.mark.parametrize("n", [300, 3000])
+def test_scores_beyond_the_rest_pick_their_token(bits, power, n):
+    """q of 2^power at the usual scale: the largest score takes all the weight, next to a row of
+    ordinary scores.  (The gap to the second one is over 20 after any halving of the scores, and
+    over what the sums of products are off.)"""
+    pool, k, v, size = _filled([n], 32, 1, 64, BF16, bits, seed=16)
+    q = torch.randn((1, 1, 2, 64), generator=torch.Generator().manual_seed(8)).bfloat16()
+    q[:, :, 1] *= 2.0 ** power
+    out, lse = flash_attn_decode(q.to(DEV), pool.cache, pool.table_dev, pool.lengths, return_softmax_lse=True)
+    score = (k[0, :, 0] @ q[0, 0, 1].double()) / 8
+    two, best = score.topk(2)
+    reach = float((k[0, :, 0].abs() @ q[0, 0, 1].double().abs()).max()) / 8
+    assert float(two[0] - two[1]) > max(40.0, 40 * 2.0 ** -23 * float(two[0]), 4 * 72 * 2.0 ** -22 * reach)
+    ref, most = v[0, int(best[0]), 0], size[0, int(best[0]), 0]
+    assert bool(((out[0, 0, 1].cpu().double() - ref).abs() <= 2 * 2.0 ** -8 * most + 2.0 ** -25).all())
+    assert abs(float(lse[0, 1, 0]) - float(two[0])) <= 2.0 ** -20 * abs(float(two[0])) + 72 * 2.0 ** -22 * reach
+    _check_decode(q[:, :, :1], out[:, :, :1], lse[:, :1], k, v, size, [n], None, True, bits)

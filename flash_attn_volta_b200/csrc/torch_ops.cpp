@@ -387,9 +387,25 @@ struct RotaryQkFn : public torch::autograd::Function<RotaryQkFn> {
   }
 };
 
+// What an operator has no derivative for is refused, not dropped: a forward-mode
+// tangent (as the C++ autograd functions do themselves), or a gradient of
+// `reverse` tensors.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+void check_derivatives(const char* op, std::initializer_list<const at::Tensor*> forward,
+                       std::initializer_list<const at::Tensor*> reverse) {
+  for (const at::Tensor* t : forward)
+    TORCH_CHECK(!t || !has_tangent(*t), op, ": forward-mode derivatives are not implemented");
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : reverse)
+    TORCH_CHECK(!t || !t->defined() || !t->requires_grad(), op, ": ",
+                "no gradient is computed for a tensor that requires one (detach it, or call under no_grad)");
+}
+const at::Tensor* ptr(const OptTensor& t) { return t ? &*t : nullptr; }
+
 at::Tensor rotary_autograd(const at::Tensor& x, const at::Tensor& inv_freq,
                            const OptTensor& positions, int64_t first, bool interleaved,
                            double magnitude, bool inverse) {
+  check_derivatives("rotary", {&x, &inv_freq}, {&inv_freq});
   if (at::GradMode::is_enabled() && x.requires_grad())
     return RotaryFn::apply(x, inv_freq, positions, first, interleaved, magnitude, inverse);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -401,6 +417,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_qk_autograd(const at::Tensor& q, const
                                                       const OptTensor& positions, int64_t first,
                                                       bool interleaved, double magnitude,
                                                       bool inverse) {
+  check_derivatives("rotary_qk", {&q, &k, &inv_freq}, {&inv_freq});
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad())) {
     auto r = RotaryQkFn::apply(q, k, inv_freq, positions, first, interleaved, magnitude, inverse);
     return {r[0], r[1]};
@@ -566,6 +583,51 @@ std::tuple<at::Tensor, at::Tensor> decode_lse_cuda(const at::Tensor& q, const at
   return {out, lse};
 }
 
+// The cache operators are for inference: under autograd they check that nothing
+// asks for a derivative, and go on below it.
+template <typename F>
+auto below_autograd(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+at::Tensor kv_append_autograd(const at::Tensor& k_pages, const OptTensor& v_pages, const at::Tensor& k,
+                              const at::Tensor& v, const OptTensor& q, const at::Tensor& table,
+                              const at::Tensor& starts, const OptTensor& counts, const OptTensor& freq,
+                              bool interleaved, double magnitude) {
+  const auto all = {&k_pages, ptr(v_pages), &k, &v, ptr(q), ptr(freq)};
+  check_derivatives("kv_append", all, all);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = below_autograd("fav::kv_append", kv_append_cuda);
+  return op.call(k_pages, v_pages, k, v, q, table, starts, counts, freq, interleaved, magnitude);
+}
+std::tuple<at::Tensor, at::Tensor> kv_read_autograd(const at::Tensor& k_pages, const OptTensor& v_pages,
+                                                    at::ScalarType dtype, const at::Tensor& table,
+                                                    const at::Tensor& lengths, int64_t max_len) {
+  const auto all = {&k_pages, ptr(v_pages)};
+  check_derivatives("kv_read", all, all);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = below_autograd("fav::kv_read", kv_read_cuda);
+  return op.call(k_pages, v_pages, dtype, table, lengths, max_len);
+}
+at::Tensor decode_autograd(const at::Tensor& q, const at::Tensor& k_pages, const OptTensor& v_pages,
+                           const at::Tensor& table, const at::Tensor& lengths, const OptTensor& starts,
+                           bool causal, double sm_scale) {
+  const auto all = {&q, &k_pages, ptr(v_pages)};
+  check_derivatives("decode", all, all);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = below_autograd("fav::decode", decode_cuda);
+  return op.call(q, k_pages, v_pages, table, lengths, starts, causal, sm_scale);
+}
+std::tuple<at::Tensor, at::Tensor> decode_lse_autograd(const at::Tensor& q, const at::Tensor& k_pages,
+                                                       const OptTensor& v_pages, const at::Tensor& table,
+                                                       const at::Tensor& lengths, const OptTensor& starts,
+                                                       bool causal, double sm_scale) {
+  const auto all = {&q, &k_pages, ptr(v_pages)};
+  check_derivatives("decode_lse", all, all);
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = below_autograd("fav::decode_lse", decode_lse_cuda);
+  return op.call(q, k_pages, v_pages, table, lengths, starts, causal, sm_scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fav, m) {
@@ -611,4 +673,8 @@ TORCH_LIBRARY_IMPL(fav, CUDA, m) {
 TORCH_LIBRARY_IMPL(fav, Autograd, m) {
   m.impl("rotary", &rotary_autograd);
   m.impl("rotary_qk", &rotary_qk_autograd);
+  m.impl("kv_append", &kv_append_autograd);
+  m.impl("kv_read", &kv_read_autograd);
+  m.impl("decode", &decode_autograd);
+  m.impl("decode_lse", &decode_lse_autograd);
 }

@@ -28,7 +28,7 @@ import math
 import torch
 
 from . import _lib, ops
-from .rotary import Rotary
+from .rotary import Rotary, _NO_GRADIENT
 
 BLOCK_TOKENS = 16
 
@@ -127,6 +127,7 @@ def _check_append(cache, k, v, page_table, starts, counts, q, rotary):
     if rotary is not None:
         assert rotary.dim <= D, f"rotary dim {rotary.dim} does not fit head_dim {D}"
         assert rotary.inv_freq.device == cache.device, "inv_freq must be on the cache's device"
+        assert not (rotary.inv_freq.requires_grad and torch.is_grad_enabled()), _NO_GRADIENT
 
 
 def _check_decode(q, cache, page_table, lengths, starts, sm_scale):

@@ -26,7 +26,8 @@ class Rotary:
     Args:
         inv_freq: 1-D tensor of R/2 angular frequencies (radians per position)
             on the device of the tensors to rotate; used in fp64 (any other
-            floating type is converted here, once).
+            floating type is converted here, once).  Gets no gradient: one that
+            requires it is refused.
         interleaved: pairs (2 i, 2 i + 1) instead of (i, i + R/2).
         magnitude: factor on cos and sin (1 but for some long-context scalings).
     """
@@ -79,6 +80,9 @@ class Rotary:
         return cls(inv.to(device), interleaved, magnitude)
 
 
+_NO_GRADIENT = "inv_freq gets no gradient: detach it"
+
+
 def _check(x: torch.Tensor, rotary: Rotary, positions, k=None) -> None:
     """Raise AssertionError for a call the operators refuse."""
     shape, dev = x.shape, x.device
@@ -88,6 +92,7 @@ def _check(x: torch.Tensor, rotary: Rotary, positions, k=None) -> None:
     assert shape[3] % 2 == 0 and rotary.dim <= shape[3], \
         f"rotary dim {rotary.dim} does not fit head_dim {shape[3]}"
     assert rotary.inv_freq.device == dev, "inv_freq must be on the tensors' device"
+    assert not (rotary.inv_freq.requires_grad and torch.is_grad_enabled()), _NO_GRADIENT
     if positions is not None:
         assert positions.device == dev, "positions must be on the tensors' device"
         assert positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64"
@@ -109,6 +114,7 @@ def rotary_embed(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor | None
 
     positions: (S,) or (B, S) int32 / int64; None: first, first + 1, ...
     The result is contiguous, in x's dtype; sums are in fp32, rounded once.
+    Reverse-mode derivatives only: a forward-mode tangent is refused.
     """
     ops.load()
     try:

@@ -3,8 +3,13 @@
 Serving next to ``flash_attn``: a prompt's attention runs in flash_attn while
 ``kv_cache_append`` stores its keys and values; then each new token is appended
 (rotated on the way) and ``flash_attn_decode`` attends to everything cached.
-A prompt that arrives in chunks reads its prefix back with ``kv_cache_read`` and
-calls flash_attn(q_chunk, k_all, v_all, causal=True).
+A prompt that arrives in chunks, where the chunk ends at the same length in every
+sequence of the call, reads its prefix back with ``kv_cache_read`` up to that length
+and calls flash_attn(q_chunk, k_all, v_all, causal=True); flash_attn knows no lengths,
+so the zeros behind a shorter sequence would count as keys and the mask would stand
+at the longest one's end.  Chunks of different starts or counts go through
+flash_attn_decode(..., starts=starts), or through read and flash_attn one sequence
+at a time.
 
 A page holds ``page_size`` tokens of one sequence; ``page_table`` (B, W) int32 names
 the page of tokens i * page_size .. of each sequence in column i (entries behind
@@ -178,7 +183,8 @@ def kv_cache_append(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
 def kv_cache_read(cache: PagedKVCache, page_table: torch.Tensor, lengths: torch.Tensor,
                   max_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The first lengths[b] cached tokens of each sequence as contiguous k and v
-    (B, max_len, H_kv, D) of the cache's dtype; rows behind a length are zero.
+    (B, max_len, H_kv, D) of the cache's dtype; rows behind a length are zero (not
+    masked: an attention over them needs the lengths).
     max_len: default the table's room; longer sequences are cut there."""
     if max_len is None:
         max_len = page_table.shape[-1] * cache.page_size
@@ -207,7 +213,8 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
         causal: query i of sequence b sees tokens j <= starts[b] + i.
         starts: (B,) int32 position of each sequence's first query (default
             lengths - S); for a batch whose sequences have different counts of
-            new tokens, pass what kv_cache_append got.
+            new tokens, pass what kv_cache_append got (rows behind a count are
+            padding: what they give means nothing).
         sm_scale, return_softmax_lse: as in flash_attn_forward.
 
     Returns:

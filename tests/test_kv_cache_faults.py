@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
-from flash_attn_volta_b200 import _lib, check_status
+from flash_attn_volta_b200 import _lib, check_status, flash_attn
 from flash_attn_volta_b200.kv_cache import flash_attn_decode, kv_cache_append, kv_cache_read
+from flash_attn_volta_b200.rotary import Rotary
 from oracle import serving_oracle as so
 from tests.test_kv_cache import BF16, DEV, F16, Pool, _check_decode, _filled, _ints
 
@@ -254,3 +255,57 @@ def test_scores_beyond_the_rest_pick_their_token(bits, power, n):
     assert bool(((out[0, 0, 1].cpu().double() - ref).abs() <= 2 * 2.0 ** -8 * most + 2.0 ** -25).all())
     assert abs(float(lse[0, 1, 0]) - float(two[0])) <= 2.0 ** -20 * abs(float(two[0])) + 72 * 2.0 ** -22 * reach
     _check_decode(q[:, :, :1], out[:, :, :1], lse[:, :1], k, v, size, [n], None, True, bits)
+
+
+# ---------------------------------------------------------------- chunks, tracing, threads
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("how", ["decode", "one at a time"])
+def test_ragged_chunks(bits, how):
+    """Prompts of different lengths in two chunks of different counts: every row that is not padding
+    is the attention over its own sequence up to its own position."""
+    B, S, H, Hkv, D = 4, 40, 6, 2, 64
+    counts = [[40, 17, 1, 33], [30, 40, 5, 0]]
+    total = [sum(c) for c in zip(*counts)]
+    g = torch.Generator().manual_seed(17)
+    mk = lambda h: torch.randn((B, 2 * S, h, D), generator=g).half()  # noqa: E731
+    q, k, v = mk(H), mk(Hkv), mk(Hkv)
+    pool = Pool(total, 16, Hkv, D, F16, bits)
+    starts, got = [0] * B, {}
+    for chunk in range(2):
+        n = counts[chunk]
+        take = lambda x: torch.stack([torch.cat([x[b, starts[b]:starts[b] + n[b]], 9 * torch.ones_like(x[b, n[b]:S])])  # noqa: E731
+                                      for b in range(B)]).to(DEV)
+        qc = kv_cache_append(pool.cache, take(k), take(v), pool.table_dev, _ints(starts), _ints(n), q=take(q))
+        ends = [a + m for a, m in zip(starts, n)]
+        if how == "decode":
+            out = flash_attn_decode(qc, pool.cache, pool.table_dev, _ints(ends), starts=_ints(starts))
+        for b in range(B):
+            if how != "decode":
+                ka, va = kv_cache_read(pool.cache, pool.table_dev[b:b + 1], _ints(ends[b:b + 1]), ends[b])
+                out = {b: flash_attn(qc[b:b + 1, :n[b]], ka, va, causal=True)[0]}
+            for i in range(n[b]):
+                got[b, starts[b] + i] = out[b][i].cpu()
+        starts = ends
+    check_status(DEV)
+    if bits == 4:
+        kc, km, ks = so.four_bit(k)
+        vc, vm, vs = so.four_bit(v)
+        k, v, size = so.values(kc, km, ks), so.values(vc, vm, vs), so.values(vc, vm.abs(), vs)
+    else:
+        k, v, size = k.double(), v.double(), v.double().abs()
+    if how == "decode":
+        rows = torch.stack([torch.stack([got.get((b, i), torch.zeros(H, D).half()) for i in range(2 * S)])
+                            for b in range(B)])
+        for b in range(B):
+            m = slice(b, b + 1), slice(0, total[b])
+            _check_decode(q[m], rows[m], None, k[b:b + 1], v[b:b + 1], size[b:b + 1], [total[b]], None, True, bits)
+        return
+    for (b, i), row in got.items():
+        for h in range(H):
+            ref, _, mass, reach = so.decode(q[b, i, h][None].double(), k[b, :, h // 3], v[b, :, h // 3],
+                                            size[b, :, h // 3], [i + 1], 1 / 8)
+            # as in test_serving_run without the rounding of a rotated q: p and out once, k and v read
+            # back in fp16 once (2^-11 of a score's reach, and of the values)
+            tol = 2.0 ** -11 * ref.abs() + (2.0 ** -9 + 2.0 ** -10 * reach[:, None]) * mass + 2.0 ** -12
+            assert bool(((row[h].double() - ref[0]).abs() <= tol[0]).all())

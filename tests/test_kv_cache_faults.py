@@ -309,3 +309,58 @@ def test_ragged_chunks(bits, how):
             # back in fp16 once (2^-11 of a score's reach, and of the values)
             tol = 2.0 ** -11 * ref.abs() + (2.0 ** -9 + 2.0 ** -10 * reach[:, None]) * mass + 2.0 ** -12
             assert bool(((row[h].double() - ref[0]).abs() <= tol[0]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_traced_step(bits):
+    """torch.compile takes append, attention and read as one graph."""
+    pool, *_ = _filled([20, 33], 16, 2, 64, F16, bits, seed=2, width=4)
+    c, table = pool.cache, pool.table_dev.clamp(min=0)
+    rot = Rotary.build(64, device=DEV)
+    g = torch.Generator().manual_seed(3)
+    mk = lambda h: torch.randn((2, 1, h, 64), generator=g).half().to(DEV)  # noqa: E731
+    q, k, v, n = mk(8), mk(2), mk(2), _ints([19, 32])
+
+    def step(q, k, v, n):
+        qr = kv_cache_append(c, k, v, table, n, q=q, rotary=rot)
+        out, lse = flash_attn_decode(qr, c, table, n + 1, return_softmax_lse=True)
+        return (out * 2, lse, *kv_cache_read(c, table, n + 1, 40))
+
+    before = [t.clone() for t in (c.k_pages, c.v_pages) if t is not None]
+    want = step(q, k, v, n)
+    after = [t.clone() for t in (c.k_pages, c.v_pages) if t is not None]
+    for t, was in zip((c.k_pages, c.v_pages), before):
+        t.copy_(was)
+    torch._dynamo.reset()
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, v, n)
+    check_status(DEV)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for t, is_now in zip((c.k_pages, c.v_pages), after):
+        assert torch.equal(t.view(torch.uint8), is_now.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_calls_from_two_threads():
+    """Two host threads, each with a stream and a cache of its own."""
+    import threading
+    pools = [_filled([700, 90], 32, 2, 64, F16, bits, seed=31)[0] for bits in (16, 4)]
+    q = torch.randn((2, 1, 8, 64), generator=torch.Generator().manual_seed(8)).half().to(DEV)
+    call = lambda p: flash_attn_decode(q, p.cache, p.table_dev, p.lengths)  # noqa: E731
+    want = [call(p) for p in pools]
+    torch.cuda.synchronize(DEV)
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream(DEV)):
+            got = [call(pools[i]) for _ in range(50)]
+            torch.cuda.current_stream(DEV).synchronize()
+            wrong.extend(i for o in got if not torch.equal(o, want[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    check_status(DEV)

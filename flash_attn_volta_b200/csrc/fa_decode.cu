@@ -25,7 +25,7 @@
 // * 4-bit codes are used as they are: a nibble masked out of its word is the
 //   fp16 subnormal c 2^-24 (bits 0..3) or c 2^-20 (bits 4..7), exact in the
 //   matrix instruction, so 8 codes cost one shift and four ANDs (the integer pipe
-//   is the busiest: 44 % at 2 x 131072 tokens).  The power of two goes into q (K) or
+//   is the busiest: 45 % at 2 x 131072 tokens).  The power of two goes into q (K) or
 //   the final factor (V).  Summing V's even dims as whole bytes 16 c1 + c0 and parting
 //   them at the end saves an AND in five and 5 % of the time, but the matrix
 //   instruction's sums are truncated, and 16 c1 is 17 times the sum that is wanted:
@@ -34,15 +34,17 @@
 //   one more matrix instruction on the parameter words themselves (q's group
 //   sums as an fp16 head and tail), and O = sum_t (p_t s_t) c_t + p_t m_t.
 //
-// Rounded to fewer than 32 bits: p to the operand type (fp16 at 4 bits, where it is
-// then multiplied by its token's scale in fp16), q to fp16 at 4 bits after a
-// power of two per row (exact but for elements below 2^-24 of the largest).
+// Rounded to fewer than 32 bits: p to the operand type (fp16 times 2^12, see kLift;
+// bf16 as it is, with fp32's range), at 4 bits its product with the token's scale to fp16
+// (the scale relative to a power of two near the largest one, see `se`), and q to fp16 at
+// 4 bits after a power of two per row (exact but for elements below 2^-24 of the
+// largest).
 //
 // Measured on one B200 (replayed): 64 sequences of 5 to 8192 tokens, 32 / 8 heads of
-// 128, 16-bit 172 to 177 us (6.1 TB/s of the cache), 96 such at 4 bits 103 us
-// (4.9 TB/s); two of 100003 and 131072 tokens at 4 bits 60 us, of which 49 stream at
-// 6 TB/s and 11 are fixed: lengths, pages and the first copy follow one another
-// (5 us), and the last tile, the join of the warps and the second launch (6 us).
+// 128, 16-bit 175 us (6.1 TB/s of the cache), 96 such at 4 bits 108 us (4.7 TB/s);
+// two of 100003 and 131072 tokens at 4 bits 61 us, of which 48 stream at 6.2 TB/s (two
+// of 131072 67 us, of 262144 121) and 13 are fixed: lengths, pages and the first copy
+// follow one another, and the last tile, the join of the warps and the second launch.
 // A CTA holds 4 warps, an SM two CTAs: 12 or 16 warps an SM with 2 blocks a tile were
 // slower (69 and 76 against 64 us for the two long ones), as a tile's fixed steps
 // then count twice.
@@ -65,15 +67,16 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-// A maximum is left as it is while no score is more than 2^kSlack above it (the
-// probabilities then reach 4, and times a scale of at most 8734 stay in fp16).
+// A maximum is left as it is while no score is more than kSlack (in log2) above it: the
+// probabilities then reach 4.
 constexpr float kSlack = 2.f;
 // Probabilities are taken times 2^kLift where they become 16-bit fp16 operands: they
 // reach 2^14 and are normal numbers down to 2^-26 of the largest (unlifted, 2^-14: of
 // 70000 tokens 18 below one in score a fifth of their part of the output was lost).
 constexpr float kLift = 12.f;
-// From 2^kFar on (in log2) a maximum is off the fused product that it was rounded from by
-// half or more, and the probabilities would leave fp16: the row's scores are then divided
+// From 2^kFar on (in log2) a maximum is off the product that it was rounded from, and that
+// the fused subtraction uses, by up to 1 and more, and the probabilities would leave fp16:
+// the row's scores are then divided
 // by the power of two that brings the maximum below 2^kFar.  (Gaps shrink with them, those
 // below 20 2^-23 of the maximum to where they count: less than the sums of products are
 // off, (D + 8) 2^-22.)
@@ -95,9 +98,9 @@ constexpr int kCtas = 2;
 // The start and end of a segment (its q, the join of the warps) take a CTA about
 // as long as so many tiles, so the list has that many empty places behind each
 // segment's tiles and shares with many short segments hold fewer tiles.  96
-// sequences of 5 to 8192 tokens at 4 bits (tiles of 256): 134, 114, 105, 108 us
-// with 0, 1, 2, 4 places; 24 sequences of 5 query tokens (tiles of 128): 45, 41,
-// 37, 36 us; 64 sequences at 16 bits (tiles of 64): 180, 177, 175, 179 us.
+// sequences of 5 to 8192 tokens at 4 bits (tiles of 256): 137, 114, 108, 111 us
+// with 0, 1, 2, 4 places; 24 sequences of 5 query tokens (tiles of 128): 46, 41,
+// 37, 36 us; 64 sequences at 16 bits (tiles of 64): 174.4, 173.6, 173.1, 173.9 us.
 constexpr int cost_of(int D, int bits, int nt) {
   return bits == 4 ? 512 / (kWarps * blocks_of(D, bits, nt) * 16) : 2;
 }
@@ -456,7 +459,9 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   int col_q[NT][2];             // query token of a column's row; -1: none
   float o[KSTEPS][NT][4], om[NT][4], l[NT][2];
   // 4-bit: exponent field of the largest scale of V so far; scales enter the products
-  // times 2^(15 - se), below 2
+  // times 2^(15 - se), below 2, and O is kept in that unit.  (As they were, products of
+  // small values or of a long tail were subnormal or 0 in fp16, up to a fifth of the
+  // output.  96 sequences of 5 to 8192 tokens 110 -> 114 us.)
   uint32_t se = 0;
   float mf[NT][2];              // running maximum in the log2 domain
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
@@ -1138,9 +1143,9 @@ int launch_decode_any(DecodeParams& p, int nt, const CUtensorMap& tk, const CUte
 
 // Tiles (of the table's room) up to which segments are not split, so that no second
 // launch joins them.  Replayed, whole against split, us: 16-bit, 16 heads of 64,
-// 300 tokens (3 tiles) 5.6 / 7.0, 777 (7) 9.1 / 7.2, where the second launch costs
-// the host 2.5 us more, 2000 (16) 16.5 / 8.0; 4-bit, 8 heads of 128, 1000 tokens (4)
-// 11.1 / 11.3, of 16 sequences 11.9 / 14.8, 2000 (8) 16.4 / 11.5.
+// 300 tokens (3 tiles) 5.8 / 7.2, 777 (7) 9.5 / 7.6, where the second launch costs
+// the host 2.5 us more, 2000 (16) 17.9 / 8.4; 4-bit, 8 heads of 128, 1000 tokens (4)
+// 12.3 / 11.6, of 16 sequences 13.3 / 16.1, 2000 (8) 17.5 / 10.7.
 constexpr int whole_tiles(int bits) { return bits == 4 ? 4 : 7; }
 // Places are counted in 31 bits.
 constexpr long long kMaxPlaces = 1LL << 31;

@@ -208,7 +208,8 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
     Args:
         q: (B, S, H, D) of the cache's dtype, H % H_kv == 0 (query head h reads
             K/V head h // (H // H_kv)).  Any S; built for S * H / H_kv up to a
-            few tens of rows (the cache is read once per 16 of them).
+            few tens of rows (the cache is read once per 16 of them, 32 for
+            head_dim up to 64).
         lengths: (B,) int32 cached tokens of each sequence, the new ones included.
         causal: query i of sequence b sees tokens j <= starts[b] + i.
         starts: (B,) int32 position of each sequence's first query (default

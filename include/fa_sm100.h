@@ -234,7 +234,8 @@ int fa_sm100_kv_read(const fa_sm100_kv_cache* cache, const int* page_table, int 
  * (batch, nheads, seqlen) as in fa_sm100_fwd.  causal: query i sees tokens
  * j <= starts[b] + i (starts NULL: lengths[b] - seqlen).  A row that sees no token
  * gets out = 0, lse = +inf.  Built for a few query tokens: the cache is read once
- * per 16 rows (query tokens x query heads of a K/V head).
+ * per 16 rows (query tokens x query heads of a K/V head; 32 for head_dim up to 64).
+ * sm_scale is finite.
  * The workspace (caller-owned, 256-byte aligned, not initialised; bytes for the
  * current device) is used by this call alone. */
 size_t fa_sm100_decode_workspace_bytes(const fa_sm100_kv_cache* cache, int table_width, int batch,

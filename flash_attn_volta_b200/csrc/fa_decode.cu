@@ -76,10 +76,9 @@ constexpr float kSlack = 2.f;
 constexpr float kLift = 12.f;
 // From 2^kFar on (in log2) a maximum is off the product that it was rounded from, and that
 // the fused subtraction uses, by up to 1 and more, and the probabilities would leave fp16:
-// the row's scores are then divided
-// by the power of two that brings the maximum below 2^kFar.  (Gaps shrink with them, those
-// below 20 2^-23 of the maximum to where they count: less than the sums of products are
-// off, (D + 8) 2^-22.)
+// the row's scores are then divided by the power of two that brings the maximum below
+// 2^kFar.  (Gaps shrink with them, those below 20 2^-23 of the maximum to where they
+// count: less than the sums of products are off, (D + 8) 2^-22.)
 constexpr int kFar = 24;
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -463,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   // small values or of a long tail were subnormal or 0 in fp16, up to a fifth of the
   // output.  96 sequences of 5 to 8192 tokens 110 -> 114 us.)
   uint32_t se = 0;
+  bool cuts = false;            // some row's scores were divided
   float mf[NT][2];              // running maximum in the log2 domain
   int min_lim = 0, max_lim = 0, qp_first = 0, qp_last = 0, start = 0;
 
@@ -509,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     min_lim = limit_of(qp_first);
     max_lim = limit_of(qp_last);
     se = 0;
+    cuts = false;
     if (lane < ROWS) sh.cut[warp][lane] = 0;
     __syncwarp();
 #pragma unroll
@@ -734,19 +735,23 @@ __global__ void __launch_bounds__(kThreads, kCtas)
           }
         }
       static_assert(kFar == 24, "the bound above");
-      if (__any_sync(0xffffffffu, far)) {
+      if (cuts |= __any_sync(0xffffffffu, far)) {
+        // the power of two of each row, from its true maximum: it shrinks again where the
+        // maximum was far below 0 and is not any more
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int by = (int)(__float_as_uint(mf[n][i]) >> 23 & 255u) - 127 - (kFar - 1);
-            if (by > 0 && by <= 128 - kFar) {  // (not an infinity)
-              const float less = __uint_as_float((uint32_t)(127 - by) << 23);
-              f[n][i] *= less;
-              mf[n][i] *= less;
-              if (g == 0) sh.cut[warp][n * 8 + 2 * t + i] += by;
-            }
+            const int had = sh.cut[warp][n * 8 + 2 * t + i];
+            const int e = (int)(__float_as_uint(mf[n][i]) >> 23 & 255u) - 127;
+            const int by = e == 128 ? 0 : max(e + had - (kFar - 1), 0) - had;
+            const float less = __uint_as_float((uint32_t)(127 - by) << 23);
+            f[n][i] *= less;
+            mf[n][i] *= less;
+            __syncwarp();
+            if (g == 0) sh.cut[warp][n * 8 + 2 * t + i] = had + by;
           }
+        __syncwarp();
       }
     }
     float from[NT][2];

@@ -65,6 +65,24 @@ def test_scores_of_minus_infinity_weigh_nothing(n, D, dtype):
     assert not out[1].any() and bool((lse[1] == math.inf).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("low", [-2.0 ** 20, -2.0 ** 28, -2.0 ** 33, -1e30])
+@pytest.mark.parametrize("D,n", [(16, 512), (64, 500), (128, 512)])
+def test_scores_far_below_the_others_weigh_nothing(D, n, low):
+    """Keys that were masked by a large negative value, before and between ordinary ones."""
+    pool, k, v, size = _filled([n], 64, 1, D, BF16, 16, seed=3)
+    hidden = torch.zeros(n, dtype=torch.bool)
+    hidden[:300], hidden[400:411] = True, True
+    j = hidden.nonzero()[:, 0]
+    pool.cache.k_pages[pool.table.long()[0, j // 64].to(DEV), 0, (j % 64).to(DEV), 3] = low
+    q = torch.randn((1, 1, 2, D), generator=torch.Generator().manual_seed(8)).bfloat16()
+    q[..., 3] = 0.5
+    out, lse = flash_attn_decode(q.to(DEV), pool.cache, pool.table_dev, pool.lengths, return_softmax_lse=True)
+    check_status(DEV)
+    seen = ~hidden
+    _check_decode(q, out, lse, k[:, seen], v[:, seen], size[:, seen], [int(seen.sum())], None, True, 16)
+
+
 # ---------------------------------------------------------------- GPU: weights far below the largest
 def _far(n, D, gap, bits, low, high, seed, order="even"):
     """One sequence of n tokens, one head: the scores of tokens 0, 16, 32 and 48 (each warp has one)

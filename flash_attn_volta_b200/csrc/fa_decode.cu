@@ -972,7 +972,6 @@ __global__ void __launch_bounds__(kThreads, kCtas)
   }
   int next_id = look_up(pc, more_to_issue());  // read ahead of its use
   int stage = 0;
-  uint32_t phase = 0;
   bool fresh = true, first = false, stopped = false;
 #pragma unroll 1
   while (left > 0 || (p.whole && !fresh)) {
@@ -988,7 +987,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     const bool goes_on = left > places || (p.whole && !last);
     if (AHEAD && last && goes_on) load_q(next);
     // a wait may run out for some lanes and end for others: the warp goes one way
-    const bool here = __all_sync(0xffffffffu, mbar_wait(my_bars + stage * 8, phase, wait));
+    const bool here = __all_sync(0xffffffffu, mbar_wait(my_bars + stage * 8, odd >> stage & 1u, wait));
     if (here) {
       in_flight &= ~(1u << stage);
       const uint32_t ok = ok_bits >> stage * U & ALL;
@@ -1007,10 +1006,7 @@ __global__ void __launch_bounds__(kThreads, kCtas)
     fresh = last;
     left -= places;
     cur = next;
-    if (++stage == NS) {
-      stage = 0;
-      phase ^= 1;
-    }
+    if (++stage == NS) stage = 0;
   }
   // After a wait that ran out, copies may still be under way into this CTA's memory.
   for (int s = 0; s < NS; ++s)

@@ -216,7 +216,8 @@ def flash_attn_decode(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Te
             lengths - S); for a batch whose sequences have different counts of
             new tokens, pass what kv_cache_append got (rows behind a count are
             padding: what they give means nothing).
-        sm_scale, return_softmax_lse: as in flash_attn_forward.
+        sm_scale, return_softmax_lse: as in flash_attn_forward (a scale that is not
+            finite is refused).
 
     Returns:
         out (B, S, H, D), with return_softmax_lse also lse (B, H, S) fp32.  A row
